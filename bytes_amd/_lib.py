@@ -20,6 +20,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libbytes_amd.so")
 
 c_int, c_i64, c_f32, c_sz, c_vp = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+c_f64 = ctypes.c_double
 c_szp = ctypes.POINTER(ctypes.c_size_t)
 
 # name -> argtypes (restype is always c_int unless listed in _RESTYPES)
@@ -144,6 +145,36 @@ SIGNATURES: Dict[str, Tuple] = {
         c_vp, c_i64, c_int, c_vp, c_int, c_int, c_int, c_int,   # ridx, row stride, kc0, pos, Qc, local_w, S, kb
         c_i64, c_vp, c_i64, c_int, c_vp, c_i64, c_vp, c_vp),    # rows, next scores, indices, final indices, stream
     "bytes_select_recent": (c_vp, c_int, c_i64, c_int, c_vp, c_vp),
+    "bytes_paged_kv_append": (
+        c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,                  # k, v + strides (token, head)
+        c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,                  # q, q_out + strides (token, head)
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)
+        c_int, c_vp, c_vp,                                       # cache is fp8, kmin, kmax
+        c_vp, c_i64, c_vp, c_vp,                                 # block table, row stride, lengths, cu_seqlens
+        c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int,           # cos, sin + row strides, positions, rot, interleaved
+        c_f32, c_f32,                                            # k_scale, v_scale
+        c_int, c_int, c_int, c_int, c_int,                       # T, B, Hq, Hk, D
+        c_int, c_int, c_int, c_vp),                              # block size, blocks, max blocks, stream
+    "bytes_paged_decode_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
+    "bytes_paged_decode_attn": (
+        c_vp, c_i64, c_i64,                                      # q, strides (b, h)
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)
+        c_int, c_vp, c_i64, c_vp,                                # cache is fp8, block table, row stride, lengths
+        c_vp, c_i64, c_i64,                                      # out, strides (b, h)
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, Hq, Hk, D, block size, blocks, max blocks
+        c_f32, c_f32, c_vp, c_sz, c_vp),                         # scale, v_scale, workspace, bytes, stream
+    "bytes_paged_page_scores": (
+        c_vp, c_i64, c_i64, c_vp, c_vp,                          # q + strides, kmin, kmax
+        c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,                   # block table, row stride, lengths, bound + strides
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, Hq, Hk, D, block size, blocks, max blocks
+        c_int, c_f64, c_vp),                                     # local_w, scale, stream
+    "bytes_paged_pick_attn": (
+        c_vp, c_i64, c_i64,                                      # q, strides (b, h)
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)
+        c_int, c_vp, c_i64, c_i64, c_int,                        # cache is fp8, pages + strides (b, h), npick
+        c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,                   # block table, row stride, lengths, out + strides
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, Hq, Hk, D, block size, blocks, max blocks
+        c_f32, c_f32, c_vp, c_sz, c_vp),                         # scale, v_scale, workspace, bytes, stream
 }
 _RESTYPES = {"bytes_error_string": ctypes.c_char_p}
 

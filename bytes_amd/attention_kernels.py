@@ -137,3 +137,5 @@ from .sparse import (quantize_and_pack_score_keys, sparse_decode_scalar, sparse_
 from .pq import (decode_attn_dequant, decode_attn_pq_lut, decode_attn_pq_lut_asym,  # noqa: E402,F401
                  decode_attn_pq_lut_kv, paged_attn_pq_lut_asym, paged_attn_pq_lut_kv, sparse_decode_pq_lut,
                  sparse_score_pq_lut_asym)
+# Paged dense caches (beside the paged product-quantized operators above).
+from .paged import paged_decode_attn, paged_kv_append, paged_page_scores, paged_quest_decode  # noqa: E402,F401

@@ -471,6 +471,69 @@ int bytes_pq_decode_vectors(const void* idx, int heads, int64_t rows_per_head, i
 int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, const void* labels,
                            const void* reseed, void* cb_f16, void* cb_f32, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged dense KV caches: append with rotation, decode, page-sparse decode.
+ * The dense counterpart of the paged product-quantized entry point above (the
+ * reference has none).  A cache is k_paged, v_paged [num_blocks, Hk,
+ * block_size, D] bf16, or float8_e4m3fn (kv_fp8 = 1) whose values stand for
+ * value * k_scale (v_scale); strides *_sb, *_sh, *_ss per block, KV head and
+ * row.  Token p of sequence b is row p % block_size of block
+ * block_table[b * bt_sb + p / block_size] (int32, max_blocks columns);
+ * sequence b holds context_lens[b] tokens (int32), held to 0 .. max_blocks *
+ * block_size.  Block ids outside [0, num_blocks) name no block: nothing is
+ * written for their tokens, and they take no part.  Lengths, tables and
+ * cu_seqlens are device memory, read when the kernels run.  D in {64, 128};
+ * max_blocks * block_size < 2^31 - 1024.
+ *
+ * bytes_paged_kv_append: k, v [T, Hk, D] bf16 (strides *_st, *_sh), the new
+ *   tokens of B sequences: rows cu_seqlens[b] .. cu_seqlens[b + 1], or row b
+ *   where cu_seqlens is NULL (T = B).  They end at position context_lens[b] -
+ *   1.  The first rot dims (a multiple of 16) of keys and queries are rotated
+ *   with row p of cos, sin (fp32 rows of rot / 2, row strides cos_st, sin_st;
+ *   positions >= max_blocks * block_size rows): pairs (j, j + rot / 2), or
+ *   (2j, 2j + 1) if interleaved, in fp32, rounded once.  fp8 rows hold
+ *   k / k_scale and v / v_scale, held to +-448 (NaN stays NaN).  kmin, kmax
+ *   [num_blocks, Hk, D] bf16 (or NULL): min / max of each block's stored keys,
+ *   started anew where a token enters a block at its first row, else folded
+ *   into.  q [T, Hq, D] bf16 (or NULL with Hq = 0): rotated into q_out; rows
+ *   without a position get zeros.
+ * bytes_paged_decode_attn: out [B, Hq, D] bf16 (strides o_sb, o_sh) =
+ *   v_scale * softmax(scale * q . K^T) V over the tokens that take part, zeros
+ *   where none does; q [B, Hq, D] bf16.  (scale includes the cache's k_scale.)
+ *   Workspace: bytes_paged_decode_workspace_size, contents arbitrary.
+ * bytes_paged_page_scores: bound [B, Hq, max_blocks] fp32 (strides b_sb, b_sh)
+ *   = scale * sum_d q_d * (q_d >= 0 ? kmax_d : kmin_d) of block table entries,
+ *   summed in fp64 and rounded once; -inf where a block holds no token that
+ *   takes part, +inf where it reaches into the last local_w tokens.
+ * bytes_paged_pick_attn: bytes_paged_decode_attn over the tokens of the blocks
+ *   at places pages [B, Hq, npick] (int32, strides p_sb, p_sh, each place at
+ *   most once) of the table; places outside the sequence stand for nothing.
+ * ------------------------------------------------------------------------- */
+int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                          const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                          void* k_paged, int64_t kp_sb, int64_t kp_sh, int64_t kp_ss, void* v_paged, int64_t vp_sb,
+                          int64_t vp_sh, int64_t vp_ss, int kv_fp8, void* kmin, void* kmax, const void* block_table,
+                          int64_t bt_sb, const void* context_lens, const void* cu_seqlens, const void* cos,
+                          int64_t cos_st, const void* sin, int64_t sin_st, int positions, int rot, int interleaved,
+                          float k_scale, float v_scale, int T, int B, int Hq, int Hk, int D, int block_size,
+                          int num_blocks, int max_blocks, void* stream);
+int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int block_size, int max_blocks, size_t* bytes);
+int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
+                            int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
+                            const void* block_table, int64_t bt_sb, const void* context_lens, void* out, int64_t o_sb,
+                            int64_t o_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
+                            float scale, float v_scale, void* workspace, size_t workspace_bytes, void* stream);
+int bytes_paged_page_scores(const void* q, int64_t q_sb, int64_t q_sh, const void* kmin, const void* kmax,
+                            const void* block_table, int64_t bt_sb, const void* context_lens, void* bound, int64_t b_sb,
+                            int64_t b_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
+                            int local_w, double scale, void* stream);
+int bytes_paged_pick_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
+                          int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
+                          const void* pages, int64_t p_sb, int64_t p_sh, int npick, const void* block_table,
+                          int64_t bt_sb, const void* context_lens, void* out, int64_t o_sb, int64_t o_sh, int B, int Hq,
+                          int Hk, int D, int block_size, int num_blocks, int max_blocks, float scale, float v_scale,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
