@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -494,6 +495,54 @@ Tensor quest(const Tensor& q, const Tensor& k, const Tensor& v, long kb, double 
   return out;
 }
 
+// ---- paged dense caches ----
+
+struct Paged {
+  int64_t N, Hk, bs, D;
+  bool f8;
+  int64_t W;
+};
+// Caches, block table and lengths of B sequences; scales as the wrapper takes them.
+Paged paged(const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& cl, int64_t B, double ks, double vs) {
+  const bool f8 = k.scalar_type() == kF8;
+  need((f8 || k.scalar_type() == at::kBFloat16) && v.scalar_type() == k.scalar_type() && k.dim() == 4 &&
+       v.sizes() == k.sizes());
+  const Paged p{k.size(0), k.size(1), k.size(2), k.size(3), f8, bt.dim() == 2 ? bt.size(1) : 0};
+  need(p.N > 0 && p.N <= 0x7FFFFFFF && p.Hk > 0 && p.bs > 0 && head_dim(p.D));
+  rows(k);
+  rows(v);
+  need(std::isfinite(ks) && std::isfinite(vs) && ks > 0 && vs > 0 && (f8 || (ks == 1.0 && vs == 1.0)));
+  need(bt.dim() == 2 && bt.size(0) == B && bt.scalar_type() == at::kInt && (bt.stride(1) == 1 || p.W == 1) && p.W > 0);
+  need(shape(cl, {B}) && cl.scalar_type() == at::kInt && cl.is_contiguous());
+  need(p.bs <= 0x7FFFFFFF - 1024 && p.W * p.bs <= 0x7FFFFFFF - 1024);
+  same_device(k, {&v, &bt, &cl});
+  return p;
+}
+void paged_query(const Tensor& q, const Tensor& k) {     // q [B, Hq, 1, D]
+  need(q.dim() == 4 && q.scalar_type() == at::kBFloat16 && q.size(0) > 0 && q.size(1) > 0 && q.size(2) == 1 &&
+       k.dim() == 4 && q.size(3) == k.size(3) && k.size(1) > 0 && q.size(1) % k.size(1) == 0);
+  same_device(k, {&q});
+  rows(q);
+}
+
+Tensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& cl, double scale,
+                    double ks, double vs) {
+  paged_query(q, k);
+  const int64_t B = q.size(0), Hq = q.size(1);
+  const Paged p = paged(k, v, bt, cl, B, ks, vs);
+  c10::DeviceGuard guard(q.device());
+  size_t n = 0;
+  need(bytes_paged_decode_workspace_size(B, Hq, p.Hk, p.D, p.bs, p.W, &n) == 0);
+  const Tensor w = empty(q, {(int64_t)n}, at::kByte);    // the call's own: calls on other streams share nothing
+  Tensor out = empty(q, {B, Hq, 1, p.D}, at::kBFloat16);
+  void* st = stream_of(q);
+  launch("bytes_paged_decode_attn", bytes_paged_decode_attn, data(q), q.stride(0), q.stride(1), data(k), k.stride(0),
+         k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), p.f8, data(bt), bt.stride(0), data(cl),
+         out.mutable_data_ptr(), out.stride(0), out.stride(1), B, Hq, p.Hk, p.D, p.bs, p.N, p.W, (float)(scale * ks),
+         (float)vs, w.mutable_data_ptr(), n, st);
+  return out;
+}
+
 // ---- bindings ----
 
 template <class F>
@@ -552,6 +601,9 @@ BIND(token_topk, 9, token_topk(tensor(a[0]), tensor(a[1]), tensor(a[2]), integer
 BIND(quest, 10, WRAP(quest(tensor(a[0]), tensor(a[1]), tensor(a[2]), integer(a[3]), number(a[4]), integer(a[5]),
                            tensor(a[6]), tensor(a[7]), integer(a[8]), integer(a[9]))))
 
+BIND(paged_decode, 8, WRAP(paged_decode(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), number(a[5]),
+                                        number(a[6]), number(a[7]))))
+
 PyObject* py_set_workspaces(PyObject*, PyObject* d) {
   if (!PyDict_Check(d)) {
     PyErr_SetString(PyExc_TypeError, "expected the workspace table");
@@ -566,6 +618,7 @@ PyObject* py_set_workspaces(PyObject*, PyObject* d) {
 PyMethodDef methods[] = {METHOD(dense),     METHOD(kivi),   METHOD(kivi_pack), METHOD(pq_fused),
                          METHOD(pq_asym),   METHOD(pq_paged), METHOD(pq_encode), METHOD(score_into), METHOD(topk),
                          METHOD(gather),    METHOD(sparse_decode), METHOD(token_topk), METHOD(quest),
+                         METHOD(paged_decode),
                          {"set_workspaces", py_set_workspaces, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the operators.", -1, methods};

@@ -39,4 +39,183 @@ inline int paged_check(int block_size, int num_blocks, int width) {
   return 0;
 }
 
+// Whether 16-row halves of a tile can be addressed from one scalar base each:
+// tiles start on multiples of 32 tokens, so with block sizes that are multiples
+// of 16 a half never crosses a block, and 32-bit lane offsets hold its rows.
+inline bool paged_halves(const PagedKv& c) {
+  return c.bs % 16 == 0 && c.k_ss >= 0 && c.k_ss <= (1 << 24) && c.v_ss >= 0 && c.v_ss <= (1 << 24);
+}
+
+// ---- one wave's attention over the tokens of some slots ----
+// A slot range is walked in 32-slot tiles through the dense tile (dense_tile.h).
+// What a slot stands for is the caller's: find(s) gives (place in the table row,
+// row in the block, whether it is a token).
+
+// One tile's table entries: lane l's slot is s0 + l % 32.
+struct PagedIds {
+  int id, off;
+  bool ok;
+};
+
+// The tile's rows in flight: K and V of 32 tokens in registers.  HALVES: two
+// scalar bases per tile (see paged_halves), else every lane's row number comes
+// from the lane that holds it.  A tile past the end (live false) reads the first
+// bytes of the cache, the same on every lane, so that every iteration issues the
+// same instructions.
+template <int D, bool FP8, bool HALVES>
+struct PagedRows {
+  using Elem = typename std::conditional<FP8, uint8_t, uint16_t>::type;
+  using Regs = typename std::conditional<FP8, DenseRegs8<D>, DenseRegs<D>>::type;
+  static constexpr int EPC = 16 / (int)sizeof(Elem);      // elements per 16-byte chunk
+  static constexpr int CPR = D / EPC;                     // chunks per row
+  static constexpr int CPL = kTile * CPR / 64;            // chunks per lane per tile
+  static constexpr int RPI = 64 / CPR;                    // rows per instruction
+  static_assert(RPI <= 16, "an instruction's rows lie in one half");
+
+  const Elem *kb, *vb;               // the KV head's first row
+  int64_t k_sb, k_ss, v_sb, v_ss;
+  int lane, r0, col;                 // this lane's row within an instruction's rows, and its first dim
+  Regs r;
+
+  __device__ __forceinline__ PagedRows(const PagedKv& c, int hk, int lane_)
+      : kb(static_cast<const Elem*>(c.k) + hk * c.k_sh), vb(static_cast<const Elem*>(c.v) + hk * c.v_sh), k_sb(c.k_sb),
+        k_ss(c.k_ss), v_sb(c.v_sb), v_ss(c.v_ss), lane(lane_), r0(lane_ / CPR), col(lane_ % CPR * EPC) {}
+
+  __device__ __forceinline__ void issue(const PagedIds& t, bool live) {
+    if constexpr (HALVES) {
+      const uint32_t ko = live ? (uint32_t)(r0 * (int)k_ss + col) : 0u, vo = live ? (uint32_t)(r0 * (int)v_ss + col) : 0u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int id = live ? __builtin_amdgcn_readlane(t.id, 16 * h) : 0;
+        const int off = live ? __builtin_amdgcn_readlane(t.off, 16 * h) : 0;
+        const Elem* kp = kb + (int64_t)id * k_sb + (int64_t)off * k_ss;
+        const Elem* vp = vb + (int64_t)id * v_sb + (int64_t)off * v_ss;
+#pragma unroll
+        for (int i = h * CPL / 2; i < (h + 1) * CPL / 2; ++i) {
+          const int row = live ? i * RPI - 16 * h : 0;
+          r.k[i] = ld16_nt(kp + (int64_t)row * k_ss + ko);
+          r.v[i] = ld16_nt(vp + (int64_t)row * v_ss + vo);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CPL; ++i) {
+        const int src = r0 + i * RPI;
+        const int id = live ? __shfl(t.id, src, 64) : 0, off = live ? __shfl(t.off, src, 64) : 0;
+        const int c = live ? col : 0;
+        r.k[i] = ld16_nt(kb + (int64_t)id * k_sb + (int64_t)off * k_ss + c);
+        r.v[i] = ld16_nt(vb + (int64_t)id * v_sb + (int64_t)off * v_ss + c);
+      }
+    }
+  }
+
+  // Into the wave's LDS tile; values of slots that are no token become 0 (their
+  // weight is 0, and 0 times what an unused row holds need not be).
+  __device__ __forceinline__ void stage(uint32_t vmask, char* kst, char* vst) {
+    if (vmask != 0xFFFFFFFFu) {
+#pragma unroll
+      for (int i = 0; i < CPL; ++i)
+        if (!((vmask >> (r0 + i * RPI)) & 1u)) r.v[i] = u32x4{0, 0, 0, 0};
+    }
+    if constexpr (FP8) dense_stage_fp8<D>(lane, r, kst, vst);
+    else dense_stage<D>(lane, r, kst, vst);
+  }
+};
+
+// Slots [s, s_end) in steps of `step` (s a multiple of 32 from the first slot):
+// online softmax over them into m_run, l_run, acc.
+template <int D, bool FP8, bool HALVES, class FIND>
+__device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t* table, int hk, int s, int s_end,
+                                                int step, int lane, float scale_log2, const bf16x8 (&qb)[D / 32],
+                                                char* wbuf, const FIND& find, float& m_run, float& l_run,
+                                                f32x4 (&acc)[D / 16]) {
+  if (s >= s_end) return;
+  char* kst = wbuf;
+  char* vst = wbuf + DenseCfg<D>::VT;
+  PagedRows<D, FP8, HALVES> rows(c, hk, lane);
+  // entries of the tile at s0: loaded well before they are used
+  auto fetch = [&](int s0) {
+    PagedIds t;
+    int place;
+    const int sl = s0 + (lane & 31);
+    find(min(sl, s_end - 1), place, t.off, t.ok);
+    t.ok = t.ok && sl < s_end;
+    t.id = table[place];
+    return t;
+  };
+  auto settle = [&](PagedIds& t) {   // ids that name a block; other slots read block 0
+    const bool in = t.id >= 0 && t.id < c.nblocks;
+    t.ok = t.ok && in;
+    t.id = in ? t.id : 0;
+  };
+  PagedIds now = fetch(s), next = fetch(s + step);
+  settle(now);
+  rows.issue(now, true);
+  for (; s < s_end; s += step) {
+    const uint32_t vmask = (uint32_t)__ballot(now.ok);
+    wave_lds_sync();
+    rows.stage(vmask, kst, vst);
+    settle(next);
+    now = next;
+    next = fetch(s + 2 * step);
+    rows.issue(now, s + step < s_end);
+    wave_lds_sync();
+    dense_compute<D>(vmask, scale_log2, lane, qb, kst, vst, m_run, l_run, acc);
+  }
+}
+
+// Merge of the workgroup's waves through LDS, in wave order: put(h, d4, A, M, L)
+// with four consecutive dims 4 * d4 .. of head h < nh, the maximum (log2 domain)
+// and the denominator.  All threads of the workgroup call this; smem is free
+// again when it returns.
+template <int D, class PUT>
+__device__ __forceinline__ void paged_merge_waves(float m_run, float l_run, f32x4 (&acc)[D / 16], float* smem, int nh,
+                                                  const PUT& put) {
+  constexpr int NW = kDenseWaves, P = acc_pitch<D>(), D4 = D / 4;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, lg = lane >> 4;
+  l_run = col_sum4(l_run);
+  float* wm = smem;
+  float* wl = wm + NW * 16;
+  float* wacc = wl + NW * 16;
+  __syncthreads();
+  if (lg == 0) {
+    wm[w * 16 + l16] = m_run;
+    wl[w * 16 + l16] = l_run;
+  }
+  f32x4* row = reinterpret_cast<f32x4*>(wacc + (w * 16 + l16) * P);
+  if (l16 < nh) {
+#pragma unroll
+    for (int db = 0; db < D / 16; ++db) row[4 * db + lg] = acc[db];
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < nh * D4; e += NW * 64) {
+    const int h = e / D4, d4 = e - h * D4;
+    float M = kNegInf;
+#pragma unroll
+    for (int u = 0; u < NW; ++u) M = fmaxf(M, wm[u * 16 + h]);
+    const float Ms = (M == kNegInf) ? 0.f : M;
+    float L = 0.f;
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < NW; ++u) {
+      const float f = fast_exp2(wm[u * 16 + h] - Ms);
+      L += f * wl[u * 16 + h];
+      A += f * reinterpret_cast<const f32x4*>(wacc + (u * 16 + h) * P)[d4];
+    }
+    put(h, d4, A, M, L);
+  }
+  __syncthreads();
+}
+
+// Four consecutive results; a row with nothing to attend to is 0.
+__device__ __forceinline__ void paged_store(uint16_t* out, const f32x4& A, float L, float v_scale) {
+  const float il = L == 0.f ? 0.f : v_scale / L;
+  u32x2 r;
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    r[j] = (uint32_t)f32_to_bf16_bits(L == 0.f ? 0.f : A[2 * j] * il) |
+           ((uint32_t)f32_to_bf16_bits(L == 0.f ? 0.f : A[2 * j + 1] * il) << 16);
+  *reinterpret_cast<u32x2*>(out) = r;
+}
+
 }  // namespace bytes_amd

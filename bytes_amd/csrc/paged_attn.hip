@@ -3,15 +3,25 @@
 //   out[b, h] = v_scale * softmax_p(scale * q[b, h] . k[b, h / G, p]) v[b, h / G, p]
 //
 // over the tokens p of sequence b that take part (paged.h); a row none of whose
-// tokens does gets zeros.  Scores, softmax statistics and sums are fp32 (K, V
-// and Q products on MFMA are exact in fp32; the weights go to bf16 for the
-// value product).
+// tokens does gets zeros.  Scores, softmax statistics and sums are fp32 (products
+// of bf16 values are exact there).
 //
-// A workgroup serves up to 16 query heads of one KV head; its waves take
-// 32-token tiles in turn through the dense decode's tile (dense_tile.h).
+// Split: the lengths are known on the device only, and may differ by any factor.
+// A unit is up to 16 query heads of one KV head of one sequence; its tokens are
+// cut into granules of 128 (one 32-token tile for each of a workgroup's four
+// waves).  All granules of all units, in the order (sequence, KV head, head
+// block, token), are dealt to the fixed grid in equal runs: every workgroup sums
+// the granules of the batch (one load of lens per 64 sequences and a wave prefix
+// sum) and finds its run.  A run covers parts of units; a part that is a whole
+// unit is finished in place, others (at most two per workgroup: its first and its
+// last) leave (max, sum, values) in fp32 for the second launch, which joins each
+// unit's parts in token order.  So the work per workgroup differs by at most one
+// granule whatever the lengths, and the result does not depend on timing.
 #include "paged.h"
 
 namespace bytes_amd {
+
+constexpr int kGranule = kDenseWaves * kTile;      // tokens
 
 struct PagedDecodeArgs {
   PagedKv c;
@@ -19,89 +29,166 @@ struct PagedDecodeArgs {
   int64_t q_sb, q_sh;
   uint16_t* out;
   int64_t o_sb, o_sh;
-  int Hk, HB, G;
+  float* part_acc;                   // [workgroup][2][16][D]
+  float* part_ml;                    // [workgroup][2][16][2]
+  int B, Hk, HB, G, U;               // U = Hk * HB units per sequence
+  int nwg;
+  FastDiv dnwg, dhb;
   float scale_log2, v_scale;
 };
 
-template <int D, bool FP8>
+// Granules of a sequence of n tokens: an empty one has one too, whose output is written like any other.
+__device__ __forceinline__ int granules(int n) { return max(1, (n + kGranule - 1) / kGranule); }
+
+// The batch's granules: lane l sums those of sequences l * per .. + per - 1.
+struct BatchGranules {
+  uint32_t mine, incl;
+  int per, total;                    // sequences per lane; granules of the batch, all units
+
+  __device__ __forceinline__ BatchGranules(const PagedDecodeArgs& a, int lane) {
+    per = (a.B + 63) / 64;
+    mine = 0u;
+    for (int i = 0; i < per; ++i) {
+      const int b = lane * per + i;
+      if (b < a.B) mine += (uint32_t)granules(paged_len(a.c, b));
+    }
+    incl = wave_prefix_sum(mine);
+    total = __builtin_amdgcn_readlane((int)incl, 63) * a.U;
+  }
+  // The sequence that granule g lies in, its length, and its first granule.
+  __device__ __forceinline__ void find(const PagedDecodeArgs& a, int g, int& b, int& len, int& first) const {
+    const int l = __ffsll((unsigned long long)__ballot((int)incl * a.U > g)) - 1;
+    first = __builtin_amdgcn_readlane((int)(incl - mine), l) * a.U;
+    b = l * per;
+    for (;; ++b) {
+      len = __builtin_amdgcn_readfirstlane(paged_len(a.c, b));
+      const int n = granules(len) * a.U;
+      if (g < first + n || b == a.B - 1) return;
+      first += n;
+    }
+  }
+  // Runs: workgroup w has granules [start(w), start(w + 1)).
+  __device__ __forceinline__ int start(const PagedDecodeArgs& a, int w) const {
+    const int q = fast_div(total, a.dnwg), r = total - q * a.nwg;
+    return w * q + min(w, r);
+  }
+  __device__ __forceinline__ int owner(const PagedDecodeArgs& a, int g) const {
+    const int q = fast_div(total, a.dnwg), r = total - q * a.nwg, big = r * (q + 1);
+    return g < big ? g / (q + 1) : r + (g - big) / q;
+  }
+};
+
+template <int D, bool FP8, bool HALVES>
 __global__ __launch_bounds__(kDenseWaves * 64, 2) void paged_decode_kernel(PagedDecodeArgs a) {
   using C = DenseCfg<D>;
   __shared__ __attribute__((aligned(16))) char smem[C::kSmem];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, lg = lane >> 4;
-  const int hb = blockIdx.x % a.HB, hk = blockIdx.x / a.HB % a.Hk, b = blockIdx.x / (a.HB * a.Hk);
-  const int hq0 = hk * a.G + hb * 16, nh = min(16, a.G - hb * 16);
-  bf16x8 qb[C::KK];
-  load_q_bf16<D>(a.q + (int64_t)b * a.q_sb + (int64_t)hq0 * a.q_sh, a.q_sh, nh, lane, qb);
-  const int len = paged_len(a.c, b);
-  const int32_t* table = a.c.table + (int64_t)b * a.c.bt_sb;
-  char* kst = smem + w * C::WAVE;
-  char* vst = kst + C::VT;
-  float m_run = kNegInf, l_run = 0.f;
-  f32x4 acc[C::DB];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const BatchGranules all(a, lane);
+  const int g0 = all.start(a, blockIdx.x), g1 = all.start(a, blockIdx.x + 1);
+  if (g0 >= g1) return;
+  int b, len, first;
+  all.find(a, g0, b, len, first);
+  int n = granules(len);                           // of one unit of the sequence
+  int u = (g0 - first) / n, t = g0 - first - u * n;
+  for (int g = g0;;) {
+    const int m = min(n - t, g1 - g);              // granules of this part
+    const int hk = fast_div(u, a.dhb), hb = u - hk * a.HB;
+    const int hq0 = hk * a.G + hb * 16, nh = min(16, a.G - hb * 16);
+    bf16x8 qb[C::KK];
+    load_q_bf16<D>(a.q + (int64_t)b * a.q_sb + (int64_t)hq0 * a.q_sh, a.q_sh, nh, lane, qb);
+    float m_run = kNegInf, l_run = 0.f;
+    f32x4 acc[C::DB];
 #pragma unroll
-  for (int db = 0; db < C::DB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
-  using Regs = typename std::conditional<FP8, DenseRegs8<D>, DenseRegs<D>>::type;
-  using Elem = typename std::conditional<FP8, uint8_t, uint16_t>::type;
-  constexpr int CPR = FP8 ? D / 16 : D / 8, CPL = kTile * CPR / 64, EPC = FP8 ? 16 : 8;
-  const Elem* kb = static_cast<const Elem*>(a.c.k) + hk * a.c.k_sh;
-  const Elem* vb = static_cast<const Elem*>(a.c.v) + hk * a.c.v_sh;
-  // row of token j, clamped into the sequence; ok: the token takes part
-  auto row = [&](int j, int& id, int& off, bool& ok) {
-    const int jj = min(j, len - 1), blk = fast_div(jj, a.c.dbs);
-    id = table[blk];
-    off = jj - blk * a.c.bs;
-    ok = j < len && id >= 0 && id < a.c.nblocks;
-    id = ok ? id : 0;
-  };
-  for (int t = w * kTile; t < len; t += kDenseWaves * kTile) {
-    int id, off;
-    bool ok;
-    row(t + (lane & 31), id, off, ok);
-    const uint32_t vmask = (uint32_t)__ballot(ok);
-    Regs r;
-#pragma unroll
-    for (int i = 0; i < CPL; ++i) {
-      const int pl = lane + 64 * i, rr = pl / CPR, col = (pl - rr * CPR) * EPC;
-      row(t + rr, id, off, ok);
-      r.k[i] = ld16(kb + id * a.c.k_sb + off * a.c.k_ss + col);
-      r.v[i] = ld16_live(vb + id * a.c.v_sb + off * a.c.v_ss + col, ok);
+    for (int db = 0; db < C::DB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto find = [&](int p, int& place, int& off, bool& ok) {
+      place = fast_div(p, a.c.dbs);
+      off = p - place * a.c.bs;
+      ok = true;
+    };
+    paged_wave_loop<D, FP8, HALVES>(a.c, a.c.table + (int64_t)b * a.c.bt_sb, hk, t * kGranule + w * kTile,
+                                    min(len, (t + m) * kGranule), kGranule, lane, a.scale_log2, qb,
+                                    smem + w * C::WAVE, find, m_run, l_run, acc);
+    const bool whole = m == n;
+    uint16_t* out = a.out + (int64_t)b * a.o_sb + (int64_t)hq0 * a.o_sh;
+    const size_t slot = ((size_t)blockIdx.x * 2 + (g == g0 ? 0 : 1)) * 16;
+    paged_merge_waves<D>(m_run, l_run, acc, reinterpret_cast<float*>(smem), nh,
+                         [&](int h, int d4, const f32x4& A, float M, float L) {
+                           if (whole) {
+                             paged_store(out + (int64_t)h * a.o_sh + 4 * d4, A, L, a.v_scale);
+                           } else {
+                             reinterpret_cast<f32x4*>(a.part_acc + (slot + h) * D)[d4] = A;
+                             if (d4 == 0) reinterpret_cast<float2*>(a.part_ml)[slot + h] = make_float2(M, L);
+                           }
+                         });
+    g += m;
+    if (g >= g1) return;
+    t = 0;
+    if (++u == a.U) {
+      u = 0;
+      ++b;
+      len = __builtin_amdgcn_readfirstlane(paged_len(a.c, b));
+      n = granules(len);
     }
-    wave_lds_sync();
-    if constexpr (FP8) dense_stage_fp8<D>(lane, r, kst, vst);
-    else dense_stage<D>(lane, r, kst, vst);
-    wave_lds_sync();
-    dense_compute<D>(vmask, a.scale_log2, lane, qb, kst, vst, m_run, l_run, acc);
-  }
-  // merge of the waves, in wave order
-  constexpr int P = acc_pitch<D>();
-  l_run = col_sum4(l_run);
-  float* wm = reinterpret_cast<float*>(smem);
-  float* wl = wm + kDenseWaves * 16;
-  float* wacc = wl + kDenseWaves * 16;
-  __syncthreads();
-  if (lg == 0) {
-    wm[w * 16 + l16] = m_run;
-    wl[w * 16 + l16] = l_run;
-  }
-  f32x4* arow = reinterpret_cast<f32x4*>(wacc + (w * 16 + l16) * P);
-#pragma unroll
-  for (int db = 0; db < C::DB; ++db) arow[4 * db + lg] = acc[db];
-  __syncthreads();
-  for (int e = threadIdx.x; e < nh * D; e += kDenseWaves * 64) {
-    const int h = e / D, d = e - h * D;
-    float M = kNegInf, L = 0.f, A = 0.f;
-#pragma unroll
-    for (int u = 0; u < kDenseWaves; ++u) M = fmaxf(M, wm[u * 16 + h]);
-    const float Ms = M == kNegInf ? 0.f : M;
-#pragma unroll
-    for (int u = 0; u < kDenseWaves; ++u) {
-      const float f = fast_exp2(wm[u * 16 + h] - Ms);
-      L += f * wl[u * 16 + h];
-      A += f * wacc[(u * 16 + h) * P + d];
-    }
-    a.out[(int64_t)b * a.o_sb + (int64_t)(hq0 + h) * a.o_sh + d] = f32_to_bf16_bits(L == 0.f ? 0.f : A / L * a.v_scale);
   }
 }
+
+// Joins the parts of each unit that more than one workgroup had: one wave per
+// (sequence, query head, 64 dims), four parts at a time (16 lanes hold a part's
+// dims), parts in token order within each of the four lane groups, the groups
+// folded by fixed row swaps.
+template <int D>
+__global__ __launch_bounds__(64) void paged_join_kernel(PagedDecodeArgs a) {
+  constexpr int NSL = D / 64;
+  const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
+  const int slice = blockIdx.x % NSL, h = blockIdx.x / NSL, b = blockIdx.y;     // h: query head
+  const BatchGranules all(a, lane);
+  const int hk = h / a.G, hb = (h - hk * a.G) / 16, hl = h - hk * a.G - hb * 16;
+  // granules of the sequences before b
+  uint32_t before = 0u;
+  {
+    const int l = b / all.per;
+    before = (uint32_t)__builtin_amdgcn_readlane((int)(all.incl - all.mine), l);
+    for (int i = l * all.per; i < b; ++i) before += (uint32_t)granules(paged_len(a.c, i));
+  }
+  const int n = granules(__builtin_amdgcn_readfirstlane(paged_len(a.c, b)));
+  const int s = (int)before * a.U + (hk * a.HB + hb) * n;
+  const int w0 = all.owner(a, s), w1 = all.owner(a, s + n - 1);
+  if (w0 == w1) return;                            // finished in place
+  const int parts = w1 - w0 + 1;
+  const int slot0 = all.start(a, w0) == s ? 0 : 1;
+  auto slot = [&](int i) { return ((size_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * 16 + hl; };
+  float M = kNegInf;
+  for (int i = lane; i < parts; i += 64) M = fmaxf(M, a.part_ml[2 * slot(i)]);
+  M = wave_max_f32(M);
+  if (M == kNegInf) M = 0.f;
+  float L = 0.f;
+  f32x4 A = {0.f, 0.f, 0.f, 0.f};
+  for (int i = grp; i < parts; i += 4) {
+    const size_t r = slot(i);
+    const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[r];
+    const float f = fast_exp2(ml.x - M);
+    L += f * ml.y;
+    A += f * reinterpret_cast<const f32x4*>(a.part_acc + r * D)[slice * 16 + item];
+  }
+  L = col_sum4(L);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) A[j] = col_sum4(A[j]);
+  if (grp == 0) paged_store(a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
+}
+
+// Workgroups of the decode grid: one per CU, at most the batch's granules.
+static int decode_grid(int64_t granules_max) {
+  const int64_t n = device_cu_count();
+  return (int)(granules_max < n ? granules_max : n);
+}
+
+static int64_t decode_granules(int B, int Hq, int Hk, int bs, int width) {
+  const int G = Hq / Hk, HB = (G + 15) / 16;
+  const int64_t per = ((int64_t)width * bs + kGranule - 1) / kGranule;
+  return (int64_t)B * Hk * HB * (per < 1 ? 1 : per);
+}
+
+static size_t decode_workspace(int nwg, int D) { return (size_t)nwg * 2 * 16 * (D + 2) * 4; }
 
 }  // namespace bytes_amd
 
@@ -113,7 +200,7 @@ int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int block_si
   if (!bytes || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128)) return (int)hipErrorInvalidValue;
   const int rc = paged_check(block_size, 1, max_blocks);
   if (rc) return rc;
-  *bytes = 0;
+  *bytes = decode_workspace(decode_grid(decode_granules(B, Hq, Hk, block_size, max_blocks)), D);
   return 0;
 }
 
@@ -122,11 +209,13 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
                             const void* block_table, int64_t bt_sb, const void* context_lens, void* out, int64_t o_sb,
                             int64_t o_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
                             float scale, float v_scale, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!q || !k_paged || !v_paged || !block_table || !context_lens || !out || B <= 0 || Hk <= 0 || Hq <= 0 ||
-      Hq % Hk != 0 || (D != 64 && D != 128))
+  if (!q || !k_paged || !v_paged || !block_table || !context_lens || !out || !workspace || B <= 0 || Hk <= 0 ||
+      Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128) || max_blocks <= 0)
     return (int)hipErrorInvalidValue;
   int rc = paged_check(block_size, num_blocks, max_blocks);
   if (rc) return rc;
+  const int64_t most = decode_granules(B, Hq, Hk, block_size, max_blocks);
+  if (most > 0x7FFFFFFF || B > 65535) return (int)hipErrorInvalidConfiguration;
   PagedDecodeArgs a;
   a.c.k = k_paged, a.c.k_sb = k_sb, a.c.k_sh = k_sh, a.c.k_ss = k_ss;
   a.c.v = v_paged, a.c.v_sb = v_sb, a.c.v_sh = v_sh, a.c.v_ss = v_ss;
@@ -136,21 +225,34 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
   a.c.dbs = make_fastdiv((uint32_t)block_size);
   a.q = static_cast<const uint16_t*>(q), a.q_sb = q_sb, a.q_sh = q_sh;
   a.out = static_cast<uint16_t*>(out), a.o_sb = o_sb, a.o_sh = o_sh;
-  a.Hk = Hk, a.G = Hq / Hk, a.HB = (a.G + 15) / 16;
+  a.B = B, a.Hk = Hk, a.G = Hq / Hk, a.HB = (a.G + 15) / 16, a.U = Hk * a.HB;
+  a.nwg = decode_grid(most);
+  a.dnwg = make_fastdiv((uint32_t)a.nwg), a.dhb = make_fastdiv((uint32_t)a.HB);
   a.scale_log2 = scale * kLog2e, a.v_scale = v_scale;
-  const int64_t units = (int64_t)B * Hk * a.HB;
-  if (units > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)units), block(kDenseWaves * 64);
+  if (workspace_bytes < decode_workspace(a.nwg, D)) return (int)hipErrorInvalidValue;
+  a.part_ml = static_cast<float*>(workspace);
+  a.part_acc = a.part_ml + (size_t)a.nwg * 2 * 16 * 2;
+  const bool halves = paged_halves(a.c);
+  const dim3 grid((unsigned)a.nwg), block(kDenseWaves * 64);
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define PD(DD, F8) hipLaunchKernelGGL((paged_decode_kernel<DD, F8>), grid, block, 0, st, a)
+#define PD(DD, F8, H) hipLaunchKernelGGL((paged_decode_kernel<DD, F8, H>), grid, block, 0, st, a)
+#define PD_H(DD, F8)       \
+  if (halves) PD(DD, F8, true); \
+  else PD(DD, F8, false)
   if (D == 128) {
-    if (kv_fp8) PD(128, true);
-    else PD(128, false);
+    if (kv_fp8) { PD_H(128, true); }
+    else { PD_H(128, false); }
   } else {
-    if (kv_fp8) PD(64, true);
-    else PD(64, false);
+    if (kv_fp8) { PD_H(64, true); }
+    else { PD_H(64, false); }
   }
+#undef PD_H
 #undef PD
+  rc = (int)hipGetLastError();
+  if (rc || (int64_t)max_blocks * block_size <= kGranule) return rc;        // no unit has two granules
+  const dim3 jgrid((unsigned)(Hq * (D / 64)), (unsigned)B);
+  if (D == 128) hipLaunchKernelGGL(paged_join_kernel<128>, jgrid, dim3(64), 0, st, a);
+  else hipLaunchKernelGGL(paged_join_kernel<64>, jgrid, dim3(64), 0, st, a);
   return (int)hipGetLastError();
 }
 

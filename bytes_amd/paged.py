@@ -27,7 +27,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _checks as C
-from ._lib import call, ptr, size_query, stream_of
+from ._lib import call, native, ptr, size_query, stream_of
 from .sparse import topk_indices
 
 _F8 = torch.float8_e4m3fn
@@ -206,6 +206,9 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     1/sqrt(D) for standard attention).  For fp8 caches the rows stand for
     k * k_scale and v * v_scale.  fp32 scores, softmax and sums.  Returns
     [B,H_q,1,D] bf16."""
+    out = native().paged_decode(q, k_paged, v_paged, block_table, context_lens, scale, k_scale, v_scale)
+    if out is not None:
+        return out
     C.cuda_tensors(q, k_paged, v_paged, block_table, context_lens)
     N, Hk, bs, D, fp8 = _cache(k_paged, v_paged, k_scale, v_scale)
     qs, B, Hq = _query(q, Hk, D)
