@@ -33,7 +33,7 @@ struct PagedDecodeArgs {
   float* part_ml;                    // [workgroup][2][16][2]
   int B, Hk, HB, G, U;               // U = Hk * HB units per sequence
   int nwg;
-  FastDiv dnwg, dhb;
+  FastDiv dnwg, dhb, dG;
   float scale_log2, v_scale;
 };
 
@@ -44,24 +44,37 @@ __device__ __forceinline__ int granules(int n) { return max(1, (n + kGranule - 1
 struct BatchGranules {
   uint32_t mine, incl;
   int per, total;                    // sequences per lane; granules of the batch, all units
+  int len0;                          // length of the lane's last sequence: its only one where per == 1
 
   __device__ __forceinline__ BatchGranules(const PagedDecodeArgs& a, int lane) {
     per = (a.B + 63) / 64;
     mine = 0u;
+    len0 = 0;
     for (int i = 0; i < per; ++i) {
       const int b = lane * per + i;
-      if (b < a.B) mine += (uint32_t)granules(paged_len(a.c, b));
+      len0 = paged_len(a.c, min(b, a.B - 1));
+      mine += b < a.B ? (uint32_t)granules(len0) : 0u;
     }
     incl = wave_prefix_sum(mine);
     total = __builtin_amdgcn_readlane((int)incl, 63) * a.U;
+  }
+  // Length of sequence b, from the lane that holds it where there are at most 64.
+  __device__ __forceinline__ int length(const PagedDecodeArgs& a, int b) const {
+    return per == 1 ? __builtin_amdgcn_readlane(len0, b) : __builtin_amdgcn_readfirstlane(paged_len(a.c, b));
+  }
+  // Granules of one unit of each sequence before b.
+  __device__ __forceinline__ int before(const PagedDecodeArgs& a, int b) const {
+    const int l = b / per;
+    int n = __builtin_amdgcn_readlane((int)(incl - mine), l);
+    for (int i = l * per; i < b; ++i) n += granules(length(a, i));
+    return n;
   }
   // The sequence that granule g lies in, its length, and its first granule.
   __device__ __forceinline__ void find(const PagedDecodeArgs& a, int g, int& b, int& len, int& first) const {
     const int l = __ffsll((unsigned long long)__ballot((int)incl * a.U > g)) - 1;
     first = __builtin_amdgcn_readlane((int)(incl - mine), l) * a.U;
-    b = l * per;
-    for (;; ++b) {
-      len = __builtin_amdgcn_readfirstlane(paged_len(a.c, b));
+    for (b = l * per;; ++b) {
+      len = length(a, b);
       const int n = granules(len) * a.U;
       if (g < first + n || b == a.B - 1) return;
       first += n;
@@ -82,6 +95,7 @@ template <int D, bool FP8, bool HALVES>
 __global__ __launch_bounds__(kDenseWaves * 64, 2) void paged_decode_kernel(PagedDecodeArgs a) {
   using C = DenseCfg<D>;
   __shared__ __attribute__((aligned(16))) char smem[C::kSmem];
+  PREFETCH_ARGS(a);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const BatchGranules all(a, lane);
   const int g0 = all.start(a, blockIdx.x), g1 = all.start(a, blockIdx.x + 1);
@@ -126,49 +140,61 @@ __global__ __launch_bounds__(kDenseWaves * 64, 2) void paged_decode_kernel(Paged
     if (++u == a.U) {
       u = 0;
       ++b;
-      len = __builtin_amdgcn_readfirstlane(paged_len(a.c, b));
+      len = all.length(a, b);
       n = granules(len);
     }
   }
 }
 
 // Joins the parts of each unit that more than one workgroup had: one wave per
-// (sequence, query head, 64 dims), four parts at a time (16 lanes hold a part's
-// dims), parts in token order within each of the four lane groups, the groups
-// folded by fixed row swaps.
+// (sequence, query head, 64 dims).  16 lanes hold a part's dims; the four lane
+// groups take the parts in turn, each in token order, and are folded by fixed row
+// swaps.  The first 32 parts and their statistics are loaded together, one round
+// trip.
 template <int D>
 __global__ __launch_bounds__(64) void paged_join_kernel(PagedDecodeArgs a) {
-  constexpr int NSL = D / 64;
+  constexpr int NSL = D / 64, PF = 8;
   const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
   const int slice = blockIdx.x % NSL, h = blockIdx.x / NSL, b = blockIdx.y;     // h: query head
   const BatchGranules all(a, lane);
-  const int hk = h / a.G, hb = (h - hk * a.G) / 16, hl = h - hk * a.G - hb * 16;
-  // granules of the sequences before b
-  uint32_t before = 0u;
-  {
-    const int l = b / all.per;
-    before = (uint32_t)__builtin_amdgcn_readlane((int)(all.incl - all.mine), l);
-    for (int i = l * all.per; i < b; ++i) before += (uint32_t)granules(paged_len(a.c, i));
-  }
-  const int n = granules(__builtin_amdgcn_readfirstlane(paged_len(a.c, b)));
-  const int s = (int)before * a.U + (hk * a.HB + hb) * n;
+  const int hk = fast_div(h, a.dG), hb = (h - hk * a.G) / 16, hl = h - hk * a.G - hb * 16;
+  const int n = granules(all.length(a, b));
+  const int s = all.before(a, b) * a.U + (hk * a.HB + hb) * n;
   const int w0 = all.owner(a, s), w1 = all.owner(a, s + n - 1);
   if (w0 == w1) return;                            // finished in place
   const int parts = w1 - w0 + 1;
   const int slot0 = all.start(a, w0) == s ? 0 : 1;
   auto slot = [&](int i) { return ((size_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * 16 + hl; };
+  const float2* pml = reinterpret_cast<const float2*>(a.part_ml);
+  const f32x4* pacc = reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item;
+  float2 ml[PF];
+  f32x4 acc[PF];
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {                   // parts past the last: its values again, with weight 0
+    const size_t r = slot(min(grp + 4 * u, parts - 1));
+    ml[u] = pml[r];
+    acc[u] = pacc[r * (D / 4)];
+  }
   float M = kNegInf;
-  for (int i = lane; i < parts; i += 64) M = fmaxf(M, a.part_ml[2 * slot(i)]);
+#pragma unroll
+  for (int u = 0; u < PF; ++u) M = fmaxf(M, ml[u].x);
+  for (int i = 4 * PF + lane; i < parts; i += 64) M = fmaxf(M, pml[slot(i)].x);
   M = wave_max_f32(M);
   if (M == kNegInf) M = 0.f;
   float L = 0.f;
   f32x4 A = {0.f, 0.f, 0.f, 0.f};
-  for (int i = grp; i < parts; i += 4) {
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {
+    const float f = grp + 4 * u < parts ? fast_exp2(ml[u].x - M) : 0.f;
+    L += f * ml[u].y;
+    A += f * acc[u];
+  }
+  for (int i = 4 * PF + grp; i < parts; i += 4) {
     const size_t r = slot(i);
-    const float2 ml = reinterpret_cast<const float2*>(a.part_ml)[r];
-    const float f = fast_exp2(ml.x - M);
-    L += f * ml.y;
-    A += f * reinterpret_cast<const f32x4*>(a.part_acc + r * D)[slice * 16 + item];
+    const float2 m = pml[r];
+    const float f = fast_exp2(m.x - M);
+    L += f * m.y;
+    A += f * pacc[r * (D / 4)];
   }
   L = col_sum4(L);
 #pragma unroll
@@ -176,16 +202,25 @@ __global__ __launch_bounds__(64) void paged_join_kernel(PagedDecodeArgs a) {
   if (grp == 0) paged_store(a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
 }
 
-// Workgroups of the decode grid: one per CU, at most the batch's granules.
-static int decode_grid(int64_t granules_max) {
-  const int64_t n = device_cu_count();
+// Workgroups of the decode grid: one per CU, whose four waves' tiles in flight
+// are what a CU's share of the memory system takes (eight sequences of up to 8K:
+// 24.3 us, 25.3 with two per CU, whose parts are twice as many to join; four of
+// 128K: 248 with either); two where the units are as many as the CUs, so that one
+// starts and ends its units while the other streams (64 sequences of up to 500
+// tokens: 14.4 with one, 13.2 with two; 32 of 16K: 228 and 229).  Never more than
+// the batch's granules.
+static int decode_grid(int64_t units, int64_t granules_max) {
+  const int64_t cus = device_cu_count(), n = units >= cus ? 2 * cus : cus;
   return (int)(granules_max < n ? granules_max : n);
 }
 
-static int64_t decode_granules(int B, int Hq, int Hk, int bs, int width) {
+struct DecodeShape {
+  int64_t units, granules;           // of the batch, at most
+};
+static DecodeShape decode_shape(int B, int Hq, int Hk, int bs, int width) {
   const int G = Hq / Hk, HB = (G + 15) / 16;
-  const int64_t per = ((int64_t)width * bs + kGranule - 1) / kGranule;
-  return (int64_t)B * Hk * HB * (per < 1 ? 1 : per);
+  const int64_t per = ((int64_t)width * bs + kGranule - 1) / kGranule, units = (int64_t)B * Hk * HB;
+  return {units, units * (per < 1 ? 1 : per)};
 }
 
 static size_t decode_workspace(int nwg, int D) { return (size_t)nwg * 2 * 16 * (D + 2) * 4; }
@@ -200,7 +235,8 @@ int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int block_si
   if (!bytes || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128)) return (int)hipErrorInvalidValue;
   const int rc = paged_check(block_size, 1, max_blocks);
   if (rc) return rc;
-  *bytes = decode_workspace(decode_grid(decode_granules(B, Hq, Hk, block_size, max_blocks)), D);
+  const DecodeShape s = decode_shape(B, Hq, Hk, block_size, max_blocks);
+  *bytes = decode_workspace(decode_grid(s.units, s.granules), D);
   return 0;
 }
 
@@ -214,8 +250,8 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
     return (int)hipErrorInvalidValue;
   int rc = paged_check(block_size, num_blocks, max_blocks);
   if (rc) return rc;
-  const int64_t most = decode_granules(B, Hq, Hk, block_size, max_blocks);
-  if (most > 0x7FFFFFFF || B > 65535) return (int)hipErrorInvalidConfiguration;
+  const DecodeShape shape = decode_shape(B, Hq, Hk, block_size, max_blocks);
+  if (shape.granules > 0x7FFFFFFF || B > 65535) return (int)hipErrorInvalidConfiguration;
   PagedDecodeArgs a;
   a.c.k = k_paged, a.c.k_sb = k_sb, a.c.k_sh = k_sh, a.c.k_ss = k_ss;
   a.c.v = v_paged, a.c.v_sb = v_sb, a.c.v_sh = v_sh, a.c.v_ss = v_ss;
@@ -226,8 +262,8 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
   a.q = static_cast<const uint16_t*>(q), a.q_sb = q_sb, a.q_sh = q_sh;
   a.out = static_cast<uint16_t*>(out), a.o_sb = o_sb, a.o_sh = o_sh;
   a.B = B, a.Hk = Hk, a.G = Hq / Hk, a.HB = (a.G + 15) / 16, a.U = Hk * a.HB;
-  a.nwg = decode_grid(most);
-  a.dnwg = make_fastdiv((uint32_t)a.nwg), a.dhb = make_fastdiv((uint32_t)a.HB);
+  a.nwg = decode_grid(shape.units, shape.granules);
+  a.dnwg = make_fastdiv((uint32_t)a.nwg), a.dhb = make_fastdiv((uint32_t)a.HB), a.dG = make_fastdiv((uint32_t)a.G);
   a.scale_log2 = scale * kLog2e, a.v_scale = v_scale;
   if (workspace_bytes < decode_workspace(a.nwg, D)) return (int)hipErrorInvalidValue;
   a.part_ml = static_cast<float*>(workspace);
