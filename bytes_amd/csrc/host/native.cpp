@@ -543,6 +543,64 @@ Tensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   return out;
 }
 
+// The rotated queries, or True without any.
+PyObject* paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const Tensor& vp, const Tensor& bt,
+                       const Tensor& cl, const Tensor* cu, const Tensor* q, const Tensor* cos, const Tensor* sin,
+                       bool interleaved, const Tensor* kmin, const Tensor* kmax, double ks, double vs) {
+  need(k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16);
+  need(bt.dim() == 2 && bt.size(0) > 0);
+  const int64_t T = k.size(0), B = bt.size(0);
+  const Paged p = paged(kp, vp, bt, cl, B, ks, vs);
+  need(T > 0 && T <= 0x7FFFFFFF && k.size(1) == p.Hk && k.size(2) == p.D);
+  rows(k);
+  rows(v);
+  same_device(kp, {&k, &v});
+  if (cu) {
+    need(shape(*cu, {B + 1}) && cu->scalar_type() == at::kInt && cu->is_contiguous());
+    same_device(kp, {cu});
+  } else {
+    need(T == B);
+  }
+  int64_t Hq = 0, rot = 0, P = 0;
+  if (q) {
+    need(q->dim() == 3 && q->scalar_type() == at::kBFloat16);
+    Hq = q->size(1);
+    need(shape(*q, {T, Hq, p.D}) && Hq > 0);
+    rows(*q);
+    same_device(kp, {q});
+  }
+  need(!cos == !sin && !kmin == !kmax);
+  if (cos) {
+    need(cos->dim() == 2 && sin->sizes() == cos->sizes() && cos->scalar_type() == at::kFloat &&
+         sin->scalar_type() == at::kFloat);
+    P = cos->size(0), rot = 2 * cos->size(1);
+    need(rot > 0 && rot % 16 == 0 && rot <= p.D && P >= p.W * p.bs && P <= 0x7FFFFFFF);
+    rows(*cos);
+    rows(*sin);
+    same_device(kp, {cos, sin});
+  }
+  if (kmin) {
+    for (const Tensor* t : {kmin, kmax}) {
+      need(t->scalar_type() == at::kBFloat16 && shape(*t, {p.N, p.Hk, p.D}) && t->is_contiguous() && addr(*t) % 16 == 0);
+      same_device(kp, {t});
+    }
+  }
+  c10::DeviceGuard guard(kp.device());
+  Tensor out;
+  if (q) out = empty(*q, {T, Hq, p.D}, at::kBFloat16);
+  void* st = stream_of(kp);
+  launch("bytes_paged_kv_append", bytes_paged_kv_append, data(k), k.stride(0), k.stride(1), data(v), v.stride(0),
+         v.stride(1), q ? data(*q) : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+         q ? out.mutable_data_ptr() : nullptr, q ? out.stride(0) : 0, q ? out.stride(1) : 0, kp.mutable_data_ptr(),
+         kp.stride(0), kp.stride(1), kp.stride(2), vp.mutable_data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2), p.f8,
+         kmin ? kmin->mutable_data_ptr() : nullptr, kmax ? kmax->mutable_data_ptr() : nullptr, data(bt), bt.stride(0),
+         data(cl), cu ? data(*cu) : nullptr, cos ? data(*cos) : nullptr, cos ? cos->stride(0) : 0,
+         sin ? data(*sin) : nullptr, sin ? sin->stride(0) : 0, (int)P, (int)rot, interleaved, (float)ks, (float)vs, (int)T,
+         (int)B, (int)Hq, (int)p.Hk, (int)p.D, (int)p.bs, (int)p.N, (int)p.W, st);
+  if (!q) Py_RETURN_TRUE;
+  return THPVariable_Wrap(out);
+}
+
 // ---- bindings ----
 
 template <class F>
@@ -601,6 +659,9 @@ BIND(token_topk, 9, token_topk(tensor(a[0]), tensor(a[1]), tensor(a[2]), integer
 BIND(quest, 10, WRAP(quest(tensor(a[0]), tensor(a[1]), tensor(a[2]), integer(a[3]), number(a[4]), integer(a[5]),
                            tensor(a[6]), tensor(a[7]), integer(a[8]), integer(a[9]))))
 
+BIND(paged_append, 15, paged_append(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]),
+                                    optional(a[6]), optional(a[7]), optional(a[8]), optional(a[9]), a[10] == Py_True,
+                                    optional(a[11]), optional(a[12]), number(a[13]), number(a[14])))
 BIND(paged_decode, 8, WRAP(paged_decode(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), number(a[5]),
                                         number(a[6]), number(a[7]))))
 
@@ -618,7 +679,7 @@ PyObject* py_set_workspaces(PyObject*, PyObject* d) {
 PyMethodDef methods[] = {METHOD(dense),     METHOD(kivi),   METHOD(kivi_pack), METHOD(pq_fused),
                          METHOD(pq_asym),   METHOD(pq_paged), METHOD(pq_encode), METHOD(score_into), METHOD(topk),
                          METHOD(gather),    METHOD(sparse_decode), METHOD(token_topk), METHOD(quest),
-                         METHOD(paged_decode),
+                         METHOD(paged_append), METHOD(paged_decode),
                          {"set_workspaces", py_set_workspaces, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the operators.", -1, methods};

@@ -8,9 +8,19 @@
 // blocks' elementwise min / max (of the values as stored) are kept for the
 // page-sparse decode.
 //
-// One workgroup per token; a thread takes 16 elements of one head: for pairs
-// (j, j + R/2) two runs of 8, R/2 apart.  The workgroup of the first new token
-// of each block also folds the block's min / max.
+// A lane takes 16 elements of one head (an item): for pairs (j, j + R/2) two runs
+// of 8, R/2 apart, so both of a pair are in its registers and its cos and sin are
+// 8 consecutive floats.  D/16 lanes cover a row; a wave's 64 lanes are 64/(D/16)
+// rows.
+//  * One token per sequence: a wave's rows are heads (keys, values and queries in
+//    one list) of one token.
+//  * Prompts: a wave's rows are consecutive tokens of one sequence, for 2 key, 4
+//    value or 4 query heads, whose cos and sin it then loads once.  Values and queries (and keys
+//    where no min / max is kept) go in spans of 32 positions, keys with min / max in blocks:
+//    a wave has a whole block's new tokens, so it folds their min / max in
+//    registers and across its lanes, without atomics or a second read.
+//    Spans are numbered over the batch; every wave finds its own from a prefix sum
+//    over the sequences (device-side lengths), rows past the last sequence being one more.
 #include "paged.h"
 
 namespace bytes_amd {
@@ -27,29 +37,19 @@ struct AppendArgs {
   int64_t cos_st, sin_st;
   int rot, interleaved;
   float k_scale, v_scale;
-  int T, B, Hq, Hk, D;
+  int T, B, Hq, Hk;
+  int cap;                           // positions a table row holds
+  // prompts: workgroups of the key spans come first; per span, the waves' head groups
+  int k_span, k_wgs, o_wgs;          // key span length; workgroups per key span, per other span
+  int64_t k_grid;                    // workgroups of all key spans
+  FastDiv dk_span, dk_wgs, do_wgs;
+  int per_token;                     // one token each: waves per token
+  FastDiv d_per_token;
 };
 
-// Row t's sequence, position and number of earlier new tokens of that sequence; false: no position.
-__device__ __forceinline__ bool append_locate(const AppendArgs& a, int t, int& b, int64_t& p, int64_t& i) {
-  if (!a.cu) {
-    b = t;
-    i = 0;
-    p = (int64_t)a.c.lens[b] - 1;
-  } else {
-    int lo = 0, hi = a.B;              // first b with cu[b + 1] > t
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.cu[mid + 1] <= t) lo = mid + 1;
-      else hi = mid;
-    }
-    b = lo;
-    if (b >= a.B) return false;
-    i = (int64_t)t - a.cu[b];
-    p = (int64_t)a.c.lens[b] - ((int64_t)a.cu[b + 1] - t);
-  }
-  return i >= 0 && p >= 0 && p < (int64_t)a.c.width * a.c.bs;
-}
+constexpr int kAppendWaves = 4;
+constexpr int kSpan = 32;            // positions per span of values and queries
+constexpr int kKeyHeads = 2, kRowHeads = 4;    // heads per wave: keys; values, queries
 
 __device__ __forceinline__ void widen8(const u32x4& r, float* x) {
 #pragma unroll
@@ -86,132 +86,336 @@ __device__ __forceinline__ void widen8_fp8(const u32x2& r, float* x) {
   }
 }
 
-// Where the two runs of 8 of item c start in a head of D dims.
-__device__ __forceinline__ void item_runs(const AppendArgs& a, int c, int& d0, int& d1) {
-  const bool halves = !a.interleaved && 16 * c < a.rot;
-  d0 = halves ? 8 * c : 16 * c;
-  d1 = halves ? 8 * c + a.rot / 2 : 16 * c + 8;
-}
 
-// Item c of a row at position p, rotated: x[0..7] and x[8..15] are its two runs.
-__device__ __forceinline__ void load_rotated(const AppendArgs& a, const uint16_t* row, int c, int64_t p, float* x) {
-  int d0, d1;
-  item_runs(a, c, d0, d1);
-  widen8(ld16(row + d0), x);
-  widen8(ld16(row + d1), x + 8);
-  if (16 * c >= a.rot) return;
-  const float* cp = a.cos + p * a.cos_st + 8 * c;
-  const float* sp = a.sin + p * a.sin_st + 8 * c;
-  float y[16];
+// What a lane does with each row: its item's two runs, and whether it is rotated.
+struct AppendItem {
+  int c, d0, d1;
+  bool turn;
+  __device__ __forceinline__ AppendItem(const AppendArgs& a, int c_) : c(c_) {
+    turn = 16 * c < a.rot;
+    const bool halves = turn && !a.interleaved;
+    d0 = halves ? 8 * c : 16 * c;
+    d1 = halves ? 8 * c + a.rot / 2 : 16 * c + 8;
+  }
+};
+
+struct Turn {                        // cos and sin of an item's 8 pairs
+  float c[8], s[8];
+};
+__device__ __forceinline__ void load_turn(const AppendArgs& a, const AppendItem& it, int64_t p, Turn& r) {
+  const float* cp = a.cos + p * a.cos_st + 8 * it.c;
+  const float* sp = a.sin + p * a.sin_st + 8 * it.c;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e0 = a.interleaved ? 2 * j : j, e1 = a.interleaved ? 2 * j + 1 : j + 8;
-    const float cs = cp[j], sn = sp[j];
-    y[e0] = x[e0] * cs - x[e1] * sn;
-    y[e1] = x[e1] * cs + x[e0] * sn;
+  for (int j = 0; j < 2; ++j) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(cp + 4 * j), y = *reinterpret_cast<const f32x4*>(sp + 4 * j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.c[4 * j + e] = x[e], r.s[4 * j + e] = y[e];
+  }
+}
+__device__ __forceinline__ void turn_item(const AppendArgs& a, const Turn& r, float* x) {
+  float y[16];
+  if (a.interleaved) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      y[2 * j] = x[2 * j] * r.c[j] - x[2 * j + 1] * r.s[j];
+      y[2 * j + 1] = x[2 * j + 1] * r.c[j] + x[2 * j] * r.s[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      y[j] = x[j] * r.c[j] - x[j + 8] * r.s[j];
+      y[j + 8] = x[j + 8] * r.c[j] + x[j] * r.s[j];
+    }
   }
 #pragma unroll
   for (int j = 0; j < 16; ++j) x[j] = y[j];
 }
 
-// Stores the item in the cache row; x becomes what the cache then holds.
+// Stores the item in its cache row (`to` the row's start); x becomes what the cache then holds.
 template <bool FP8>
-__device__ __forceinline__ void store_cache(void* row, int d0, int d1, float scale, float* x) {
+__device__ __forceinline__ void store_cache(char* to, const AppendItem& it, float scale, float* x) {
   if constexpr (FP8) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) x[j] = x[j] / scale;
     const u32x2 r0 = narrow8_fp8(x), r1 = narrow8_fp8(x + 8);
-    if (row) {
-      *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(row) + d0) = r0;
-      *reinterpret_cast<u32x2*>(static_cast<uint8_t*>(row) + d1) = r1;
-    }
+    *reinterpret_cast<u32x2*>(to + it.d0) = r0;
+    *reinterpret_cast<u32x2*>(to + it.d1) = r1;
     widen8_fp8(r0, x);
     widen8_fp8(r1, x + 8);
   } else {
     const u32x4 r0 = narrow8(x), r1 = narrow8(x + 8);
-    if (row) {
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(row) + d0) = r0;
-      *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(row) + d1) = r1;
-    }
+    *reinterpret_cast<u32x4*>(to + 2 * it.d0) = r0;
+    *reinterpret_cast<u32x4*>(to + 2 * it.d1) = r1;
     widen8(r0, x);
     widen8(r1, x + 8);
   }
 }
-
+__device__ __forceinline__ void store_item(uint16_t* row, const AppendItem& it, const float* x) {
+  *reinterpret_cast<u32x4*>(row + it.d0) = narrow8(x);
+  *reinterpret_cast<u32x4*>(row + it.d1) = narrow8(x + 8);
+}
+__device__ __forceinline__ void load_item(const uint16_t* row, const AppendItem& it, float* x) {
+  widen8(ld16(row + it.d0), x);
+  widen8(ld16(row + it.d1), x + 8);
+}
 template <bool FP8>
-__global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
-  const int t = blockIdx.x;
-  const int items = a.D / 16;
-  int b = 0;
-  int64_t p = 0, i = 0;
-  const bool placed = append_locate(a, t, b, p, i);
-  const int blk = placed ? fast_div((int)p, a.c.dbs) : 0, off = placed ? (int)p - blk * a.c.bs : 0;
-  const int id = placed ? a.c.table[(int64_t)b * a.c.bt_sb + blk] : -1;
-  const bool held = id >= 0 && id < a.c.nblocks;
-  constexpr int ES = FP8 ? 1 : 2;
-  char* kc = static_cast<char*>(const_cast<void*>(a.c.k)) + ((int64_t)(held ? id : 0) * a.c.k_sb + off * a.c.k_ss) * ES;
-  char* vc = static_cast<char*>(const_cast<void*>(a.c.v)) + ((int64_t)(held ? id : 0) * a.c.v_sb + off * a.c.v_ss) * ES;
+__device__ __forceinline__ char* cache_row(const void* base, int64_t sb, int64_t sh, int64_t ss, int id, int h, int off) {
+  return static_cast<char*>(const_cast<void*>(base)) + (id * sb + h * sh + off * ss) * (FP8 ? 1 : 2);
+}
+
+// IEEE minimum / maximum: a NaN stays, and the order of the values does not matter.
+__device__ __forceinline__ float lower(float a, float b) { return __builtin_elementwise_minimum(a, b); }
+__device__ __forceinline__ float upper(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Folds v over the lanes that hold the same item of other rows (lane bits from
+// log2(LPR) up): rotations within the rows of 16, then the row and half swaps.
+template <int LPR, class OP>
+__device__ __forceinline__ float fold_rows(float v, OP op) {
+  v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x128, 0xF, 0xF, false)));
+  if (LPR == 4)
+    v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x124, 0xF, 0xF, false)));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// One token of one sequence per wave and up to 64 / LPR of its heads' rows.
+template <int D, bool FP8>
+__global__ __launch_bounds__(kAppendWaves * 64) void paged_append_one_kernel(AppendArgs a) {
+  PREFETCH_ARGS(a);
+  constexpr int LPR = D / 16, ROWS = 64 / LPR;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int gid = blockIdx.x * kAppendWaves + w;
+  const int t = fast_div(gid, a.d_per_token);
+  if (t >= a.T) return;
+  const int len = a.c.lens[t];
+  const AppendItem it(a, lane % LPR);
+  const int r = (gid - t * a.per_token) * ROWS + lane / LPR, rows = 2 * a.Hk + a.Hq;
+  const bool live = r < rows, key = r < a.Hk, value = !key && r < 2 * a.Hk;
+  const int h = key ? r : value ? r - a.Hk : live ? r - 2 * a.Hk : 0;
+  // the row, at once with the length; values are never rotated: their item is 16 dims in a row
+  const int d0 = value ? 16 * it.c : it.d0, d1 = value ? 16 * it.c + 8 : it.d1;
+  const uint16_t* src = key || !live ? a.k + t * a.k_st + h * a.k_sh : value ? a.v + t * a.v_st + h * a.v_sh
+                                                                              : a.q + t * a.q_st + h * a.q_sh;
+  const u32x4 x0 = ld16(src + d0), x1 = ld16(src + d1);
+  const int p = len - 1;
+  const bool placed = len > 0 && p < a.cap;
+  const int ps = placed ? p : 0, blk = fast_div(ps, a.c.dbs), off = ps - blk * a.c.bs;
+  const int id = a.c.table[(int64_t)t * a.c.bt_sb + blk];
+  const bool held = placed && id >= 0 && id < a.c.nblocks;
   float x[16];
-  for (int e = threadIdx.x; e < (2 * a.Hk + a.Hq) * items; e += blockDim.x) {
-    const int h = e / items, c = e - h * items;
-    if (h < a.Hk) {
-      if (!held) continue;
-      int d0, d1;
-      item_runs(a, c, d0, d1);
-      load_rotated(a, a.k + t * a.k_st + h * a.k_sh, c, p, x);
-      store_cache<FP8>(kc + h * a.c.k_sh * ES, d0, d1, a.k_scale, x);
-    } else if (h < 2 * a.Hk) {
-      if (!held) continue;
-      const int hh = h - a.Hk;
-      const uint16_t* row = a.v + t * a.v_st + hh * a.v_sh + 16 * c;
-      widen8(ld16(row), x);
-      widen8(ld16(row + 8), x + 8);
-      store_cache<FP8>(vc + hh * a.c.v_sh * ES, 16 * c, 16 * c + 8, a.v_scale, x);
-    } else {
-      const int hh = h - 2 * a.Hk;
-      int d0, d1;
-      item_runs(a, c, d0, d1);
-      if (placed) {
-        load_rotated(a, a.q + t * a.q_st + hh * a.q_sh, c, p, x);
-      } else {
+  widen8(x0, x);
+  widen8(x1, x + 8);
+  if (live && !value && it.turn && placed) {
+    Turn tr;
+    load_turn(a, it, ps, tr);
+    turn_item(a, tr, x);
+  }
+  if (!live) return;
+  if (key) {
+    if (!held) return;
+    float mn[16], mx[16];
+    uint16_t* pmn = a.kmin + ((int64_t)id * a.Hk + h) * D;
+    uint16_t* pmx = a.kmax + ((int64_t)id * a.Hk + h) * D;
+    if (a.kmin && off) {
+      load_item(pmn, it, mn);
+      load_item(pmx, it, mx);
+    }
+    store_cache<FP8>(cache_row<FP8>(a.c.k, a.c.k_sb, a.c.k_sh, a.c.k_ss, id, h, off), it, a.k_scale, x);
+    if (!a.kmin) return;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = 0.f;
+    for (int j = 0; j < 16; ++j) {
+      mn[j] = off ? lower(mn[j], x[j]) : x[j];
+      mx[j] = off ? upper(mx[j], x[j]) : x[j];
+    }
+    store_item(pmn, it, mn);
+    store_item(pmx, it, mx);
+  } else if (value) {
+    if (!held) return;
+    char* to = cache_row<FP8>(a.c.v, a.c.v_sb, a.c.v_sh, a.c.v_ss, id, h, off);
+    if constexpr (FP8) {
+      AppendItem flat = it;
+      flat.d0 = d0, flat.d1 = d1;
+      store_cache<FP8>(to, flat, a.v_scale, x);
+    } else {
+      *reinterpret_cast<u32x4*>(to + 2 * d0) = x0;
+      *reinterpret_cast<u32x4*>(to + 2 * d1) = x1;
+    }
+  } else {
+    if (!placed) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] = 0.f;
+    }
+    store_item(a.q_out + t * a.qo_st + h * a.qo_sh, it, x);
+  }
+}
+
+// A span of new tokens: rows t0 .. t0 + n - 1 of sequence b (b = B: rows past the
+// last sequence), the first at position p0 (negative: no position).
+struct Span {
+  int b, t0, n, p0;
+};
+
+__device__ __forceinline__ int floor_div(int p, const FastDiv& d) { return p >= 0 ? fast_div(p, d) : -1 - fast_div(-1 - p, d); }
+
+// Span number r of the batch, spans being aligned to multiples of `len`
+// positions; false past the last.  Lane l looks at sequence 64 i + l.
+__device__ __forceinline__ bool find_span(const AppendArgs& a, int r, int len, const FastDiv& dlen, int lane, Span& s) {
+  for (int b0 = 0; b0 <= a.B; b0 += 64) {
+    const int b = b0 + lane, bc = min(b, a.B);
+    const int c0 = min(max(a.cu[bc], 0), a.T), c1 = b < a.B ? min(max(a.cu[bc + 1], 0), a.T) : a.T;
+    const int n = b <= a.B ? max(c1 - c0, 0) : 0;
+    const int end = b < a.B ? max(a.c.lens[min(b, a.B - 1)], 0) : 0, first = end - n;
+    const int f0 = floor_div(first, dlen);
+    const uint32_t mine = n > 0 ? (uint32_t)(floor_div(end - 1, dlen) - f0 + 1) : 0u;
+    const uint32_t incl = wave_prefix_sum(mine);
+    const int total = __builtin_amdgcn_readlane((int)incl, 63);
+    if (r < total) {
+      const int l = __ffsll((unsigned long long)__ballot((int)incl > r)) - 1;
+      const int j = r - __builtin_amdgcn_readlane((int)(incl - mine), l);
+      const int sn = __builtin_amdgcn_readlane(n, l), sc = __builtin_amdgcn_readlane(c0, l);
+      const int sf = __builtin_amdgcn_readlane(first, l), s0 = __builtin_amdgcn_readlane(f0, l) + j;
+      const int64_t lo = max((int64_t)s0 * len, (int64_t)sf), hi = min(((int64_t)s0 + 1) * len, (int64_t)sf + sn);
+      s.b = b0 + l;
+      s.p0 = (int)lo;
+      s.t0 = sc + (int)(lo - sf);
+      s.n = (int)(hi - lo);
+      if (s.b == a.B) s.p0 = -0x40000000;          // no sequence: no position
+      return true;
+    }
+    r -= total;
+  }
+  return false;
+}
+
+enum : int { kKeys = 0, kValues = 1, kQueries = 2 };
+
+// The span's rows of NH heads from h0 (nh of them exist): ROWS tokens at a time.
+template <int D, bool FP8, int KIND, int NH>
+__device__ __forceinline__ void append_span(const AppendArgs& a, const Span& s, int h0, int nh, int lane) {
+  constexpr int LPR = D / 16, ROWS = 64 / LPR;
+  AppendItem it(a, lane % LPR);
+  if (KIND == kValues) it.d0 = 16 * it.c, it.d1 = 16 * it.c + 8;
+  const bool fold = KIND == kKeys && a.kmin != nullptr;
+  float mn[NH][16], mx[NH][16];
+  if (fold) {
+#pragma unroll
+    for (int u = 0; u < NH; ++u)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mn[u][j] = __builtin_inff(), mx[u][j] = kNegInf;
+  }
+  const uint16_t* src = KIND == kKeys ? a.k : KIND == kValues ? a.v : a.q;
+  const int64_t st = KIND == kKeys ? a.k_st : KIND == kValues ? a.v_st : a.q_st;
+  const int64_t sh = KIND == kKeys ? a.k_sh : KIND == kValues ? a.v_sh : a.q_sh;
+  const int32_t* table = a.c.table + (int64_t)min(s.b, a.B - 1) * a.c.bt_sb;
+  int block = -1;                                  // (one block per span where min / max are folded)
+  for (int i0 = 0; i0 < s.n; i0 += ROWS) {
+    const int i = i0 + lane / LPR;
+    const bool row = i < s.n;
+    const int t = s.t0 + (row ? i : 0), p = s.p0 + (row ? i : 0);
+    const bool placed = row && p >= 0 && p < a.cap;
+    const int ps = placed ? p : 0;
+    u32x4 raw[NH][2];
+#pragma unroll
+    for (int u = 0; u < NH; ++u) {
+      const uint16_t* x = src + t * st + (h0 + min(u, nh - 1)) * sh;
+      raw[u][0] = ld16(x + it.d0);
+      raw[u][1] = ld16(x + it.d1);
+    }
+    int id = -1, off = 0;
+    if (KIND != kQueries) {
+      const int blk = fast_div(ps, a.c.dbs);
+      off = ps - blk * a.c.bs;
+      id = table[blk];
+    }
+    const bool held = placed && id >= 0 && id < a.c.nblocks;
+    Turn tr;
+    if (KIND != kValues && it.turn) load_turn(a, it, ps, tr);
+#pragma unroll
+    for (int u = 0; u < NH; ++u) {
+      if (u >= nh) break;
+      float x[16];
+      widen8(raw[u][0], x);
+      widen8(raw[u][1], x + 8);
+      if (KIND != kValues && it.turn) turn_item(a, tr, x);
+      if (KIND == kQueries) {
+        if (!placed) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] = 0.f;
+        }
+        if (row) store_item(a.q_out + t * a.qo_st + (h0 + u) * a.qo_sh, it, x);
+      } else if (held) {
+        char* to = KIND == kKeys ? cache_row<FP8>(a.c.k, a.c.k_sb, a.c.k_sh, a.c.k_ss, id, h0 + u, off)
+                                 : cache_row<FP8>(a.c.v, a.c.v_sb, a.c.v_sh, a.c.v_ss, id, h0 + u, off);
+        if constexpr (KIND == kValues && !FP8) {
+          *reinterpret_cast<u32x4*>(to + 2 * it.d0) = raw[u][0];
+          *reinterpret_cast<u32x4*>(to + 2 * it.d1) = raw[u][1];
+        } else {
+          store_cache<FP8>(to, it, KIND == kKeys ? a.k_scale : a.v_scale, x);
+        }
+        if (fold) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            mn[u][j] = lower(mn[u][j], x[j]);
+            mx[u][j] = upper(mx[u][j], x[j]);
+          }
+        }
       }
-      uint16_t* row = a.q_out + t * a.qo_st + hh * a.qo_sh;
-      *reinterpret_cast<u32x4*>(row + d0) = narrow8(x);
-      *reinterpret_cast<u32x4*>(row + d1) = narrow8(x + 8);
+    }
+    if (fold) {
+      const unsigned long long m = __ballot(held);
+      if (m) block = __builtin_amdgcn_readlane(id, __ffsll(m) - 1);
     }
   }
-  // first new token of its block: the block's min / max over the run
-  if (!a.kmin || !held || (off != 0 && i != 0)) return;
-  const int64_t left = (int64_t)(a.cu ? min(a.cu[b + 1], a.T) : t + 1) - t;
-  const int n = (int)(left < a.c.bs - off ? left : a.c.bs - off);
-  for (int e = threadIdx.x; e < a.Hk * items; e += blockDim.x) {
-    const int h = e / items, c = e - h * items;
-    int d0, d1;
-    item_runs(a, c, d0, d1);
-    float mn[16], mx[16];
-    uint16_t* pmn = a.kmin + ((int64_t)id * a.Hk + h) * a.D;
-    uint16_t* pmx = a.kmax + ((int64_t)id * a.Hk + h) * a.D;
-    if (off) {
-      widen8(ld16(pmn + d0), mn);
-      widen8(ld16(pmn + d1), mn + 8);
-      widen8(ld16(pmx + d0), mx);
-      widen8(ld16(pmx + d1), mx + 8);
-    }
-    for (int j = 0; j < n; ++j) {
-      load_rotated(a, a.k + (t + j) * a.k_st + h * a.k_sh, c, p + j, x);
-      store_cache<FP8>(nullptr, d0, d1, a.k_scale, x);
+  if (!fold || block < 0) return;
+  const int p1 = max(s.p0, 0);
+  const bool entered = p1 - fast_div(p1, a.c.dbs) * a.c.bs == 0;         // at the block's first row
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        mn[u] = j == 0 && !off ? x[u] : nan_min(mn[u], x[u]);
-        mx[u] = j == 0 && !off ? x[u] : nan_max(mx[u], x[u]);
-      }
+  for (int u = 0; u < NH; ++u) {
+    if (u >= nh) break;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      mn[u][j] = fold_rows<LPR>(mn[u][j], lower);
+      mx[u][j] = fold_rows<LPR>(mx[u][j], upper);
     }
-    *reinterpret_cast<u32x4*>(pmn + d0) = narrow8(mn);
-    *reinterpret_cast<u32x4*>(pmn + d1) = narrow8(mn + 8);
-    *reinterpret_cast<u32x4*>(pmx + d0) = narrow8(mx);
-    *reinterpret_cast<u32x4*>(pmx + d1) = narrow8(mx + 8);
+    if (lane >= LPR) continue;
+    uint16_t* pmn = a.kmin + ((int64_t)block * a.Hk + h0 + u) * D;
+    uint16_t* pmx = a.kmax + ((int64_t)block * a.Hk + h0 + u) * D;
+    if (!entered) {
+      float o[16];
+      load_item(pmn, it, o);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mn[u][j] = lower(mn[u][j], o[j]);
+      load_item(pmx, it, o);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx[u][j] = upper(mx[u][j], o[j]);
+    }
+    store_item(pmn, it, mn[u]);
+    store_item(pmx, it, mx[u]);
+  }
+}
+
+template <int D, bool FP8>
+__global__ __launch_bounds__(kAppendWaves * 64) void paged_append_kernel(AppendArgs a) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Span s;
+  if (blockIdx.x < a.k_grid) {
+    const int r = fast_div((int)blockIdx.x, a.dk_wgs);
+    const int h0 = (((int)blockIdx.x - r * a.k_wgs) * kAppendWaves + w) * kKeyHeads;
+    if (h0 >= a.Hk || !find_span(a, r, a.k_span, a.dk_span, lane, s) || s.b == a.B) return;
+    append_span<D, FP8, kKeys, kKeyHeads>(a, s, h0, min(kKeyHeads, a.Hk - h0), lane);
+  } else {
+    const int x = (int)((int64_t)blockIdx.x - a.k_grid), r = fast_div(x, a.do_wgs);
+    const int g = (x - r * a.o_wgs) * kAppendWaves + w, gv = (a.Hk + kRowHeads - 1) / kRowHeads;
+    const bool values = g < gv;
+    const int h0 = (values ? g : g - gv) * kRowHeads, heads = values ? a.Hk : a.Hq;
+    if (h0 >= heads || !find_span(a, r, kSpan, FastDiv{1u, 5u, 32u}, lane, s)) return;
+    if (values) {
+      if (s.b < a.B) append_span<D, FP8, kValues, kRowHeads>(a, s, h0, min(kRowHeads, heads - h0), lane);
+    } else {
+      append_span<D, FP8, kQueries, kRowHeads>(a, s, h0, min(kRowHeads, heads - h0), lane);
+    }
   }
 }
 
@@ -239,7 +443,7 @@ int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void*
   if (rc) return rc;
   if (rot && (!cos || !sin || (int64_t)positions < (int64_t)max_blocks * block_size)) return (int)hipErrorInvalidValue;
   if (T == 0) return 0;
-  AppendArgs a;
+  AppendArgs a = {};
   a.c.k = k_paged;
   a.c.v = v_paged;
   a.c.k_sb = kp_sb, a.c.k_sh = kp_sh, a.c.k_ss = kp_ss;
@@ -259,12 +463,45 @@ int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void*
   a.cos_st = cos_st, a.sin_st = sin_st;
   a.rot = rot, a.interleaved = interleaved ? 1 : 0;
   a.k_scale = k_scale, a.v_scale = v_scale;
-  a.T = T, a.B = B, a.Hq = Hq, a.Hk = Hk, a.D = D;
+  a.T = T, a.B = B, a.Hq = Hq, a.Hk = Hk;
+  a.cap = max_blocks * block_size;
+  int64_t grid;
+  if (!cu_seqlens) {
+    const int rows_per_wave = 64 / (D / 16);
+    a.per_token = (2 * Hk + Hq + rows_per_wave - 1) / rows_per_wave;
+    a.d_per_token = make_fastdiv((uint32_t)a.per_token);
+    grid = ((int64_t)T * a.per_token + kAppendWaves - 1) / kAppendWaves;
+  } else {
+    // a sequence's n tokens lie in at most n / span + 2 spans, and in at most n
+    auto spans = [&](int len) {
+      const int64_t n = (int64_t)T / len + 2 * ((int64_t)B + 1);
+      return n < T ? n : (int64_t)T;
+    };
+    const int per_key = kAppendWaves * kKeyHeads;
+    a.k_span = kmin ? block_size : kSpan;
+    a.dk_span = make_fastdiv((uint32_t)a.k_span);
+    a.k_wgs = (Hk + per_key - 1) / per_key;
+    a.k_grid = spans(a.k_span) * a.k_wgs;
+    a.dk_wgs = make_fastdiv((uint32_t)a.k_wgs);
+    const int groups = (Hk + kRowHeads - 1) / kRowHeads + (Hq + kRowHeads - 1) / kRowHeads;
+    a.o_wgs = (groups + kAppendWaves - 1) / kAppendWaves;
+    a.do_wgs = make_fastdiv((uint32_t)a.o_wgs);
+    grid = a.k_grid + spans(kSpan) * a.o_wgs;
+  }
+  if (grid > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
+  const dim3 g((unsigned)grid), block(kAppendWaves * 64);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (kv_fp8)
-    hipLaunchKernelGGL(paged_append_kernel<true>, dim3((unsigned)T), dim3(256), 0, st, a);
-  else
-    hipLaunchKernelGGL(paged_append_kernel<false>, dim3((unsigned)T), dim3(256), 0, st, a);
+#define PA(DD, F8)                                                                   \
+  if (cu_seqlens) hipLaunchKernelGGL((paged_append_kernel<DD, F8>), g, block, 0, st, a); \
+  else hipLaunchKernelGGL((paged_append_one_kernel<DD, F8>), g, block, 0, st, a)
+  if (D == 128) {
+    if (kv_fp8) { PA(128, true); }
+    else { PA(128, false); }
+  } else {
+    if (kv_fp8) { PA(64, true); }
+    else { PA(64, false); }
+  }
+#undef PA
   return (int)hipGetLastError();
 }
 

@@ -139,6 +139,11 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
     Without q the result is None.
 
     Blocks that receive tokens must belong to one sequence each (blocks of a shared prefix are only read)."""
+    kmin, kmax = meta if meta is not None else (None, None)
+    out = native().paged_append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin,
+                                bool(interleaved), kmin, kmax, k_scale, v_scale)
+    if out is not None:
+        return out if q is not None else None
     C.cuda_tensors(k, v, k_paged, v_paged, block_table, context_lens,
                    *(t for t in (cu_seqlens, q, cos, sin, *(meta or ())) if t is not None))
     N, Hk, bs, D, fp8 = _cache(k_paged, v_paged, k_scale, v_scale)
@@ -176,7 +181,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
         if P < bt.shape[1] * bs:
             raise ValueError(f"cos, sin hold {P} positions, the block table {bt.shape[1] * bs}")
         cos, sin = C.rows16(cos), C.rows16(sin)
-    kmin, kmax = _meta(meta, N, Hk, D) if meta is not None else (None, None)
+    if meta is not None:
+        kmin, kmax = _meta(meta, N, Hk, D)
     k, v = C.rows16(k), C.rows16(v)
     out = None
     if q is not None:
