@@ -514,7 +514,7 @@ Paged paged(const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& cl
   need(std::isfinite(ks) && std::isfinite(vs) && ks > 0 && vs > 0 && (f8 || (ks == 1.0 && vs == 1.0)));
   need(bt.dim() == 2 && bt.size(0) == B && bt.scalar_type() == at::kInt && (bt.stride(1) == 1 || p.W == 1) && p.W > 0);
   need(shape(cl, {B}) && cl.scalar_type() == at::kInt && cl.is_contiguous());
-  need(p.bs <= 0x7FFFFFFF - 1024 && p.W * p.bs <= 0x7FFFFFFF - 1024);
+  need(p.bs <= (1 << 30) && p.W * p.bs <= (1 << 30));
   same_device(k, {&v, &bt, &cl});
   return p;
 }
@@ -540,6 +540,36 @@ Tensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
          k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), p.f8, data(bt), bt.stride(0), data(cl),
          out.mutable_data_ptr(), out.stride(0), out.stride(1), B, Hq, p.Hk, p.D, p.bs, p.N, p.W, (float)(scale * ks),
          (float)vs, w.mutable_data_ptr(), n, st);
+  return out;
+}
+
+// Selection inside the attention kernel: up to 4096 blocks in a table row.
+Tensor paged_quest(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kmin, const Tensor& kmax,
+                   const Tensor& bt, const Tensor& cl, long kb, double scaling, long local_w, double ks, double vs) {
+  paged_query(q, k);
+  const int64_t B = q.size(0), Hq = q.size(1);
+  const Paged p = paged(k, v, bt, cl, B, ks, vs);
+  need(p.W <= 4096 && kb >= 1 && local_w >= 0 && local_w <= (1 << 30));
+  for (const Tensor* t : {&kmin, &kmax})
+    need(t->scalar_type() == at::kBFloat16 && shape(*t, {p.N, p.Hk, p.D}) && t->is_contiguous() && addr(*t) % 16 == 0);
+  same_device(k, {&kmin, &kmax});
+  const int64_t all = (kb + p.bs - 1) / p.bs, npick = all < p.W ? all : p.W;
+  c10::DeviceGuard guard(q.device());
+  size_t n = 0;
+  need(bytes_paged_quest_workspace_size(B, Hq, p.Hk, p.D, p.bs, npick, &n) == 0);
+  const Tensor bound = empty(q, {B, Hq, p.W}, at::kFloat);
+  const Tensor w = empty(q, {(int64_t)n}, at::kByte);
+  Tensor out = empty(q, {B, Hq, 1, p.D}, at::kBFloat16);
+  const double scale = scaling * ks;
+  void* st = stream_of(q);
+  launch("bytes_paged_page_scores", bytes_paged_page_scores, data(q), q.stride(0), q.stride(1), data(kmin), data(kmax),
+         data(bt), bt.stride(0), data(cl), bound.mutable_data_ptr(), bound.stride(0), bound.stride(1), B, Hq, p.Hk, p.D,
+         p.bs, p.N, p.W, (int)local_w, (int)npick, scale, st);
+  launch("bytes_paged_quest_attn", bytes_paged_quest_attn, data(q), q.stride(0), q.stride(1), data(k), k.stride(0),
+         k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), p.f8, data(bound), bound.stride(0),
+         bound.stride(1), nullptr, 0, 0, (int)npick, data(bt), bt.stride(0), data(cl), out.mutable_data_ptr(),
+         out.stride(0), out.stride(1), B, Hq, p.Hk, p.D, p.bs, p.N, p.W, (float)scale, (float)vs,
+         n ? w.mutable_data_ptr() : nullptr, n, st);
   return out;
 }
 
@@ -659,6 +689,9 @@ BIND(token_topk, 9, token_topk(tensor(a[0]), tensor(a[1]), tensor(a[2]), integer
 BIND(quest, 10, WRAP(quest(tensor(a[0]), tensor(a[1]), tensor(a[2]), integer(a[3]), number(a[4]), integer(a[5]),
                            tensor(a[6]), tensor(a[7]), integer(a[8]), integer(a[9]))))
 
+BIND(paged_quest, 12, WRAP(paged_quest(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]),
+                                       tensor(a[6]), integer(a[7]), number(a[8]), integer(a[9]), number(a[10]),
+                                       number(a[11]))))
 BIND(paged_append, 15, paged_append(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), tensor(a[5]),
                                     optional(a[6]), optional(a[7]), optional(a[8]), optional(a[9]), a[10] == Py_True,
                                     optional(a[11]), optional(a[12]), number(a[13]), number(a[14])))
@@ -679,7 +712,7 @@ PyObject* py_set_workspaces(PyObject*, PyObject* d) {
 PyMethodDef methods[] = {METHOD(dense),     METHOD(kivi),   METHOD(kivi_pack), METHOD(pq_fused),
                          METHOD(pq_asym),   METHOD(pq_paged), METHOD(pq_encode), METHOD(score_into), METHOD(topk),
                          METHOD(gather),    METHOD(sparse_decode), METHOD(token_topk), METHOD(quest),
-                         METHOD(paged_append), METHOD(paged_decode),
+                         METHOD(paged_append), METHOD(paged_decode), METHOD(paged_quest),
                          {"set_workspaces", py_set_workspaces, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the operators.", -1, methods};

@@ -32,10 +32,11 @@ __device__ __forceinline__ int paged_len(const PagedKv& c, int b) {
 __device__ __forceinline__ float nan_min(float a, float b) { return (a < b || a != a) ? a : b; }
 __device__ __forceinline__ float nan_max(float a, float b) { return (a > b || a != a) ? a : b; }
 
-// Host-side checks of a cache's shape; 0 or a hipError_t.
+// Host-side checks of a cache's shape; 0 or a hipError_t.  (Positions up to 2^30:
+// sums of two stay in 32 bits.)
 inline int paged_check(int block_size, int num_blocks, int width) {
   if (block_size <= 0 || num_blocks <= 0 || width < 0) return (int)hipErrorInvalidValue;
-  if ((int64_t)width * block_size > 0x7FFFFFFF - 1024) return (int)hipErrorInvalidConfiguration;
+  if (block_size > (1 << 30) || (int64_t)width * block_size > (1 << 30)) return (int)hipErrorInvalidConfiguration;
   return 0;
 }
 
@@ -245,6 +246,50 @@ __device__ __forceinline__ void paged_store(uint16_t* out, const f32x4& A, float
     r[j] = (uint32_t)f32_to_bf16_bits(L == 0.f ? 0.f : A[2 * j] * il) |
            ((uint32_t)f32_to_bf16_bits(L == 0.f ? 0.f : A[2 * j + 1] * il) << 16);
   *reinterpret_cast<u32x2*>(out) = r;
+}
+
+// Join of a row's parts by one wave: 16 lanes hold a part's dims (64 of them), the
+// four lane groups take the parts in turn, each in order, and are folded by fixed
+// row swaps.  slot(i): part i's place; pml: (maximum, denominator) by place; pacc:
+// the lane's four values of place 0, places `pitch` apart.  The first 4 * PF parts
+// and their statistics are loaded together, one round trip.
+template <int PF, class SLOT, class PUT>
+__device__ __forceinline__ void paged_join(int parts, int lane, const SLOT& slot, const float2* pml, const f32x4* pacc,
+                                           int pitch, const PUT& put) {
+  const int grp = lane >> 4;
+  float2 ml[PF];
+  f32x4 acc[PF];
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {                   // parts past the last: its values again, with weight 0
+    const size_t r = slot(min(grp + 4 * u, parts - 1));
+    ml[u] = pml[r];
+    acc[u] = pacc[r * pitch];
+  }
+  float M = kNegInf;
+#pragma unroll
+  for (int u = 0; u < PF; ++u) M = fmaxf(M, ml[u].x);
+  for (int i = 4 * PF + lane; i < parts; i += 64) M = fmaxf(M, pml[slot(i)].x);
+  M = wave_max_f32(M);
+  if (M == kNegInf) M = 0.f;
+  float L = 0.f;
+  f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int u = 0; u < PF; ++u) {
+    const float f = grp + 4 * u < parts ? fast_exp2(ml[u].x - M) : 0.f;
+    L += f * ml[u].y;
+    A += f * acc[u];
+  }
+  for (int i = 4 * PF + grp; i < parts; i += 4) {
+    const size_t r = slot(i);
+    const float2 m = pml[r];
+    const float f = fast_exp2(m.x - M);
+    L += f * m.y;
+    A += f * pacc[r * pitch];
+  }
+  L = col_sum4(L);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) A[j] = col_sum4(A[j]);
+  put(A, L);
 }
 
 }  // namespace bytes_amd

@@ -147,13 +147,10 @@ __global__ __launch_bounds__(kDenseWaves * 64, 2) void paged_decode_kernel(Paged
 }
 
 // Joins the parts of each unit that more than one workgroup had: one wave per
-// (sequence, query head, 64 dims).  16 lanes hold a part's dims; the four lane
-// groups take the parts in turn, each in token order, and are folded by fixed row
-// swaps.  The first 32 parts and their statistics are loaded together, one round
-// trip.
+// (sequence, query head, 64 dims).
 template <int D>
 __global__ __launch_bounds__(64) void paged_join_kernel(PagedDecodeArgs a) {
-  constexpr int NSL = D / 64, PF = 8;
+  constexpr int NSL = D / 64;
   const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
   const int slice = blockIdx.x % NSL, h = blockIdx.x / NSL, b = blockIdx.y;     // h: query head
   const BatchGranules all(a, lane);
@@ -165,41 +162,11 @@ __global__ __launch_bounds__(64) void paged_join_kernel(PagedDecodeArgs a) {
   const int parts = w1 - w0 + 1;
   const int slot0 = all.start(a, w0) == s ? 0 : 1;
   auto slot = [&](int i) { return ((size_t)(w0 + i) * 2 + (i == 0 ? slot0 : 0)) * 16 + hl; };
-  const float2* pml = reinterpret_cast<const float2*>(a.part_ml);
-  const f32x4* pacc = reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item;
-  float2 ml[PF];
-  f32x4 acc[PF];
-#pragma unroll
-  for (int u = 0; u < PF; ++u) {                   // parts past the last: its values again, with weight 0
-    const size_t r = slot(min(grp + 4 * u, parts - 1));
-    ml[u] = pml[r];
-    acc[u] = pacc[r * (D / 4)];
-  }
-  float M = kNegInf;
-#pragma unroll
-  for (int u = 0; u < PF; ++u) M = fmaxf(M, ml[u].x);
-  for (int i = 4 * PF + lane; i < parts; i += 64) M = fmaxf(M, pml[slot(i)].x);
-  M = wave_max_f32(M);
-  if (M == kNegInf) M = 0.f;
-  float L = 0.f;
-  f32x4 A = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int u = 0; u < PF; ++u) {
-    const float f = grp + 4 * u < parts ? fast_exp2(ml[u].x - M) : 0.f;
-    L += f * ml[u].y;
-    A += f * acc[u];
-  }
-  for (int i = 4 * PF + grp; i < parts; i += 4) {
-    const size_t r = slot(i);
-    const float2 m = pml[r];
-    const float f = fast_exp2(m.x - M);
-    L += f * m.y;
-    A += f * pacc[r * (D / 4)];
-  }
-  L = col_sum4(L);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) A[j] = col_sum4(A[j]);
-  if (grp == 0) paged_store(a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
+  paged_join<8>(parts, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
+                reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4, [&](const f32x4& A, float L) {
+                  if (grp == 0) paged_store(a.out + (int64_t)b * a.o_sb + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L,
+                                            a.v_scale);
+                });
 }
 
 // Workgroups of the decode grid: one per CU, whose four waves' tiles in flight

@@ -28,7 +28,7 @@ import torch
 
 from . import _checks as C
 from ._lib import call, native, ptr, size_query, stream_of
-from .sparse import topk_indices
+from .sparse import _topk
 
 _F8 = torch.float8_e4m3fn
 Meta = Tuple[torch.Tensor, torch.Tensor]
@@ -78,8 +78,8 @@ def _tables(block_table: torch.Tensor, context_lens: torch.Tensor, B: int, bs: i
                          f"{tuple(block_table.shape)}, {tuple(context_lens.shape)}")
     if block_table.shape[1] == 0:
         raise ValueError("block_table has no columns")
-    if block_table.shape[1] * bs > 2 ** 31 - 1 - 1024:
-        raise ValueError(f"block_table names {block_table.shape[1]} blocks of {bs} tokens: positions pass 32 bits")
+    if block_table.shape[1] * bs > 2 ** 30:
+        raise ValueError(f"block_table names {block_table.shape[1]} blocks of {bs} tokens: more than 2^30 positions")
     bt = _int32(block_table, "block_table")
     if bt.stride(-1) != 1 and bt.shape[1] > 1:
         bt = bt.contiguous()
@@ -244,20 +244,29 @@ def paged_page_scores(q: torch.Tensor, meta: Meta, block_table: torch.Tensor, co
     C.cuda_tensors(q, *meta, block_table, context_lens)
     C.ndim(meta[0], 3, "kmin")
     N, Hk, D = meta[0].shape
-    if N == 0 or Hk == 0 or int(block_size) < 1 or int(local_w) < 0:
-        raise ValueError(f"bad metadata / block_size / local_w: {tuple(meta[0].shape)}, {block_size}, {local_w}")
+    if N == 0 or Hk == 0 or int(block_size) < 1:
+        raise ValueError(f"bad metadata / block_size: {tuple(meta[0].shape)}, {block_size}")
     if D not in (64, 128):
         raise ValueError(f"head_dim {D} not supported (64 or 128)")
     kmin, kmax = _meta(meta, N, Hk, D)
     qs, B, Hq = _query(q, Hk, D)
     bt, cl = _tables(block_table, context_lens, B, int(block_size))
-    W = bt.shape[1]
-    with torch.cuda.device(q.device):
-        bound = torch.empty((B, Hq, W), dtype=torch.float32, device=q.device)
+    return _page_scores(qs, kmin, kmax, bt, cl, int(block_size), float(scaling), local_w, -1)
+
+
+def _page_scores(qs, kmin, kmax, bt, cl, bs: int, scale: float, local_w: int, skip: int) -> torch.Tensor:
+    if int(local_w) < 0:
+        raise ValueError(f"local_w={local_w} is negative")
+    (B, Hq, D), (N, Hk, _), W = qs.shape, kmin.shape, bt.shape[1]
+    with torch.cuda.device(qs.device):
+        bound = torch.empty((B, Hq, W), dtype=torch.float32, device=qs.device)
         call("bytes_paged_page_scores", ptr(qs), qs.stride(0), qs.stride(1), ptr(kmin), ptr(kmax), ptr(bt), bt.stride(0),
-             ptr(cl), ptr(bound), bound.stride(0), bound.stride(1), B, Hq, Hk, D, int(block_size), N, W, int(local_w),
-             float(scaling), stream_of(q))
+             ptr(cl), ptr(bound), bound.stride(0), bound.stride(1), B, Hq, Hk, D, bs, N, W, min(int(local_w), 2 ** 30),
+             skip, scale, stream_of(qs))
     return bound
+
+
+_SELECT_IN_KERNEL_MAX = 4096        # blocks of a sequence that the attention kernel selects from itself
 
 
 def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Tensor, meta: Meta,
@@ -271,22 +280,36 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     bf16 (and the selected blocks' places in the table, int32
     [B,H_q,min(ceil(kb / block_size), max_blocks)] ascending, if return_pages;
     places past a short sequence's blocks stand for nothing)."""
+    if not return_pages:
+        out = native().paged_quest(q, k_paged, v_paged, *meta, block_table, context_lens, kb, scaling, local_w, k_scale,
+                                   v_scale)
+        if out is not None:
+            return out
     C.cuda_tensors(q, k_paged, v_paged, *meta, block_table, context_lens)
     N, Hk, bs, D, fp8 = _cache(k_paged, v_paged, k_scale, v_scale)
     if kb < 1:
         raise ValueError(f"kb={kb} must be at least 1")
     qs, B, Hq = _query(q, Hk, D)
     bt, cl = _tables(block_table, context_lens, B, bs)
+    kmin, kmax = _meta(meta, N, Hk, D)
     W = bt.shape[1]
-    bound = paged_page_scores(q, _meta(meta, N, Hk, D), bt, cl, bs, float(scaling) * float(k_scale), local_w=local_w)
     npick = min((int(kb) + bs - 1) // bs, W)
+    scale = float(scaling) * float(k_scale)
+    listed = return_pages or W > _SELECT_IN_KERNEL_MAX
+    bound = _page_scores(qs, kmin, kmax, bt, cl, bs, scale, local_w, -1 if listed else npick)
     with torch.cuda.device(q.device):
-        pages = topk_indices(bound, npick, sorted=False)
+        pages = None
+        if listed:                               # with a top-k workspace of the call's own, as all else here
+            n = size_query("bytes_topk_workspace_size", B * Hq, W, npick)
+            pages = _topk(bound, npick, sorted=False, ws=torch.zeros(max(n, 16), dtype=torch.uint8, device=q.device))
         out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device)
-        call("bytes_paged_pick_attn", ptr(qs), qs.stride(0), qs.stride(1),
+        n = size_query("bytes_paged_quest_workspace_size", B, Hq, Hk, D, bs, npick)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+        call("bytes_paged_quest_attn", ptr(qs), qs.stride(0), qs.stride(1),
              ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),
              ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), int(fp8),
-             ptr(pages), pages.stride(0), pages.stride(1), npick, ptr(bt), bt.stride(0), ptr(cl), ptr(out),
-             out.stride(0), out.stride(1), B, Hq, Hk, D, bs, N, W, float(scaling) * float(k_scale), float(v_scale),
-             None, 0, stream_of(q))
+             None if listed else ptr(bound), bound.stride(0), bound.stride(1),
+             ptr(pages) if listed else None, pages.stride(0) if listed else 0, pages.stride(1) if listed else 0, npick,
+             ptr(bt), bt.stride(0), ptr(cl), ptr(out), out.stride(0), out.stride(1), B, Hq, Hk, D, bs, N, W, scale,
+             float(v_scale), ptr(ws), ws.numel(), stream_of(q))
     return (out.unsqueeze(2), pages) if return_pages else out.unsqueeze(2)

@@ -483,7 +483,7 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  * block_size.  Block ids outside [0, num_blocks) name no block: nothing is
  * written for their tokens, and they take no part.  Lengths, tables and
  * cu_seqlens are device memory, read when the kernels run.  D in {64, 128};
- * max_blocks * block_size < 2^31 - 1024.
+ * max_blocks * block_size <= 2^30.
  *
  * bytes_paged_kv_append: k, v [T, Hk, D] bf16 (strides *_st, *_sh), the new
  *   tokens of B sequences: rows cu_seqlens[b] .. cu_seqlens[b + 1], or row b
@@ -502,12 +502,19 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  *   where none does; q [B, Hq, D] bf16.  (scale includes the cache's k_scale.)
  *   Workspace: bytes_paged_decode_workspace_size, contents arbitrary.
  * bytes_paged_page_scores: bound [B, Hq, max_blocks] fp32 (strides b_sb, b_sh)
- *   = scale * sum_d q_d * (q_d >= 0 ? kmax_d : kmin_d) of block table entries,
- *   summed in fp64 and rounded once; -inf where a block holds no token that
- *   takes part, +inf where it reaches into the last local_w tokens.
- * bytes_paged_pick_attn: bytes_paged_decode_attn over the tokens of the blocks
- *   at places pages [B, Hq, npick] (int32, strides p_sb, p_sh, each place at
- *   most once) of the table; places outside the sequence stand for nothing.
+ *   = scale * sum_d q_d * (q_d >= 0 ? kmax_d : kmin_d) of the block table's
+ *   entries, summed in fp64 and rounded once; -inf where a block holds no token
+ *   that takes part, +inf where it reaches into the last local_w tokens.
+ *   Sequences of at most `skip` blocks are left out (-1: none; their bounds are
+ *   not written).
+ * bytes_paged_quest_attn: bytes_paged_decode_attn over the tokens of npick
+ *   blocks per query head: the best of bound (as bytes_paged_page_scores gives
+ *   them, skip <= npick; bound descending, lowest place first on equal bounds;
+ *   max_blocks <= 4096, hipErrorNotSupported above; sequences of at most npick
+ *   blocks whole), or, where bound is NULL, those at places pages [B, Hq, npick]
+ *   (int32, strides p_sb, p_sh, no place twice; places outside the sequence
+ *   stand for nothing).  Workspace: bytes_paged_quest_workspace_size, contents
+ *   arbitrary.
  * ------------------------------------------------------------------------- */
 int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                           const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
@@ -526,13 +533,15 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
 int bytes_paged_page_scores(const void* q, int64_t q_sb, int64_t q_sh, const void* kmin, const void* kmax,
                             const void* block_table, int64_t bt_sb, const void* context_lens, void* bound, int64_t b_sb,
                             int64_t b_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
-                            int local_w, double scale, void* stream);
-int bytes_paged_pick_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
-                          int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
-                          const void* pages, int64_t p_sb, int64_t p_sh, int npick, const void* block_table,
-                          int64_t bt_sb, const void* context_lens, void* out, int64_t o_sb, int64_t o_sh, int B, int Hq,
-                          int Hk, int D, int block_size, int num_blocks, int max_blocks, float scale, float v_scale,
-                          void* workspace, size_t workspace_bytes, void* stream);
+                            int local_w, int skip, double scale, void* stream);
+int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int block_size, int npick, size_t* bytes);
+int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
+                           int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
+                           const void* bound, int64_t b_sb, int64_t b_sh, const void* pages, int64_t p_sb, int64_t p_sh,
+                           int npick, const void* block_table, int64_t bt_sb, const void* context_lens, void* out,
+                           int64_t o_sb, int64_t o_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks,
+                           int max_blocks, float scale, float v_scale, void* workspace, size_t workspace_bytes,
+                           void* stream);
 
 #ifdef __cplusplus
 }  /* extern "C" */
