@@ -32,6 +32,21 @@ __device__ __forceinline__ int paged_len(const PagedKv& c, int b) {
 __device__ __forceinline__ float nan_min(float a, float b) { return (a < b || a != a) ? a : b; }
 __device__ __forceinline__ float nan_max(float a, float b) { return (a > b || a != a) ? a : b; }
 
+// Folds v over the lanes that hold the same part of other rows, LPR lanes to a row:
+// rotations within the rows of 16, then the row and half swaps.  Every lane of the
+// wave takes part and receives the result.
+template <int LPR, class OP>
+__device__ __forceinline__ float fold_rows(float v, OP op) {
+  if (LPR <= 8)
+    v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x128, 0xF, 0xF, false)));
+  if (LPR <= 4)
+    v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x124, 0xF, 0xF, false)));
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 // Host-side checks of a cache's shape; 0 or a hipError_t.  (Positions up to 2^30:
 // sums of two stay in 32 bits.)
 inline int paged_check(int block_size, int num_blocks, int width) {

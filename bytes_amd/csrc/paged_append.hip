@@ -176,19 +176,6 @@ __device__ __forceinline__ char* cache_row(const void* base, int64_t sb, int64_t
 __device__ __forceinline__ float lower(float a, float b) { return __builtin_elementwise_minimum(a, b); }
 __device__ __forceinline__ float upper(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Folds v over the lanes that hold the same item of other rows (lane bits from
-// log2(LPR) up): rotations within the rows of 16, then the row and half swaps.
-template <int LPR, class OP>
-__device__ __forceinline__ float fold_rows(float v, OP op) {
-  v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x128, 0xF, 0xF, false)));
-  if (LPR == 4)
-    v = op(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), 0x124, 0xF, 0xF, false)));
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return op(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 // One token of one sequence per wave and up to 64 / LPR of its heads' rows.
 template <int D, bool FP8>
 __global__ __launch_bounds__(kAppendWaves * 64) void paged_append_one_kernel(AppendArgs a) {

@@ -303,7 +303,7 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
             n = size_query("bytes_topk_workspace_size", B * Hq, W, npick)
             pages = _topk(bound, npick, sorted=False, ws=torch.zeros(max(n, 16), dtype=torch.uint8, device=q.device))
         out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device)
-        n = size_query("bytes_paged_quest_workspace_size", B, Hq, Hk, D, bs, npick)
+        n = size_query("bytes_paged_quest_workspace_size", B, Hq, Hk, D, int(fp8), bs, npick)
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
         call("bytes_paged_quest_attn", ptr(qs), qs.stride(0), qs.stride(1),
              ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),

@@ -534,7 +534,8 @@ int bytes_paged_page_scores(const void* q, int64_t q_sb, int64_t q_sh, const voi
                             const void* block_table, int64_t bt_sb, const void* context_lens, void* bound, int64_t b_sb,
                             int64_t b_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
                             int local_w, int skip, double scale, void* stream);
-int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int block_size, int npick, size_t* bytes);
+int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int npick,
+                                     size_t* bytes);
 int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
                            int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
                            const void* bound, int64_t b_sb, int64_t b_sh, const void* pages, int64_t p_sb, int64_t p_sh,
