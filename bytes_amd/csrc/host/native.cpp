@@ -557,7 +557,7 @@ Tensor paged_quest(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   c10::DeviceGuard guard(q.device());
   size_t n = 0;
   need(bytes_paged_quest_workspace_size(B, Hq, p.Hk, p.D, p.f8, p.bs, npick, &n) == 0);
-  const Tensor bound = empty(q, {B, Hq, p.W}, at::kFloat);
+  const Tensor bound = empty(q, {B, Hq, (p.W + 3) / 4 * 4}, at::kFloat);       // rows of whole 16-byte chunks
   const Tensor w = empty(q, {(int64_t)n}, at::kByte);
   Tensor out = empty(q, {B, Hq, 1, p.D}, at::kBFloat16);
   const double scale = scaling * ks;

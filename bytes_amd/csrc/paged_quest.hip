@@ -162,6 +162,7 @@ struct PagedQuestArgs {
   float* part_acc;                   // [B * Hq][nsplit][D]
   float* part_ml;                    // [B * Hq][nsplit][2]
   int Hq, G, npick, chunk, nsplit, nwg;
+  int b_vec;                         // bound rows are whole 16-byte chunks
   FastDiv dsplit, dHq, dG;
   float scale_log2, v_scale;
 };
@@ -180,14 +181,26 @@ struct PickCfg {
 };
 
 // Selection of the k best of n bounds (k < n <= 256 * PER): put(rank in ascending place order, place).
+// vec: the row starts on a 16-byte boundary and its storage ends on one.
 template <int PER, class PUT>
-__device__ __forceinline__ void pick_blocks(const float* bound, int n, int k, uint32_t* ws, const PUT& put) {
+__device__ __forceinline__ void pick_blocks(const float* bound, bool vec, int n, int k, uint32_t* ws, const PUT& put) {
   uint32_t key[PER];
-  float v[PER];
+  if (vec) {
+    u32x4 v[PER / 4];
 #pragma unroll
-  for (int u = 0; u < PER; ++u) v[u] = bound[min(PER * (int)threadIdx.x + u, n - 1)];
+    for (int u = 0; u < PER / 4; ++u) v[u] = ld16(bound + 4 * min(PER / 4 * (int)threadIdx.x + u, (n - 1) / 4));
 #pragma unroll
-  for (int u = 0; u < PER; ++u) key[u] = score_order_key(v[u]);
+    for (int u = 0; u < PER; ++u) {
+      const uint32_t x = v[u / 4][u % 4];
+      key[u] = score_order_key(__uint_as_float(x));
+    }
+  } else {
+    float v[PER];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) v[u] = bound[min(PER * (int)threadIdx.x + u, n - 1)];
+#pragma unroll
+    for (int u = 0; u < PER; ++u) key[u] = score_order_key(v[u]);
+  }
   const BlockSel sel = block_select<kPickThreads, PER>(key, n, k, ws);
   block_select_emit<kPickThreads, PER>(key, n, sel, ws, [&](uint32_t pos, int idx, uint32_t) { put((int)pos, idx); });
 }
@@ -277,9 +290,10 @@ __global__ __launch_bounds__(kPickThreads, 4) void paged_quest_kernel(PagedQuest
   };
   if (a.bound && full > a.npick) {
     const float* bound = a.bound + (int64_t)b * a.b_sb + (int64_t)h * a.b_sh;
-    if (full <= 4 * kPickThreads) pick_blocks<4>(bound, full, a.npick, work, put);
-    else if (full <= 8 * kPickThreads) pick_blocks<8>(bound, full, a.npick, work, put);
-    else pick_blocks<16>(bound, full, a.npick, work, put);
+    const bool vec = a.b_vec != 0;
+    if (full <= 4 * kPickThreads) pick_blocks<4>(bound, vec, full, a.npick, work, put);
+    else if (full <= 8 * kPickThreads) pick_blocks<8>(bound, vec, full, a.npick, work, put);
+    else pick_blocks<16>(bound, vec, full, a.npick, work, put);
   } else {
     const int32_t* pages = a.pages + b * a.p_sb + h * a.p_sh;
     for (int i = i0 + threadIdx.x; i < i1; i += kPickThreads) put(i, a.bound ? i : pages[i]);
@@ -511,6 +525,7 @@ int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void
   a.c.dbs = make_fastdiv((uint32_t)block_size);
   a.q = static_cast<const uint16_t*>(q), a.q_sb = q_sb, a.q_sh = q_sh;
   a.bound = static_cast<const float*>(bound), a.b_sb = b_sb, a.b_sh = b_sh;
+  a.b_vec = reinterpret_cast<uintptr_t>(bound) % 16 == 0 && b_sb % 4 == 0 && b_sh % 4 == 0 && b_sh >= (max_blocks + 3) / 4 * 4;
   a.pages = static_cast<const int32_t*>(pages), a.p_sb = p_sb, a.p_sh = p_sh;
   a.out = static_cast<uint16_t*>(out), a.o_sb = o_sb, a.o_sh = o_sh;
   a.Hq = Hq, a.G = Hq / Hk, a.npick = npick;

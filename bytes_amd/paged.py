@@ -259,7 +259,8 @@ def _page_scores(qs, kmin, kmax, bt, cl, bs: int, scale: float, local_w: int, sk
         raise ValueError(f"local_w={local_w} is negative")
     (B, Hq, D), (N, Hk, _), W = qs.shape, kmin.shape, bt.shape[1]
     with torch.cuda.device(qs.device):
-        bound = torch.empty((B, Hq, W), dtype=torch.float32, device=qs.device)
+        # rows that a kernel reads on are whole 16-byte chunks
+        bound = torch.empty((B, Hq, W if skip < 0 else (W + 3) // 4 * 4), dtype=torch.float32, device=qs.device)
         call("bytes_paged_page_scores", ptr(qs), qs.stride(0), qs.stride(1), ptr(kmin), ptr(kmax), ptr(bt), bt.stride(0),
              ptr(cl), ptr(bound), bound.stride(0), bound.stride(1), B, Hq, Hk, D, bs, N, W, min(int(local_w), 2 ** 30),
              skip, scale, stream_of(qs))
