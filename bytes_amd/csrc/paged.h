@@ -167,6 +167,64 @@ struct PagedRows {
   }
 };
 
+// One staged tile: scores, online softmax and values, as dense_compute, with each
+// weight as the sum of two bf16 numbers (2^-17 of it is lost and not 2^-9): a
+// second product per value block, whose matrix instructions have time to spare
+// here.  Error of a long context's output against 64 bits: 0.0023 of its norm with
+// one, 0.0017, the rounding of the result itself, with two.
+template <int D>
+__device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int lane, const bf16x8 (&qb)[D / 32],
+                                           const char* kst, const char* vst, float& m_run, float& l_run,
+                                           f32x4 (&acc)[D / 16]) {
+  using C = DenseCfg<D>;
+  const int l16 = lane & 15, lg = lane >> 4;
+  f32x4 s[2];
+#pragma unroll
+  for (int blk = 0; blk < 2; ++blk) {
+    s[blk] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int row = blk * 16 + l16;
+#pragma unroll
+    for (int kk = 0; kk < C::KK; ++kk) {
+      const bf16x8 ka = __builtin_bit_cast(
+          bf16x8, *reinterpret_cast<const u32x4*>(kst + row * (D * 2) + kswz<D>(row, kk * 4 + lg) * 16));
+      s[blk] = mfma_bf16(ka, qb[kk], s[blk]);
+    }
+  }
+  float x[8], mx = kNegInf;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    x[j] = ((vmask >> ((j >> 2) * 16 + lg * 4 + (j & 3))) & 1u) ? s[j >> 2][j & 3] * scale_log2 : kNegInf;
+    mx = __builtin_elementwise_maximum(mx, x[j]);
+  }
+  mx = col_max4(mx);
+  const float m_new = fmaxf(m_run, mx);
+  const float m_use = (m_new == kNegInf) ? 0.f : m_new;
+  const float alpha = fast_exp2(m_run - m_use);
+  float psum = 0.f;
+  bf16x8 hi, lo;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float p = fast_exp2(x[j] - m_use);
+    psum += p;
+    hi[j] = (__bf16)p;
+    lo[j] = (__bf16)(p - (float)hi[j]);
+  }
+  l_run = l_run * alpha + psum;
+  m_run = m_new;
+  // V^T through two transposed reads per block of 16 dims (tile_softmax_pv_at's layout)
+  const StagedV<D> vaddr{vst};
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db) {
+    acc[db] *= alpha;
+    u32x2 h[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) h[hf] = tr16(vaddr(hf, hf * 16 + lg * 4 + (l16 >> 2), db * 16 + (l16 & 3) * 4));
+    const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{h[0][0], h[0][1], h[1][0], h[1][1]});
+    acc[db] = mfma_bf16(v, hi, acc[db]);
+    acc[db] = mfma_bf16(v, lo, acc[db]);
+  }
+}
+
 // Slots [s, s_end) in steps of `step` (s a multiple of 32 from the first slot):
 // online softmax over them into m_run, l_run, acc.
 template <int D, bool FP8, bool HALVES, class FIND>
@@ -205,7 +263,7 @@ __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t*
     next = fetch(s + 2 * step);
     rows.issue(now, s + step < s_end);
     wave_lds_sync();
-    dense_compute<D>(vmask, scale_log2, lane, qb, kst, vst, m_run, l_run, acc);
+    paged_tile<D>(vmask, scale_log2, lane, qb, kst, vst, m_run, l_run, acc);
   }
 }
 

@@ -512,10 +512,10 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  *   them, skip <= npick; bound descending, lowest place first on equal bounds;
  *   max_blocks <= 4096, hipErrorNotSupported above; sequences of at most npick
  *   blocks whole; where b_sb, b_sh are multiples of 4 and b_sh at least
- *   max_blocks rounded up to one, rows are read in whole 16-byte chunks), or, where bound is NULL, those at places pages [B, Hq, npick]
- *   (int32, strides p_sb, p_sh, no place twice; places outside the sequence
- *   stand for nothing).  Workspace: bytes_paged_quest_workspace_size, contents
- *   arbitrary.
+ *   max_blocks rounded up to one, rows are read in whole 16-byte chunks), or,
+ *   where bound is NULL, those at places pages [B, Hq, npick] (int32, strides
+ *   p_sb, p_sh, no place twice; places outside the sequence stand for nothing).
+ *   Workspace: bytes_paged_quest_workspace_size, contents arbitrary.
  * ------------------------------------------------------------------------- */
 int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                           const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,

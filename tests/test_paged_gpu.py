@@ -259,10 +259,11 @@ def test_append_in_pieces_equals_at_once(dev, fp8):
 # decode
 # ---------------------------------------------------------------------------
 def _tol(out, mag, dots, D):
-    """|error| of a decode's output: half a bf16 step of the result; half a bf16 step on each
-    weight (2^-8 of the weighted |v|); scores off by D roundings of 2^-24 of their
-    products, twice (numerator and denominator); fp32 sums and exponentials 2^-16."""
-    return 2.0 ** -8 * out.abs() + mag * (2.0 ** -8 + 2 * D * 2.0 ** -24 * dots + 2.0 ** -16)
+    """|error| of a decode's output: half a bf16 step of the result; weights as sums of two
+    bf16 numbers, each rounding at most 2^-8 of what it rounds (2^-16 of the weighted |v|);
+    scores off by D roundings of 2^-24 of their products, twice (numerator and
+    denominator); fp32 sums and exponentials 2^-16."""
+    return 2.0 ** -8 * out.abs() + mag * (2.0 ** -16 + 2 * D * 2.0 ** -24 * dots + 2.0 ** -16)
 
 
 def _check_decode(dev, got, q, kc, vc, scale, ks, vs, table, lens, picks=None):
