@@ -155,7 +155,7 @@ SIGNATURES: Dict[str, Tuple] = {
         c_f32, c_f32,                                            # k_scale, v_scale
         c_int, c_int, c_int, c_int, c_int,                       # T, B, Hq, Hk, D
         c_int, c_int, c_int, c_vp),                              # block size, blocks, max blocks, stream
-    "bytes_paged_decode_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
+    "bytes_paged_decode_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
     "bytes_paged_decode_attn": (
         c_vp, c_i64, c_i64,                                      # q, strides (b, h)
         c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)

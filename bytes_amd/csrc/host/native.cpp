@@ -532,14 +532,15 @@ Tensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   const Paged p = paged(k, v, bt, cl, B, ks, vs);
   c10::DeviceGuard guard(q.device());
   size_t n = 0;
-  need(bytes_paged_decode_workspace_size(B, Hq, p.Hk, p.D, p.bs, p.W, &n) == 0);
-  const Tensor w = empty(q, {(int64_t)n}, at::kByte);    // the call's own: calls on other streams share nothing
+  need(bytes_paged_decode_workspace_size(B, Hq, p.Hk, p.D, p.f8, p.bs, p.W, &n) == 0);
+  Tensor w;                                              // the call's own: calls on other streams share nothing
+  if (n) w = empty(q, {(int64_t)n}, at::kByte);
   Tensor out = empty(q, {B, Hq, 1, p.D}, at::kBFloat16);
   void* st = stream_of(q);
   launch("bytes_paged_decode_attn", bytes_paged_decode_attn, data(q), q.stride(0), q.stride(1), data(k), k.stride(0),
          k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), p.f8, data(bt), bt.stride(0), data(cl),
          out.mutable_data_ptr(), out.stride(0), out.stride(1), B, Hq, p.Hk, p.D, p.bs, p.N, p.W, (float)(scale * ks),
-         (float)vs, w.mutable_data_ptr(), n, st);
+         (float)vs, n ? w.mutable_data_ptr() : nullptr, n, st);
   return out;
 }
 
@@ -558,7 +559,8 @@ Tensor paged_quest(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   size_t n = 0;
   need(bytes_paged_quest_workspace_size(B, Hq, p.Hk, p.D, p.f8, p.bs, npick, &n) == 0);
   const Tensor bound = empty(q, {B, Hq, (p.W + 3) / 4 * 4}, at::kFloat);       // rows of whole 16-byte chunks
-  const Tensor w = empty(q, {(int64_t)n}, at::kByte);
+  Tensor w;
+  if (n) w = empty(q, {(int64_t)n}, at::kByte);
   Tensor out = empty(q, {B, Hq, 1, p.D}, at::kBFloat16);
   const double scale = scaling * ks;
   void* st = stream_of(q);

@@ -271,10 +271,10 @@ __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t*
 // with four consecutive dims 4 * d4 .. of head h < nh, the maximum (log2 domain)
 // and the denominator.  All threads of the workgroup call this; smem is free
 // again when it returns.
-template <int D, class PUT>
+template <int D, int NW, class PUT>
 __device__ __forceinline__ void paged_merge_waves(float m_run, float l_run, f32x4 (&acc)[D / 16], float* smem, int nh,
                                                   const PUT& put) {
-  constexpr int NW = kDenseWaves, P = acc_pitch<D>(), D4 = D / 4;
+  constexpr int P = acc_pitch<D>(), D4 = D / 4;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, l16 = lane & 15, lg = lane >> 4;
   l_run = col_sum4(l_run);
   float* wm = smem;

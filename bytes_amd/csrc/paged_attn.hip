@@ -17,6 +17,8 @@
 // last) leave (max, sum, values) in fp32 for the second launch, which joins each
 // unit's parts in token order.  So the work per workgroup differs by at most one
 // granule whatever the lengths, and the result does not depend on timing.
+// Tables that hold short contexts only take a workgroup per unit and no second
+// launch (short_waves).
 #include "paged.h"
 
 namespace bytes_amd {
@@ -33,7 +35,7 @@ struct PagedDecodeArgs {
   float* part_ml;                    // [workgroup][2][16][2]
   int B, Hk, HB, G, U;               // U = Hk * HB units per sequence
   int nwg;
-  FastDiv dnwg, dhb, dG;
+  FastDiv dnwg, dhb, dG, dU;
   float scale_log2, v_scale;
 };
 
@@ -125,7 +127,7 @@ __global__ __launch_bounds__(kDenseWaves * 64, 2) void paged_decode_kernel(Paged
     const bool whole = m == n;
     uint16_t* out = a.out + (int64_t)b * a.o_sb + (int64_t)hq0 * a.o_sh;
     const size_t slot = ((size_t)blockIdx.x * 2 + (g == g0 ? 0 : 1)) * 16;
-    paged_merge_waves<D>(m_run, l_run, acc, reinterpret_cast<float*>(smem), nh,
+    paged_merge_waves<D, kDenseWaves>(m_run, l_run, acc, reinterpret_cast<float*>(smem), nh,
                          [&](int h, int d4, const f32x4& A, float M, float L) {
                            if (whole) {
                              paged_store(out + (int64_t)h * a.o_sh + 4 * d4, A, L, a.v_scale);
@@ -144,6 +146,37 @@ __global__ __launch_bounds__(kDenseWaves * 64, 2) void paged_decode_kernel(Paged
       n = granules(len);
     }
   }
+}
+
+// Short contexts: a workgroup of NW waves per unit, which it finishes itself.
+template <int D, bool FP8, bool HALVES, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_decode_short_kernel(PagedDecodeArgs a) {
+  using C = DenseCfg<D>;
+  static_assert(NW * C::WAVE >= splitk_smem_floats<D, NW>() * 4, "the merge fits the tile buffers");
+  __shared__ __attribute__((aligned(16))) char smem[NW * C::WAVE];
+  PREFETCH_ARGS(a);
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = fast_div((int)blockIdx.x, a.dU), u = (int)blockIdx.x - b * a.U, hk = fast_div(u, a.dhb), hb = u - hk * a.HB;
+  const int hq0 = hk * a.G + hb * 16, nh = min(16, a.G - hb * 16);
+  const int len = __builtin_amdgcn_readfirstlane(paged_len(a.c, b));
+  bf16x8 qb[C::KK];
+  load_q_bf16<D>(a.q + (int64_t)b * a.q_sb + (int64_t)hq0 * a.q_sh, a.q_sh, nh, lane, qb);
+  float m_run = kNegInf, l_run = 0.f;
+  f32x4 acc[C::DB];
+#pragma unroll
+  for (int db = 0; db < C::DB; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto find = [&](int p, int& place, int& off, bool& ok) {
+    place = fast_div(p, a.c.dbs);
+    off = p - place * a.c.bs;
+    ok = true;
+  };
+  paged_wave_loop<D, FP8, HALVES>(a.c, a.c.table + (int64_t)b * a.c.bt_sb, hk, w * kTile, len, NW * kTile, lane,
+                                  a.scale_log2, qb, smem + w * C::WAVE, find, m_run, l_run, acc);
+  uint16_t* out = a.out + (int64_t)b * a.o_sb + (int64_t)hq0 * a.o_sh;
+  paged_merge_waves<D, NW>(m_run, l_run, acc, reinterpret_cast<float*>(smem), nh,
+                           [&](int h, int d4, const f32x4& A, float, float L) {
+                             paged_store(out + (int64_t)h * a.o_sh + 4 * d4, A, L, a.v_scale);
+                           });
 }
 
 // Joins the parts of each unit that more than one workgroup had: one wave per
@@ -181,6 +214,21 @@ static int decode_grid(int64_t units, int64_t granules_max) {
   return (int)(granules_max < n ? granules_max : n);
 }
 
+// Waves of a workgroup that does a whole unit by itself (one launch, no parts to
+// join), or 0 for the even split.  By the bytes of a full table row, which one CU
+// reads at about 50 GB/s: up to 256 KB (us, whole unit and split: one sequence of
+// 2 KV heads of 64, 500 tokens 5.7 and 7.1, 1000 tokens 8.0 and 7.1; of 4 heads of
+// 128, 500 tokens 7.8 and 8.3, 1000 tokens 13.4 and 8.9), twice that where the
+// units keep half the CUs busy anyway (64 sequences of 4 heads of 128, 500 tokens
+// 10.7 and 13.3, 1000 tokens 17.2 and 20.8).  Four waves where a tile each
+// covers the row, or where two workgroups to a CU have units enough (200 sequences
+// of 4 heads, 100 tokens: 15.8 with eight, 9.1 with four; split 18.0).
+static int short_waves(int64_t units, int64_t cap, int D, int fp8) {
+  const int64_t cus = device_cu_count(), bytes = cap * D * (fp8 ? 2 : 4);
+  if (bytes > (2 * units >= cus ? 512 << 10 : 256 << 10)) return 0;
+  return cap <= 4 * kTile || units >= 2 * cus ? 4 : 8;
+}
+
 struct DecodeShape {
   int64_t units, granules;           // of the batch, at most
 };
@@ -198,12 +246,14 @@ using namespace bytes_amd;
 
 extern "C" {
 
-int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int block_size, int max_blocks, size_t* bytes) {
+int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int max_blocks,
+                                      size_t* bytes) {
   if (!bytes || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128)) return (int)hipErrorInvalidValue;
   const int rc = paged_check(block_size, 1, max_blocks);
   if (rc) return rc;
   const DecodeShape s = decode_shape(B, Hq, Hk, block_size, max_blocks);
-  *bytes = decode_workspace(decode_grid(s.units, s.granules), D);
+  *bytes = short_waves(s.units, (int64_t)max_blocks * block_size, D, kv_fp8)
+               ? 0 : decode_workspace(decode_grid(s.units, s.granules), D);
   return 0;
 }
 
@@ -212,8 +262,8 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
                             const void* block_table, int64_t bt_sb, const void* context_lens, void* out, int64_t o_sb,
                             int64_t o_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
                             float scale, float v_scale, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!q || !k_paged || !v_paged || !block_table || !context_lens || !out || !workspace || B <= 0 || Hk <= 0 ||
-      Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128) || max_blocks <= 0)
+  if (!q || !k_paged || !v_paged || !block_table || !context_lens || !out || B <= 0 || Hk <= 0 || Hq <= 0 ||
+      Hq % Hk != 0 || (D != 64 && D != 128) || max_blocks <= 0)
     return (int)hipErrorInvalidValue;
   int rc = paged_check(block_size, num_blocks, max_blocks);
   if (rc) return rc;
@@ -231,13 +281,36 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
   a.B = B, a.Hk = Hk, a.G = Hq / Hk, a.HB = (a.G + 15) / 16, a.U = Hk * a.HB;
   a.nwg = decode_grid(shape.units, shape.granules);
   a.dnwg = make_fastdiv((uint32_t)a.nwg), a.dhb = make_fastdiv((uint32_t)a.HB), a.dG = make_fastdiv((uint32_t)a.G);
+  a.dU = make_fastdiv((uint32_t)a.U);
   a.scale_log2 = scale * kLog2e, a.v_scale = v_scale;
-  if (workspace_bytes < decode_workspace(a.nwg, D)) return (int)hipErrorInvalidValue;
+  const bool halves = paged_halves(a.c);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const int waves = short_waves(shape.units, (int64_t)max_blocks * block_size, D, kv_fp8);
+  if (waves) {
+    const dim3 ugrid((unsigned)shape.units);
+#define PW(DD, F8, H, N) hipLaunchKernelGGL((paged_decode_short_kernel<DD, F8, H, N>), ugrid, dim3(N * 64), 0, st, a)
+#define PW_N(DD, F8, H)                  \
+  if (waves == 4) PW(DD, F8, H, 4);      \
+  else PW(DD, F8, H, 8)
+#define PW_H(DD, F8)                  \
+  if (halves) { PW_N(DD, F8, true); } \
+  else { PW_N(DD, F8, false); }
+    if (D == 128) {
+      if (kv_fp8) { PW_H(128, true) }
+      else { PW_H(128, false) }
+    } else {
+      if (kv_fp8) { PW_H(64, true) }
+      else { PW_H(64, false) }
+    }
+#undef PW_H
+#undef PW_N
+#undef PW
+    return (int)hipGetLastError();
+  }
+  const dim3 grid((unsigned)a.nwg), block(kDenseWaves * 64);
+  if (!workspace || workspace_bytes < decode_workspace(a.nwg, D)) return (int)hipErrorInvalidValue;
   a.part_ml = static_cast<float*>(workspace);
   a.part_acc = a.part_ml + (size_t)a.nwg * 2 * 16 * 2;
-  const bool halves = paged_halves(a.c);
-  const dim3 grid((unsigned)a.nwg), block(kDenseWaves * 64);
-  hipStream_t st = static_cast<hipStream_t>(stream);
 #define PD(DD, F8, H) hipLaunchKernelGGL((paged_decode_kernel<DD, F8, H>), grid, block, 0, st, a)
 #define PD_H(DD, F8)       \
   if (halves) PD(DD, F8, true); \
@@ -252,7 +325,7 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
 #undef PD_H
 #undef PD
   rc = (int)hipGetLastError();
-  if (rc || (int64_t)max_blocks * block_size <= kGranule) return rc;        // no unit has two granules
+  if (rc) return rc;
   const dim3 jgrid((unsigned)(Hq * (D / 64)), (unsigned)B);
   if (D == 128) hipLaunchKernelGGL(paged_join_kernel<128>, jgrid, dim3(64), 0, st, a);
   else hipLaunchKernelGGL(paged_join_kernel<64>, jgrid, dim3(64), 0, st, a);

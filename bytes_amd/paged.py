@@ -222,7 +222,7 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     W = bt.shape[1]
     with torch.cuda.device(q.device):
         out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device)
-        n = size_query("bytes_paged_decode_workspace_size", B, Hq, Hk, D, bs, W)
+        n = size_query("bytes_paged_decode_workspace_size", B, Hq, Hk, D, int(fp8), bs, W)
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)   # the call's own: calls on other streams share nothing
         call("bytes_paged_decode_attn", ptr(qs), qs.stride(0), qs.stride(1),
              ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),

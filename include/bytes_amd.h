@@ -500,7 +500,7 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  * bytes_paged_decode_attn: out [B, Hq, D] bf16 (strides o_sb, o_sh) =
  *   v_scale * softmax(scale * q . K^T) V over the tokens that take part, zeros
  *   where none does; q [B, Hq, D] bf16.  (scale includes the cache's k_scale.)
- *   Workspace: bytes_paged_decode_workspace_size, contents arbitrary.
+ *   Workspace: bytes_paged_decode_workspace_size (may be 0), contents arbitrary.
  * bytes_paged_page_scores: bound [B, Hq, max_blocks] fp32 (strides b_sb, b_sh)
  *   = scale * sum_d q_d * (q_d >= 0 ? kmax_d : kmin_d) of the block table's
  *   entries, summed in fp64 and rounded once; -inf where a block holds no token
@@ -515,7 +515,8 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  *   max_blocks rounded up to one, rows are read in whole 16-byte chunks), or,
  *   where bound is NULL, those at places pages [B, Hq, npick] (int32, strides
  *   p_sb, p_sh, no place twice; places outside the sequence stand for nothing).
- *   Workspace: bytes_paged_quest_workspace_size, contents arbitrary.
+ *   Workspace: bytes_paged_quest_workspace_size (may be 0), contents
+ *   arbitrary.
  * ------------------------------------------------------------------------- */
 int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
                           const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
@@ -525,7 +526,8 @@ int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void*
                           int64_t cos_st, const void* sin, int64_t sin_st, int positions, int rot, int interleaved,
                           float k_scale, float v_scale, int T, int B, int Hq, int Hk, int D, int block_size,
                           int num_blocks, int max_blocks, void* stream);
-int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int block_size, int max_blocks, size_t* bytes);
+int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int max_blocks,
+                                      size_t* bytes);
 int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
                             int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
                             const void* block_table, int64_t bt_sb, const void* context_lens, void* out, int64_t o_sb,
