@@ -168,7 +168,7 @@ SIGNATURES: Dict[str, Tuple] = {
         c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,                   # block table, row stride, lengths, bound + strides
         c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, Hq, Hk, D, block size, blocks, max blocks
         c_int, c_int, c_f64, c_vp),                              # local_w, skip, scale, stream
-    "bytes_paged_quest_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
+    "bytes_paged_quest_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
     "bytes_paged_quest_attn": (
         c_vp, c_i64, c_i64,                                      # q, strides (b, h)
         c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)

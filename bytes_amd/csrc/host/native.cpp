@@ -544,20 +544,20 @@ Tensor paged_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   return out;
 }
 
-// Selection inside the attention kernel: up to 4096 blocks in a table row.
+// Up to 16384 blocks in a table row (longer ones are selected from by the top-k).
 Tensor paged_quest(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& kmin, const Tensor& kmax,
                    const Tensor& bt, const Tensor& cl, long kb, double scaling, long local_w, double ks, double vs) {
   paged_query(q, k);
   const int64_t B = q.size(0), Hq = q.size(1);
   const Paged p = paged(k, v, bt, cl, B, ks, vs);
-  need(p.W <= 4096 && kb >= 1 && local_w >= 0 && local_w <= (1 << 30));
+  need(p.W <= 16384 && kb >= 1 && local_w >= 0 && local_w <= (1 << 30));
   for (const Tensor* t : {&kmin, &kmax})
     need(t->scalar_type() == at::kBFloat16 && shape(*t, {p.N, p.Hk, p.D}) && t->is_contiguous() && addr(*t) % 16 == 0);
   same_device(k, {&kmin, &kmax});
   const int64_t all = (kb + p.bs - 1) / p.bs, npick = all < p.W ? all : p.W;
   c10::DeviceGuard guard(q.device());
   size_t n = 0;
-  need(bytes_paged_quest_workspace_size(B, Hq, p.Hk, p.D, p.f8, p.bs, npick, &n) == 0);
+  need(bytes_paged_quest_workspace_size(B, Hq, p.Hk, p.D, p.f8, p.bs, p.W, npick, &n) == 0);
   const Tensor bound = empty(q, {B, Hq, (p.W + 3) / 4 * 4}, at::kFloat);       // rows of whole 16-byte chunks
   Tensor w;
   if (n) w = empty(q, {(int64_t)n}, at::kByte);

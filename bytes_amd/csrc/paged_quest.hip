@@ -168,6 +168,7 @@ struct PagedQuestArgs {
 };
 
 constexpr int kPickMax = 4096;       // blocks of a sequence that a workgroup selects from; blocks of a run
+constexpr int kSelectThreads = 1024, kSelectMax = 16 * kSelectThreads;     // the same of the selection launch
 constexpr int kPickWaves = 4, kPickThreads = kPickWaves * 64;
 
 // A wave's tile: 16-byte chunks, LPR lanes to a row, RPI rows to an instruction, NB
@@ -180,9 +181,9 @@ struct PickCfg {
   static constexpr int TILE = NB * RPI;            // rows
 };
 
-// Selection of the k best of n bounds (k < n <= 256 * PER): put(rank in ascending place order, place).
+// Selection of the k best of n bounds (k < n <= NT * PER): put(rank in ascending place order, place).
 // vec: the row starts on a 16-byte boundary and its storage ends on one.
-template <int PER, class PUT>
+template <int NT, int PER, class PUT>
 __device__ __forceinline__ void pick_blocks(const float* bound, bool vec, int n, int k, uint32_t* ws, const PUT& put) {
   uint32_t key[PER];
   if (vec) {
@@ -201,8 +202,8 @@ __device__ __forceinline__ void pick_blocks(const float* bound, bool vec, int n,
 #pragma unroll
     for (int u = 0; u < PER; ++u) key[u] = score_order_key(v[u]);
   }
-  const BlockSel sel = block_select<kPickThreads, PER>(key, n, k, ws);
-  block_select_emit<kPickThreads, PER>(key, n, sel, ws, [&](uint32_t pos, int idx, uint32_t) { put((int)pos, idx); });
+  const BlockSel sel = block_select<NT, PER>(key, n, k, ws);
+  block_select_emit<NT, PER>(key, n, sel, ws, [&](uint32_t pos, int idx, uint32_t) { put((int)pos, idx); });
 }
 
 // Dot product of the lane's dims of a K row with its q (bf16 pairs), fp32 sums.
@@ -291,9 +292,9 @@ __global__ __launch_bounds__(kPickThreads, 4) void paged_quest_kernel(PagedQuest
   if (a.bound && full > a.npick) {
     const float* bound = a.bound + (int64_t)b * a.b_sb + (int64_t)h * a.b_sh;
     const bool vec = a.b_vec != 0;
-    if (full <= 4 * kPickThreads) pick_blocks<4>(bound, vec, full, a.npick, work, put);
-    else if (full <= 8 * kPickThreads) pick_blocks<8>(bound, vec, full, a.npick, work, put);
-    else pick_blocks<16>(bound, vec, full, a.npick, work, put);
+    if (full <= 4 * kPickThreads) pick_blocks<kPickThreads, 4>(bound, vec, full, a.npick, work, put);
+    else if (full <= 8 * kPickThreads) pick_blocks<kPickThreads, 8>(bound, vec, full, a.npick, work, put);
+    else pick_blocks<kPickThreads, 16>(bound, vec, full, a.npick, work, put);
   } else {
     const int32_t* pages = a.pages + b * a.p_sb + h * a.p_sh;
     for (int i = i0 + threadIdx.x; i < i1; i += kPickThreads) put(i, a.bound ? i : pages[i]);
@@ -408,6 +409,24 @@ __global__ __launch_bounds__(kPickThreads, 4) void paged_quest_kernel(PagedQuest
   }
 }
 
+// The selection as a launch of its own, for sequences of more blocks than a
+// workgroup of the attention selects from: one workgroup per query head, its
+// places ascending, -1 past a short sequence's.
+__global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(PagedQuestArgs a, int32_t* pages) {
+  __shared__ __attribute__((aligned(16))) uint32_t work[block_select_words<kSelectThreads>()];
+  const int b = fast_div((int)blockIdx.x, a.dHq), h = (int)blockIdx.x - b * a.Hq;
+  const int full = fast_div(paged_len(a.c, b) + a.c.bs - 1, a.c.dbs);
+  int32_t* to = pages + (int64_t)blockIdx.x * a.npick;
+  if (full <= a.npick) {
+    for (int i = threadIdx.x; i < a.npick; i += kSelectThreads) to[i] = i < full ? i : -1;
+    return;
+  }
+  const float* bound = a.bound + (int64_t)b * a.b_sb + (int64_t)h * a.b_sh;
+  auto put = [&](int i, int place) { to[i] = place; };
+  if (full <= 8 * kSelectThreads) pick_blocks<kSelectThreads, 8>(bound, a.b_vec != 0, full, a.npick, work, put);
+  else pick_blocks<kSelectThreads, 16>(bound, a.b_vec != 0, full, a.npick, work, put);
+}
+
 // Joins the runs of each head that has several, in order: one wave per (sequence,
 // head, 64 dims), four runs at a time, as the decode's join.
 template <int D>
@@ -445,6 +464,10 @@ static void quest_plan(int64_t units, int64_t slots, int bs, int step, int* chun
   if (c < step) c = step;
   *chunk = (int)c;
   *nsplit = (int)((slots + c - 1) / c);
+}
+// The selection launch's lists.
+static size_t selected_bytes(int64_t units, int max_blocks, int npick) {
+  return max_blocks <= kPickMax || max_blocks > kSelectMax ? 0 : (size_t)units * npick * 4;
 }
 static size_t quest_workspace(int64_t units, int nsplit, int D) {
   return nsplit <= 1 ? 0 : (size_t)units * nsplit * (D + 2) * 4;
@@ -492,14 +515,15 @@ int bytes_paged_page_scores(const void* q, int64_t q_sb, int64_t q_sh, const voi
   return (int)hipGetLastError();
 }
 
-int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int npick, size_t* bytes) {
+int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int max_blocks, int npick,
+                                     size_t* bytes) {
   if (!bytes || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128) || npick <= 0)
     return (int)hipErrorInvalidValue;
-  const int rc = paged_check(block_size, 1, npick);
+  const int rc = paged_check(block_size, 1, max_blocks > npick ? max_blocks : npick);
   if (rc) return rc;
   int chunk, ns;
   quest_plan((int64_t)B * Hq, (int64_t)npick * block_size, block_size, pick_step(D, kv_fp8), &chunk, &ns);
-  *bytes = quest_workspace((int64_t)B * Hq, ns, D);
+  *bytes = quest_workspace((int64_t)B * Hq, ns, D) + selected_bytes((int64_t)B * Hq, max_blocks, npick);
   return 0;
 }
 
@@ -515,7 +539,7 @@ int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void
     return (int)hipErrorInvalidValue;
   int rc = paged_check(block_size, num_blocks, max_blocks);
   if (rc) return rc;
-  if (bound && max_blocks > kPickMax) return (int)hipErrorNotSupported;
+  if (bound && max_blocks > kSelectMax) return (int)hipErrorNotSupported;
   PagedQuestArgs a = {};
   a.c.k = k_paged, a.c.k_sb = k_sb, a.c.k_sh = k_sh, a.c.k_ss = k_ss;
   a.c.v = v_paged, a.c.v_sb = v_sb, a.c.v_sh = v_sh, a.c.v_ss = v_ss;
@@ -536,15 +560,24 @@ int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void
   if (units * a.nsplit > 0x7FFFFFFF || units * (D / 64) > 0x7FFFFFFF) return (int)hipErrorInvalidConfiguration;
   a.nwg = (int)(units * a.nsplit);
   a.dsplit = make_fastdiv((uint32_t)a.nsplit);
-  const size_t need = quest_workspace(units, a.nsplit, D);
+  const size_t parts = quest_workspace(units, a.nsplit, D);
+  const size_t need = parts + (bound ? selected_bytes(units, max_blocks, npick) : 0);
   if (need && (!workspace || workspace_bytes < need)) return (int)hipErrorInvalidValue;
-  if (need) {
+  if (parts) {
     a.part_acc = static_cast<float*>(workspace);
     a.part_ml = a.part_acc + (size_t)units * a.nsplit * D;
   }
   const bool small = k_ss >= 0 && k_ss <= (1 << 24) && v_ss >= 0 && v_ss <= (1 << 24);      // 32-bit lane offsets
   const dim3 grid((unsigned)a.nwg), block(kPickThreads);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (bound && max_blocks > kPickMax) {
+    int32_t* list = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + parts);
+    hipLaunchKernelGGL(paged_select_kernel, dim3((unsigned)units), dim3(kSelectThreads), 0, st, a, list);
+    rc = (int)hipGetLastError();
+    if (rc) return rc;
+    a.bound = nullptr;
+    a.pages = list, a.p_sh = npick, a.p_sb = (int64_t)Hq * npick;
+  }
 #define PS(DD, F8)                                                                                                 \
   if (small && block_size % PickCfg<DD, F8>::RPI == 0)                                                             \
     hipLaunchKernelGGL((paged_quest_kernel<DD, F8, true>), grid, block, 0, st, a);                                 \

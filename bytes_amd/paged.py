@@ -267,7 +267,7 @@ def _page_scores(qs, kmin, kmax, bt, cl, bs: int, scale: float, local_w: int, sk
     return bound
 
 
-_SELECT_IN_KERNEL_MAX = 4096        # blocks of a sequence that the attention kernel selects from itself
+_SELECT_MAX = 16384        # blocks of a sequence that bytes_paged_quest_attn selects from
 
 
 def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Tensor, meta: Meta,
@@ -296,7 +296,7 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     W = bt.shape[1]
     npick = min((int(kb) + bs - 1) // bs, W)
     scale = float(scaling) * float(k_scale)
-    listed = return_pages or W > _SELECT_IN_KERNEL_MAX
+    listed = return_pages or W > _SELECT_MAX
     bound = _page_scores(qs, kmin, kmax, bt, cl, bs, scale, local_w, -1 if listed else npick)
     with torch.cuda.device(q.device):
         pages = None
@@ -304,7 +304,7 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
             n = size_query("bytes_topk_workspace_size", B * Hq, W, npick)
             pages = _topk(bound, npick, sorted=False, ws=torch.zeros(max(n, 16), dtype=torch.uint8, device=q.device))
         out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device)
-        n = size_query("bytes_paged_quest_workspace_size", B, Hq, Hk, D, int(fp8), bs, npick)
+        n = size_query("bytes_paged_quest_workspace_size", B, Hq, Hk, D, int(fp8), bs, W, npick)
         ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
         call("bytes_paged_quest_attn", ptr(qs), qs.stride(0), qs.stride(1),
              ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),

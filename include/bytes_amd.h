@@ -510,7 +510,7 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  * bytes_paged_quest_attn: bytes_paged_decode_attn over the tokens of npick
  *   blocks per query head: the best of bound (as bytes_paged_page_scores gives
  *   them, skip <= npick; bound descending, lowest place first on equal bounds;
- *   max_blocks <= 4096, hipErrorNotSupported above; sequences of at most npick
+ *   max_blocks <= 16384, hipErrorNotSupported above; sequences of at most npick
  *   blocks whole; where b_sb, b_sh are multiples of 4 and b_sh at least
  *   max_blocks rounded up to one, rows are read in whole 16-byte chunks), or,
  *   where bound is NULL, those at places pages [B, Hq, npick] (int32, strides
@@ -537,8 +537,8 @@ int bytes_paged_page_scores(const void* q, int64_t q_sb, int64_t q_sh, const voi
                             const void* block_table, int64_t bt_sb, const void* context_lens, void* bound, int64_t b_sb,
                             int64_t b_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks,
                             int local_w, int skip, double scale, void* stream);
-int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int npick,
-                                     size_t* bytes);
+int bytes_paged_quest_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, int block_size, int max_blocks,
+                                     int npick, size_t* bytes);
 int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
                            int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_fp8,
                            const void* bound, int64_t b_sb, int64_t b_sh, const void* pages, int64_t p_sb, int64_t p_sh,

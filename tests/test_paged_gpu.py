@@ -464,26 +464,30 @@ def test_quest_ties_and_nonfinite_bounds(dev):
         assert bool((pages == 33).any(-1).all())
 
 
-def test_quest_many_pages(dev):
-    """More pages than the selection holds in one workgroup's registers."""
+@pytest.mark.parametrize("bs,L", [(4, 20001), (2, 25000), (1, 16384), (1, 16700)])
+def test_quest_many_pages(dev, bs, L):
+    """More pages than a workgroup of the attention selects from (a launch of its own up
+    to 16384, the top-k above)."""
     g = torch.Generator().manual_seed(8)
-    bs, L, Hq, Hk, D = 4, 20001, 4, 2, 64
-    table, N = _table(g, [L, 777], bs)
+    Hq, Hk, D = 4, 2, 64
+    kb = 100 * bs
+    table, N = _table(g, [L, 777, 0], bs, slack=0)
     kc, vc = _make_cache(g, N, Hk, bs, D, False)
-    n = torch.tensor([L, 777], dtype=torch.int32)
+    n = torch.tensor([L, 777, 0], dtype=torch.int32)
     meta = _page_meta(kc, table, n, bs)
-    q = _rand(g, 2, Hq, 1, D)
-    out, pages = PG.paged_quest_decode(q.to(dev), kc.to(dev), vc.to(dev), tuple(m.to(dev) for m in meta), table.to(dev),
-                                       n.to(dev), 400, 0.125, return_pages=True)
-    qd = q.double().reshape(2, Hk, Hq // Hk, D)
+    q = _rand(g, 3, Hq, 1, D)
+    a = (q.to(dev), kc.to(dev), vc.to(dev), tuple(m.to(dev) for m in meta), table.to(dev), n.to(dev), kb, 0.125)
+    out, pages = PG.paged_quest_decode(*a, return_pages=True)
+    alone = PG.paged_quest_decode(*a)
+    qd = q.double().reshape(3, Hk, Hq // Hk, D)
     ids = table.clamp(min=0).long()
     kmin, kmax = (m.double()[ids].permute(0, 2, 3, 1) for m in meta)
-    b = (qd.clamp(min=0) @ kmax.nan_to_num(0) + qd.clamp(max=0) @ kmin.nan_to_num(0)).reshape(2, Hq, -1) * 0.125
+    b = (qd.clamp(min=0) @ kmax.nan_to_num(0) + qd.clamp(max=0) @ kmin.nan_to_num(0)).reshape(3, Hq, -1) * 0.125
     b = b.float().masked_fill((torch.arange(table.shape[1]) * bs >= n[:, None])[:, None], -INF)
     want = b.argsort(dim=-1, descending=True, stable=True)[..., :100].sort(-1).values
-    assert torch.equal(pages.cpu().long(), want)
+    assert torch.equal(pages.cpu().long(), want) and torch.equal(alone, out)
     _check_decode(dev, out, q, kc, vc, 0.125, 1.0, 1.0, table, n,
-                  [[set(want[i, h].tolist()) for h in range(Hq)] for i in range(2)])
+                  [[set(want[i, h].tolist()) for h in range(Hq)] for i in range(3)])
 
 
 # ---------------------------------------------------------------------------
