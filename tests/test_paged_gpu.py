@@ -6,6 +6,8 @@ import pytest
 import torch
 
 import paged_oracle as O
+from test_native_path_gpu import _both
+from bytes_amd import _lib
 from bytes_amd import attention_kernels as AK
 from bytes_amd import paged as PG
 from bytes_amd import quest as QU
@@ -597,3 +599,109 @@ def test_streams_share_nothing(dev):
     for i in range(2):
         for r in got[i]:
             assert torch.equal(r[0], want[i][0]) and torch.equal(r[1], want[i][1])
+
+
+def test_native_path_and_wrapper_agree(dev, monkeypatch):
+    """The native call path and the Python wrapper: the same bits, for the layouts either takes."""
+    g = torch.Generator().manual_seed(31)
+    B, Hq, Hk, D, bs = 3, 14, 2, 64, 16
+    lens = [300, 17, 0]
+    for fp8 in (False, True):
+        table, N = _table(g, lens, bs)
+        kc, vc = (c.to(dev) for c in _make_cache(g, N, Hk, bs, D, fp8))
+        n, table = torch.tensor(lens, dtype=torch.int32, device=dev), table.to(dev)
+        sc = 0.03 if fp8 else 1.0
+        meta = tuple(m.to(dev) for m in _page_meta(kc.cpu(), table.cpu(), torch.tensor(lens), bs))
+        qkv = _rand(g, B, Hq + 2 * Hk, D).to(dev)
+        q = qkv[:, :Hq].unsqueeze(2)                      # a strided view
+        ks = dict(k_scale=sc, v_scale=sc)
+        _both(monkeypatch, PG.paged_decode_attn, q, kc, vc, table, n, 0.125, **ks)
+        _both(monkeypatch, PG.paged_decode_attn, q, kc, vc, table, n, **ks)
+        _both(monkeypatch, PG.paged_decode_attn, q, kc, vc, table.long(), n, 0.125, taken=False, **ks)
+        _both(monkeypatch, PG.paged_decode_attn, q, kc, vc, table[:, :8], n, 1, **ks)      # a view of a wider table
+        wide = torch.zeros(B, Hq, 1, D + 1, dtype=BF16, device=dev)[..., 1:]
+        _both(monkeypatch, PG.paged_decode_attn, wide, kc, vc, table, n, 0.125, taken=False, **ks)
+        a = (q, kc, vc, meta, table, n)
+        _both(monkeypatch, PG.paged_quest_decode, *a, 64, 0.125, **ks)
+        _both(monkeypatch, PG.paged_quest_decode, *a, 33, 0.125, local_w=20, **ks)
+        _both(monkeypatch, PG.paged_quest_decode, *a, 64, 0.125, return_pages=True, taken=False, **ks)
+        cos, sin = (x.to(dev) for x in _cos_sin(table.shape[1] * bs, 32))
+        x = (qkv[:, Hq:Hq + Hk], qkv[:, Hq + Hk:], kc, vc, table, n)
+        kw = dict(q=qkv[:, :Hq], cos=cos, sin=sin, meta=meta, **ks)
+        _both(monkeypatch, PG.paged_kv_append, *x, **kw)
+        _both(monkeypatch, PG.paged_kv_append, *x, interleaved=True, **{**kw, "meta": None})
+        cu = torch.tensor([0, 2, 3, 3], dtype=torch.int32, device=dev)
+        _both(monkeypatch, PG.paged_kv_append, *x, cu_seqlens=cu, **kw)
+        _both(monkeypatch, PG.paged_kv_append, *x, cu_seqlens=cu.long(), taken=False, **kw)
+        got = []
+        for native in (_lib.native(), _lib._NoNative()):
+            monkeypatch.setattr(_lib, "_native", native)
+            k2, v2, m2 = kc.clone(), vc.clone(), tuple(m.clone() for m in meta)
+            assert PG.paged_kv_append(*x[:2], k2, v2, table, n, cos=cos, sin=sin, meta=m2, **ks) is None
+            got.append((k2, v2, *m2))
+            monkeypatch.undo()
+        for u, v in zip(*got):
+            assert _same(u, v)
+        for bad in ((q, kc, vc[:, :1], table, n), (q, kc, vc, table[:2], n), (q, kc, vc, table, n.float()),
+                    (q[..., :32], kc, vc, table, n), (q.half(), kc, vc, table, n), (q.cpu(), kc, vc, table, n),
+                    (q, kc, vc, table.cpu(), n), (q, kc.transpose(2, 3), vc, table, n)):
+            with pytest.raises(ValueError):
+                PG.paged_decode_attn(*bad, 0.125, **ks)
+
+
+def test_shared_and_repeated_blocks(dev):
+    """Sequences that share a prefix, one table row for all (stride 0), a block named twice by one sequence."""
+    g = torch.Generator().manual_seed(41)
+    Hq, Hk, D, bs = 8, 2, 128, 16
+    kc, vc = _make_cache(g, 40, Hk, bs, D, False)
+    q = _rand(g, 4, Hq, 1, D)
+    row = torch.randperm(40, generator=g)[:30].to(torch.int32)
+    row[7] = row[3]
+    n = torch.tensor([480, 100, 1, 301], dtype=torch.int32)
+    shared = row.to(dev)[None].expand(4, 30)
+    out = PG.paged_decode_attn(q.to(dev), kc.to(dev), vc.to(dev), shared, n.to(dev), 0.09)
+    _check_decode(dev, out, q, kc, vc, 0.09, 1.0, 1.0, row[None].expand(4, 30), n)
+    meta = QU.quest_page_minmax(kc.to(dev), bs)
+    meta = tuple(m[:, :, 0] for m in meta)
+    got, pages = PG.paged_quest_decode(q.to(dev), kc.to(dev), vc.to(dev), meta, shared, n.to(dev), 96, 0.09, return_pages=True)
+    picks = [[set(pages[b, h].tolist()) for h in range(Hq)] for b in range(4)]
+    _check_decode(dev, got, q, kc, vc, 0.09, 1.0, 1.0, row[None].expand(4, 30), n, picks)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_offsets_past_32_bits(dev, fp8):
+    """Blocks more than 2^32 bytes and 2^31 elements into the cache: append, decode and page-sparse decode."""
+    Hq, Hk, D, bs = 8, 8, 128, 128
+    per = Hk * bs * D
+    N = 2 ** 31 // per * (2 if fp8 else 1) + 6
+    dt = F8 if fp8 else BF16
+    kc = torch.empty(N, Hk, bs, D, dtype=dt, device=dev)
+    vc = torch.empty(N, Hk, bs, D, dtype=dt, device=dev)
+    g = torch.Generator().manual_seed(51)
+    table = torch.tensor([[N - 1, 0, N - 3], [N - 2, N - 5, -1]], dtype=torch.int32)
+    lens, new = [300, 140], [300, 139]
+    qkv = _rand(g, sum(new), Hq + 2 * Hk, D)
+    meta = tuple(torch.zeros(N, Hk, D, dtype=BF16, device=dev) for _ in range(2))
+    used = table[table >= 0].unique().long()
+    for c in (kc, vc):
+        c.view(torch.uint8)[used.to(dev)] = 0
+    cu = torch.tensor([0, 300, 439], dtype=torch.int32)
+    n = torch.tensor(lens, dtype=torch.int32)
+    x = qkv.to(dev)
+    q = PG.paged_kv_append(x[:, Hq:Hq + Hk], x[:, Hq + Hk:], kc, vc, table.to(dev), n.to(dev), cu_seqlens=cu.to(dev),
+                           q=x[:, :Hq], meta=meta)
+    assert torch.equal(q, x[:, :Hq])                      # no rotation asked for
+    small_k, small_v = (torch.zeros(N if N < 8 else 8, Hk, bs, D).to(dt) for _ in range(2))
+    place = {int(b): i for i, b in enumerate(used)}
+    for b, i in place.items():
+        small_k.view(torch.uint8)[i], small_v.view(torch.uint8)[i] = (c[b].view(torch.uint8).cpu() for c in (kc, vc))
+    st = torch.tensor([[place.get(int(b), -1) for b in r] for r in table], dtype=torch.int32)
+    for t, b, p in O.placed(sum(new), table, n, cu, bs):
+        row = small_v[int(st[b, p // bs]), :, p % bs].float()
+        assert torch.equal(row, qkv[t, Hq + Hk:].to(dt).float()), (t, b, p)
+    dq = q[[299, 438]].unsqueeze(2)
+    out = PG.paged_decode_attn(dq, kc, vc, table.to(dev), n.to(dev), 0.09)
+    _check_decode(dev, out, dq.cpu(), small_k, small_v, 0.09, 1.0, 1.0, st, n)
+    out, pages = PG.paged_quest_decode(dq, kc, vc, meta, table.to(dev), n.to(dev), 2 * bs, 0.09, return_pages=True)
+    picks = [[set(pages[b, h].tolist()) for h in range(Hq)] for b in range(2)]
+    _check_decode(dev, out, dq.cpu(), small_k, small_v, 0.09, 1.0, 1.0, st, n, picks)
