@@ -243,6 +243,7 @@ __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t*
     const int sl = s0 + (lane & 31);
     find(min(sl, s_end - 1), place, t.off, t.ok);
     t.ok = t.ok && sl < s_end;
+    t.off = sl < s_end ? t.off : 0;  // (16 rows from there are read in HALVES: they have to be the block's)
     t.id = table[place];
     return t;
   };

@@ -466,6 +466,7 @@ int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void*
     const int rows_per_wave = 64 / (D / 16);
     a.per_token = (2 * Hk + Hq + rows_per_wave - 1) / rows_per_wave;
     a.d_per_token = make_fastdiv((uint32_t)a.per_token);
+    if ((int64_t)T * a.per_token > 0x7FFFFFF0) return (int)hipErrorInvalidConfiguration;
     grid = ((int64_t)T * a.per_token + kAppendWaves - 1) / kAppendWaves;
   } else {
     // a sequence's n tokens lie in at most n / span + 2 spans, and in at most n

@@ -446,20 +446,19 @@ __global__ __launch_bounds__(64) void paged_quest_join_kernel(PagedQuestArgs a) 
                 });
 }
 
-// Runs of a head's slots: as many as make about PER_CU workgroups per CU, whole
+// Runs of a head's slots: as many as make about four workgroups per CU, whole
 // rounds of the four waves' tiles, and no more blocks than a run's list holds.
 static int pick_step(int D, int fp8) {
   if (D == 128) return kPickWaves * (fp8 ? PickCfg<128, true>::TILE : PickCfg<128, false>::TILE);
   return kPickWaves * (fp8 ? PickCfg<64, true>::TILE : PickCfg<64, false>::TILE);
 }
-#ifndef PER_CU
-#define PER_CU 4
-#endif
 static void quest_plan(int64_t units, int64_t slots, int bs, int step, int* chunk, int* nsplit) {
-  const int64_t target = PER_CU * (int64_t)device_cu_count();
+  const int64_t target = 4 * (int64_t)device_cu_count();
   int64_t c = (slots * units + target - 1) / target;
   c = (c + step - 1) / step * step;
   const int64_t most = (int64_t)(kPickMax - 1) * bs / step * step;       // a run may start within a block
+  const int64_t whole = (slots + step - 1) / step * step;
+  if (c > whole) c = whole;
   if (c > most) c = most;
   if (c < step) c = step;
   *chunk = (int)c;
