@@ -3,8 +3,8 @@
 // Token i of sequence b's n new ones has position p = lens[b] - n + i (lens
 // counts the new tokens).  Its key's (and query's) first R dims are rotated in
 // pairs (x0, x1) -> (x0 c - x1 s, x1 c + x0 s) with row p of the cos / sin
-// tables, pairs (j, j + R/2) or neighbours (2j, 2j + 1), in fp32; the result,
-// divided by the cache's scale, is rounded once to the cache's type.  The
+// tables, pairs (j, j + R/2) or neighbours (2j, 2j + 1); the result, divided by the
+// cache's scale in fp32, is rounded to the cache's type.  The
 // blocks' elementwise min / max (of the values as stored) are kept for the
 // page-sparse decode.
 //
@@ -121,23 +121,34 @@ __device__ __forceinline__ void load_turn(const AppendArgs& a, const AppendItem&
     for (int e = 0; e < 4; ++e) r.c[4 * j + e] = x[e], r.s[4 * j + e] = y[e];
   }
 }
+// x0 c - x1 s from its exact products (8 by 24 bits), rounded to fp32 once.
+__device__ __forceinline__ float turned_exact(double x0, double c, double x1, double s) {
+  return (float)__builtin_fma(x0, c, -(x1 * s));
+}
+// EXACT for keys, which stay in the cache and in its min / max: with the products
+// rounded to fp32 one in some 2^16 came out on the other side of a bf16 step.
+// Queries, most of a prompt's rows, take fp32.
+template <bool EXACT>
 __device__ __forceinline__ void turn_item(const AppendArgs& a, const Turn& r, float* x) {
   float y[16];
-  if (a.interleaved) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y[2 * j] = x[2 * j] * r.c[j] - x[2 * j + 1] * r.s[j];
-      y[2 * j + 1] = x[2 * j + 1] * r.c[j] + x[2 * j] * r.s[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      y[j] = x[j] * r.c[j] - x[j + 8] * r.s[j];
-      y[j + 8] = x[j + 8] * r.c[j] + x[j] * r.s[j];
+  for (int j = 0; j < 8; ++j) {
+    const float x0 = a.interleaved ? x[2 * j] : x[j], x1 = a.interleaved ? x[2 * j + 1] : x[j + 8];
+    if constexpr (EXACT) {
+      y[j] = turned_exact(x0, r.c[j], x1, r.s[j]);
+      y[j + 8] = turned_exact(x1, r.c[j], -x0, r.s[j]);
+    } else {
+      y[j] = x0 * r.c[j] - x1 * r.s[j];
+      y[j + 8] = x1 * r.c[j] + x0 * r.s[j];
     }
   }
+  if (a.interleaved) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) x[j] = y[j];
+    for (int j = 0; j < 8; ++j) x[2 * j] = y[j], x[2 * j + 1] = y[j + 8];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) x[j] = y[j];
+  }
 }
 
 // Stores the item in its cache row (`to` the row's start); x becomes what the cache then holds.
@@ -206,7 +217,8 @@ __global__ __launch_bounds__(kAppendWaves * 64) void paged_append_one_kernel(App
   if (live && !value && it.turn && placed) {
     Turn tr;
     load_turn(a, it, ps, tr);
-    turn_item(a, tr, x);
+    if (key) turn_item<true>(a, tr, x);
+    else turn_item<false>(a, tr, x);
   }
   if (!live) return;
   if (key) {
@@ -334,7 +346,7 @@ __device__ __forceinline__ void append_span(const AppendArgs& a, const Span& s, 
       float x[16];
       widen8(raw[u][0], x);
       widen8(raw[u][1], x + 8);
-      if (KIND != kValues && it.turn) turn_item(a, tr, x);
+      if (KIND != kValues && it.turn) turn_item<KIND == kKeys>(a, tr, x);
       if (KIND == kQueries) {
         if (!placed) {
 #pragma unroll
