@@ -13,7 +13,8 @@
 // 8 consecutive floats.  D/16 lanes cover a row; a wave's 64 lanes are 64/(D/16)
 // rows.
 //  * One token per sequence: a wave's rows are heads (keys, values and queries in
-//    one list) of one token.
+//    one list) of one token.  3.9 us for a single token, 5.2 for 30 with min / max:
+//    length, block id, rows and min / max follow one another.
 //  * Prompts: a wave's rows are consecutive tokens of one sequence.  Values and
 //    queries (and keys where no min / max is kept) go in spans of as many positions
 //    as a wave has rows, keys with min / max in blocks: a wave has a whole block's

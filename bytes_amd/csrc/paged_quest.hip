@@ -53,6 +53,10 @@ __device__ __forceinline__ double bound_literal(const uint16_t* q, const uint16_
 // A and B agree); q's parts are widened once per workgroup, in LDS.  The result is
 // at lane: head l / 16, block l % 16.  A tile with an infinite or NaN entry, where
 // the part of q that is 0 would give NaN, takes the literal sum.
+// Bound by memory for large batches: 44 MB of min / max (seven sequences of 32K to 64K,
+// 8 KV heads of 128, blocks of 32) take 16.5 us from a graph, 12.4 of them the loads
+// alone; with the sums on the vector unit 24.  One sequence of 32K (4.2 MB): 5.2, launch and round trips; two tiles per wave,
+// half the waves, 7.7 (and 17.2 for the 44 MB).
 template <int D, int NG>
 __global__ __launch_bounds__(kBoundWaves * 64, 4) void page_bound_kernel(PageBoundArgs a) {
   PREFETCH_ARGS(a);
@@ -249,6 +253,10 @@ __device__ __forceinline__ void add_chunk(const u32x4& v, float p, float (&acc)[
 // throughout), and groups and waves are merged at the end.  No LDS stage, so
 // registers alone bound the waves in flight.  RUNS: block sizes that are multiples of
 // RPI, whose instructions' rows lie in one block and start at a scalar address.
+// Bound by reads of short runs of rows anywhere in the cache: 2048 of 32K to 64K
+// fp8 tokens of 7 x 24 heads (84 MB of distinct rows) take 24 us, 3.5 TB/s, 4 of
+// them the selection; 2048 of 32K bf16 tokens of 28 heads (24 MB) 10.5.  With two tiles
+// in flight per wave a whole call takes 53 for 46.5 and 22 for 20.
 template <int D, bool FP8, bool RUNS>
 __global__ __launch_bounds__(kPickThreads, 4) void paged_quest_kernel(PagedQuestArgs a) {
   using P = PickCfg<D, FP8>;
@@ -411,7 +419,10 @@ __global__ __launch_bounds__(kPickThreads, 4) void paged_quest_kernel(PagedQuest
 
 // The selection as a launch of its own, for sequences of more blocks than a
 // workgroup of the attention selects from: one workgroup per query head, its
-// places ascending, -1 past a short sequence's.
+// places ascending, -1 past a short sequence's.  Below that it costs more than the
+// selection that every run of a head repeats (us of a call, in the kernel and as a
+// launch: one sequence of 32K, 28 heads, 2048 blocks 19.3 and 22.9; one of 60000, 8
+// heads, 3750 blocks 16.4 and 17.6; 16 of 8K, 64 heads, 512 blocks 49 and 69).
 __global__ __launch_bounds__(kSelectThreads) void paged_select_kernel(PagedQuestArgs a, int32_t* pages) {
   __shared__ __attribute__((aligned(16))) uint32_t work[block_select_words<kSelectThreads>()];
   const int b = fast_div((int)blockIdx.x, a.dHq), h = (int)blockIdx.x - b * a.Hq;
@@ -448,6 +459,9 @@ __global__ __launch_bounds__(64) void paged_quest_join_kernel(PagedQuestArgs a) 
 
 // Runs of a head's slots: as many as make about four workgroups per CU, whole
 // rounds of the four waves' tiles, and no more blocks than a run's list holds.
+// Four are what fit a CU's registers (us of a call, 2048 of 32K to 64K fp8 tokens of
+// 7 x 24 heads: 47; one per CU 54, two 49, eight 56; one sequence of 32K, 28 heads:
+// 19.3 with any of them).
 static int pick_step(int D, int fp8) {
   if (D == 128) return kPickWaves * (fp8 ? PickCfg<128, true>::TILE : PickCfg<128, false>::TILE);
   return kPickWaves * (fp8 ? PickCfg<64, true>::TILE : PickCfg<64, false>::TILE);

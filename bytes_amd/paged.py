@@ -11,12 +11,12 @@ sequence b is row p % block_size of block block_table[b, p // block_size].
 `context_lens[b]` is the number of tokens of sequence b in the cache, in every
 operator here: the append takes it with the new tokens counted, so one tensor
 serves a whole decode step.  Lengths, block tables and cu_seqlens stay on the
-device; nothing here synchronises, and every call can be captured in a graph (lengths and tables
-are read at replay).  Lengths are held to 0 .. max_blocks * block_size.  A block id
-outside [0, num_blocks) names no block (-1 past a sequence's blocks, or a hole
-where a block was evicted): nothing is written for its tokens and they take no
-part in attention.  A sequence none of whose tokens take part (length 0, as in the padding rows of a
-batch) gets zeros.
+device; nothing here synchronises, and every call can be captured in a graph
+(lengths and tables are read at replay).  Lengths are held to 0 .. max_blocks *
+block_size.  A block id outside [0, num_blocks) names no block (-1 past a
+sequence's blocks, or a hole where a block was evicted): nothing is written for
+its tokens and they take no part in attention.  A sequence none of whose tokens
+take part (length 0, as in the padding rows of a batch) gets zeros.
 
 Results carry no autograd graph.  H_q must be a multiple of H_k and D 64 or 128.
 """
@@ -117,28 +117,32 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
 
     k, v [T, H_k, D] bf16 hold the new tokens of all sequences one after another
     (views of a fused projection are fine): sequence b's are rows cu_seqlens[b] ..
-    cu_seqlens[b+1] (int32 [B+1], cu_seqlens[0] = 0), or row b alone without
+    cu_seqlens[b+1] (int32 [B+1], ascending from 0), or row b alone without
     cu_seqlens (T = B, the decode step).  Its n new tokens end at context_lens[b]:
     token i has position context_lens[b] - n + i.  Tokens without a position in
     0 .. max_blocks * block_size, and rows past cu_seqlens[B], are not written;
     cache rows that no new token names keep their bytes.
 
-    cos, sin [P, R/2] fp32 (P >= max_blocks * block_size, R a multiple of 16, at most D): the first R dims of
-    keys (and queries) are rotated in pairs (x0, x1) -> (x0 cos - x1 sin,
-    x1 cos + x0 sin), pairs (j, j + R/2), or (2j, 2j + 1) if interleaved.
+    cos, sin [P, R/2] fp32 (P >= max_blocks * block_size, R a multiple of 16, at
+    most D): the first R dims of keys (and queries) are rotated in pairs (x0, x1)
+    -> (x0 cos - x1 sin, x1 cos + x0 sin), pairs (j, j + R/2), or (2j, 2j + 1) if
+    interleaved.
     fp8 caches store k / k_scale and v / v_scale, values beyond the format's range
     (infinities too) as its largest ones.
 
     meta (kmin, kmax), each [num_blocks, H_k, D] bf16: the elementwise min / max of
     every block's stored keys, kept for paged_quest_decode.  A block that a
-    sequence enters at its first row starts anew, others are folded into.  (For a
-    cache filled otherwise, quest_page_minmax(k_paged, block_size) gives them where all blocks are full.)
+    sequence enters at its first row starts anew, others are folded into: rows
+    written again (after a rollback) widen them until then, so they stay bounds.
+    (For a cache filled otherwise, quest_page_minmax(k_paged, block_size) gives
+    them where all blocks are full.)
 
     q [T, H_q, D] bf16: returned rotated, [T, H_q, D] bf16 (with T = B,
-    q_rot.unsqueeze(2) is paged_decode_attn's query); zeros in rows that have no position.
-    Without q the result is None.
+    q_rot.unsqueeze(2) is paged_decode_attn's query); zeros in rows that have no
+    position.  Without q the result is None.
 
-    Blocks that receive tokens must belong to one sequence each (blocks of a shared prefix are only read)."""
+    Blocks that receive tokens must belong to one sequence each (blocks of a
+    shared prefix are only read)."""
     kmin, kmax = meta if meta is not None else (None, None)
     out = native().paged_append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin,
                                 bool(interleaved), kmin, kmax, k_scale, v_scale)
@@ -223,7 +227,8 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     with torch.cuda.device(q.device):
         out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device)
         n = size_query("bytes_paged_decode_workspace_size", B, Hq, Hk, D, int(fp8), bs, W)
-        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)   # the call's own: calls on other streams share nothing
+        # the call's own: calls on other streams share nothing
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
         call("bytes_paged_decode_attn", ptr(qs), qs.stride(0), qs.stride(1),
              ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),
              ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), int(fp8), ptr(bt), bt.stride(0),
