@@ -349,6 +349,34 @@ def test_decode_large_scores_and_nonfinite_rows(dev):
     assert bool(out[0, 4:].isnan().all()) and bool(torch.isfinite(out[0, :4]).all()) and bool(torch.isfinite(out[1]).all())
 
 
+@pytest.mark.parametrize("L", [100, 3000])
+def test_infinite_values_that_take_part(dev, L):
+    """An infinite value gives its infinity in its dim, whatever the weight (1 of a
+    single token, one that two bf16 numbers hold exactly or not), and nothing elsewhere;
+    both signs in one dim give NaN."""
+    g = torch.Generator().manual_seed(L)
+    lens, Hq, Hk, D, bs = [L, 1, L - 7], 8, 2, 64, 16
+    table, N = _table(g, lens, bs)
+    kc, vc = _make_cache(g, N, Hk, bs, D, False)
+    q = _rand(g, 3, Hq, 1, D)
+    q[2] = 0.0                                            # equal weights
+    n = torch.tensor(lens, dtype=torch.int32)
+    vc[int(table[0, 2]), 0, 3, 5], vc[int(table[0, 4]), 0, 9, 6] = INF, -INF
+    vc[int(table[0, 1]), 0, 0, 7], vc[int(table[0, 5]), 0, 0, 7] = INF, -INF
+    vc[int(table[1, 0]), 1, 0, 63], vc[int(table[2, 3]), 1, 15, 0] = -INF, INF
+    meta = tuple(t.to(dev) for t in _page_meta(kc, table, lens, bs))
+    outs = [PG.paged_decode_attn(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev), n.to(dev), 0.1),
+            PG.paged_quest_decode(q.to(dev), kc.to(dev), vc.to(dev), meta, table.to(dev), n.to(dev), L + bs, 0.1)]
+    want, mag, dots = O.attend(q, kc, vc, 0.1, 1.0, 1.0, table, n)
+    fin = torch.isfinite(want)
+    for out in outs:
+        got = out.double().cpu().reshape(want.shape)
+        for b, h, d, x in ((0, 0, 5, INF), (0, 0, 6, -INF), (1, 4, 63, -INF), (2, 4, 0, INF)):
+            assert bool((want[b, h:h + 4, d] == x).all()) and bool((got[b, h:h + 4, d] == x).all()), (b, h, d, got[b, h:h + 4, d])
+        assert bool(got[0, :4, 7].isnan().all())
+        assert int((~fin).sum()) == 5 * 4 and bool(((got - want).abs() <= _tol(want, mag, dots, D))[fin].all())
+
+
 @pytest.mark.parametrize("B,Hq,Hk,D,L,bs,fp8", [(3, 28, 4, 128, 9001, 16, False), (1, 14, 2, 64, 40000, 16, False),
                                                 (70, 8, 8, 64, 700, 16, True), (150, 4, 1, 128, 300, 12, False)])
 def test_decode_long_and_wide(dev, B, Hq, Hk, D, L, bs, fp8):
