@@ -344,7 +344,9 @@ __device__ __forceinline__ void paged_store(uint16_t* out, const f32x4& A, float
 // four lane groups take the parts in turn, each in order, and are folded by fixed
 // row swaps.  slot(i): part i's place; pml: (maximum, denominator) by place; pacc:
 // the lane's four values of place 0, places `pitch` apart.  The first 4 * PF parts
-// and their statistics are loaded together, one round trip.
+// and their statistics are loaded together, one round trip; a lane group past the
+// last part adds zeros (0 times the last part's values again would not be 0 where
+// those are infinite).
 template <int PF, class SLOT, class PUT>
 __device__ __forceinline__ void paged_join(int parts, int lane, const SLOT& slot, const float2* pml, const f32x4* pacc,
                                            int pitch, const PUT& put) {
@@ -352,7 +354,7 @@ __device__ __forceinline__ void paged_join(int parts, int lane, const SLOT& slot
   float2 ml[PF];
   f32x4 acc[PF];
 #pragma unroll
-  for (int u = 0; u < PF; ++u) {                   // parts past the last: its values again, with weight 0
+  for (int u = 0; u < PF; ++u) {                   // parts past the last: its values again, not used
     const size_t r = slot(min(grp + 4 * u, parts - 1));
     ml[u] = pml[r];
     acc[u] = pacc[r * pitch];
@@ -367,9 +369,10 @@ __device__ __forceinline__ void paged_join(int parts, int lane, const SLOT& slot
   f32x4 A = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int u = 0; u < PF; ++u) {
-    const float f = grp + 4 * u < parts ? fast_exp2(ml[u].x - M) : 0.f;
+    const bool part = grp + 4 * u < parts;
+    const float f = part ? fast_exp2(ml[u].x - M) : 0.f;
     L += f * ml[u].y;
-    A += f * acc[u];
+    A += f * (part ? acc[u] : f32x4{0.f, 0.f, 0.f, 0.f});
   }
   for (int i = 4 * PF + grp; i < parts; i += 4) {
     const size_t r = slot(i);

@@ -733,3 +733,56 @@ def test_offsets_past_32_bits(dev, fp8):
     out, pages = PG.paged_quest_decode(dq, kc, vc, meta, table.to(dev), n.to(dev), 2 * bs, 0.09, return_pages=True)
     picks = [[set(pages[b, h].tolist()) for h in range(Hq)] for b in range(2)]
     _check_decode(dev, out, dq.cpu(), small_k, small_v, 0.09, 1.0, 1.0, st, n, picks)
+
+
+# ---------------------------------------------------------------------------
+# infinite values, weights and stored keys
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("B,Hk,L", [(1, 2, 700), (1, 2, 2100), (1, 2, 9000), (30, 8, 3000)])
+def test_infinite_values_in_any_part(dev, B, Hk, L):
+    """Infinite values in the first, a middle and the last of 2 to more than 32 joined
+    parts (a unit's tokens are split over workgroups): that infinity, in its dim alone."""
+    g = torch.Generator().manual_seed(L)
+    Hq, D, bs = 2 * Hk, 64, 16
+    lens = [L - 40 * b for b in range(B)]
+    table, N = _table(g, lens, bs, slack=max(2, 1200 // bs - L // bs))     # past what one workgroup takes alone
+    kc, vc = _make_cache(g, N, Hk, bs, D, False)
+    q, n = _rand(g, B, Hq, 1, D), torch.tensor(lens, dtype=torch.int32)
+    at = {}
+    for b in range(B):
+        for hk in range(Hk):
+            for i, p in enumerate((0, 5, lens[b] // 3, lens[b] // 2, lens[b] - 140, lens[b] - 2, lens[b] - 1)):
+                x = INF if (i + hk) % 2 else -INF
+                vc[int(table[b, p // bs]), hk, p % bs, 3 * i + hk] = x
+                at[b, hk, 3 * i + hk] = x
+    meta = tuple(t.to(dev) for t in _page_meta(kc, table, lens, bs))
+    a = (q.to(dev), kc.to(dev), vc.to(dev))
+    t = (table.to(dev), n.to(dev))
+    outs = {"decode": PG.paged_decode_attn(*a, *t, 0.1), "quest": PG.paged_quest_decode(*a, meta, *t, L + bs, 0.1)}
+    some = [0] if B == 1 else [0, B // 2, B - 1]
+    want, mag, dots = O.attend(q[some], kc, vc, 0.1, 1.0, 1.0, table[some], n[some])
+    for name, out in outs.items():
+        got = out.double().cpu().reshape(B, Hq, D)
+        for (b, hk, d), x in at.items():
+            assert bool((got[b, 2 * hk:2 * hk + 2, d] == x).all()), (name, b, hk, d, x, got[b, 2 * hk:2 * hk + 2, d])
+        assert int((~torch.isfinite(got)).sum()) == 2 * len(at), name
+        fin = torch.isfinite(want)
+        assert bool(((got[some] - want).abs() <= _tol(want, mag, dots, D))[fin].all()), name
+
+
+def test_infinite_values_of_selected_pages(dev):
+    """The same where the pages are selected: the newest one, kept by the window, is in the last run."""
+    g = torch.Generator().manual_seed(77)
+    Hq, Hk, D, bs, L, kb = 4, 2, 64, 16, 5000, 1600
+    table, N = _table(g, [L], bs)
+    kc, vc = _make_cache(g, N, Hk, bs, D, False)
+    q, n = _rand(g, 1, Hq, 1, D), torch.tensor([L], dtype=torch.int32)
+    for d, p, x in ((7, L - 1, INF), (9, L - 8, -INF)):
+        vc[int(table[0, p // bs]), :, p % bs, d] = x
+    meta = tuple(t.to(dev) for t in _page_meta(kc, table, [L], bs))
+    out, pages = PG.paged_quest_decode(q.to(dev), kc.to(dev), vc.to(dev), meta, table.to(dev), n.to(dev), kb, 0.1,
+                                       local_w=1, return_pages=True)
+    assert bool((pages[..., -1] == (L - 1) // bs).all())
+    out = out.float().cpu()[0, :, 0]
+    assert bool((out[:, 7] == INF).all()) and bool((out[:, 9] == -INF).all())
+    assert int((~torch.isfinite(out)).sum()) == 2 * Hq
