@@ -167,19 +167,27 @@ struct PagedRows {
   }
 };
 
+// The number of 8 significant bits that x >= 0 starts with, as fp32 bits (a bf16
+// number's, 16 zeros below); BELOW: the largest that is less than x (0 for 0).
+template <bool BELOW>
+__device__ __forceinline__ uint32_t leading8(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (BELOW ? __builtin_elementwise_sub_sat(u, 1u) : u) & 0xFFFF0000u;
+}
+// bf16 pair of the upper halves of two fp32 numbers' bits.
+__device__ __forceinline__ uint32_t upper16(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+
 // One staged tile: scores, online softmax and values, as dense_compute, with each
-// weight as the sum of two bf16 numbers (at most 2^-16 of it is lost and not 2^-8): a
-// second product per value block, whose matrix instructions have time to spare
-// here.  Error of a long context's output against 64 bits: 0.0023 of its norm with
-// one, 0.0017, the rounding of the result itself, with two.
-// INF, values that can be infinite: the first is the bf16 number next below the
-// weight, so that both are positive wherever it is, and an infinite value that takes
-// part gives that infinity and not the NaN that 0 or a negative number times it would
-// add.  (The second is at most a step of the first, 2^-7 of the weight's power of
-// two.  A whole step is exact; what is smaller rounds by at most 2^-8 of half a
-// step.)  Else, e4m3 having no infinities, the first is the nearest one, which needs
-// fewer instructions (eight sequences of up to 8K over an fp8 cache: 18.4 us against
-// 17.8; bf16 caches, which wait for memory longer: no difference).
+// weight as the sum of three bf16 numbers, which hold its 24 bits: three products
+// per value block, whose matrix instructions have time to spare here (two, which lose
+// up to 2^-16 of a weight, and three, us: eight sequences of up to 8K 22.7 and 22.8,
+// four of 128K 245.8 and 246.3, 29 of up to 16K over an fp8 cache 116.9 and 117.2).
+// INF, values that can be infinite: the first two are the numbers next below what
+// they stand for, so that all three are positive wherever the weight is, and an
+// infinite value that takes part gives that infinity and not the NaN that 0 or a
+// negative number times it would add.  (What the first leaves is at most a whole step
+// of it, 2^16 units of the weight's last place, the second's remainder then one of
+// 2^8: either fits.)  Caches of e4m3, which has no infinities, need no such care.
 template <int D, bool INF>
 __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int lane, const bf16x8 (&qb)[D / 32],
                                            const char* kst, const char* vst, float& m_run, float& l_run,
@@ -209,37 +217,46 @@ __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int
   const float m_use = (m_new == kNegInf) ? 0.f : m_new;
   const float alpha = fast_exp2(m_run - m_use);
   float psum = 0.f;
-  u32x4 first;
-  bf16x8 hi, lo;
-  uint32_t below = 0u;
+  u32x4 w[3];                                      // the weights' parts, in pairs
+  uint32_t even[3];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const float p = fast_exp2(x[j] - m_use);
     psum += p;
-    if constexpr (INF) {
-      const uint32_t u = __builtin_elementwise_sub_sat(__float_as_uint(p), 1u) & 0xFFFF0000u;    // 0 stays 0
-      lo[j] = (__bf16)(p - __uint_as_float(u));
-      if (j & 1) first[j >> 1] = u | (below >> 16);
-      below = u;
-    } else {
-      hi[j] = (__bf16)p;
-      lo[j] = (__bf16)(p - (float)hi[j]);
+    uint32_t u[3];
+    u[0] = leading8<INF>(p);
+    const float r1 = p - __uint_as_float(u[0]);    // (exact, as is the next)
+    u[1] = leading8<INF>(r1);
+    u[2] = __float_as_uint(r1 - __uint_as_float(u[1]));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      if (j & 1) w[i][j >> 1] = upper16(even[i], u[i]);
+      else even[i] = u[i];
     }
   }
-  if constexpr (INF) hi = __builtin_bit_cast(bf16x8, first);
   l_run = l_run * alpha + psum;
   m_run = m_new;
-  // V^T through two transposed reads per block of 16 dims (tile_softmax_pv_at's layout)
+  // V^T through two transposed reads per block of 16 dims (tile_softmax_pv_at's
+  // layout), half of the blocks at a time: their products of one part do not wait for
+  // each other (eight sequences of up to 8K: 22.8 us, 23.2 with a block at a time)
+  constexpr int HALF = C::DB / 2;
   const StagedV<D> vaddr{vst};
 #pragma unroll
-  for (int db = 0; db < C::DB; ++db) {
-    acc[db] *= alpha;
-    u32x2 h[2];
+  for (int d0 = 0; d0 < C::DB; d0 += HALF) {
+    bf16x8 v[HALF];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) h[hf] = tr16(vaddr(hf, hf * 16 + lg * 4 + (l16 >> 2), db * 16 + (l16 & 3) * 4));
-    const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{h[0][0], h[0][1], h[1][0], h[1][1]});
-    acc[db] = mfma_bf16(v, hi, acc[db]);
-    acc[db] = mfma_bf16(v, lo, acc[db]);
+    for (int u = 0; u < HALF; ++u) {
+      u32x2 h[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+        h[hf] = tr16(vaddr(hf, hf * 16 + lg * 4 + (l16 >> 2), (d0 + u) * 16 + (l16 & 3) * 4));
+      v[u] = __builtin_bit_cast(bf16x8, u32x4{h[0][0], h[0][1], h[1][0], h[1][1]});
+      acc[d0 + u] *= alpha;
+    }
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+#pragma unroll
+      for (int u = 0; u < HALF; ++u) acc[d0 + u] = mfma_bf16(v[u], __builtin_bit_cast(bf16x8, w[i]), acc[d0 + u]);
   }
 }
 

@@ -786,3 +786,50 @@ def test_infinite_values_of_selected_pages(dev):
     out = out.float().cpu()[0, :, 0]
     assert bool((out[:, 7] == INF).all()) and bool((out[:, 9] == -INF).all())
     assert int((~torch.isfinite(out)).sum()) == 2 * Hq
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("W", [6, 40, 400])               # 4 and 8 waves of one workgroup, and the split over the grid
+@pytest.mark.parametrize("fp8", [False, True])
+def test_weights_are_fp32(dev, fp8, W, D):
+    """Values that cancel to 2^-14 of their size and less show what the weights lose.
+
+    Scores are exact (one product each, 0 the largest), so a weight is off by the
+    rounding of scale * log2(e) and of its product with a score of at most 1 in size
+    (2 * 2^-24 of 1.5, times ln 2: 3 * 2^-24 with what they do to each other), by the
+    exponential's unit (2 * 2^-24), and the sum by a rounding per addition: of at most
+    seven values (less than 27 * 2^-24 however a weight is cut into products).  Together
+    2^-19 of the weighted |v|, beside the rounding of the result."""
+    dt = F8 if fp8 else BF16
+    # scores whose weights two bf16 numbers miss by the most, upwards and downwards
+    up, down = (((0.140625, 0.021484375, 0.9375, 0.34375), (0.875, 0.46875, 0.109375, 0.625)) if fp8 else
+                ((0.71875, 0.96875, 0.84375, 0.296875), (0.671875, 0.8125, 0.390625, 0.359375)))
+    Hq, bs, m = 8, 16, 5
+    kc, vc = (torch.zeros(3, 1, bs, D) for _ in range(2))
+    q = torch.zeros(1, Hq, 1, D, dtype=BF16)
+    for h in range(Hq):                                   # head h looks at dim h of the keys, and alone at dims h + 8 i of the values
+        q[0, h, 0, h] = 1.0
+        a, b = up[h % 4], down[(h + h // 4) % 4]
+        kc[1, 0, 1, h], kc[1, 0, 2:2 + m, h] = -a, -b
+        for i, d in enumerate(range(h, D, 8)):
+            x = 128.0 + 16.0 * (i % 8) if fp8 else 1.0 + i / 16
+            vc[1, 0, 1, d] = x
+            rest = x * math.exp(0.5 * (b - a))
+            for j in range(m):                            # what the others take away again
+                y = float(torch.tensor(rest).to(dt).float())
+                vc[1, 0, 2 + j, d] = -y
+                rest -= y
+    assert torch.equal(kc.to(dt).float(), kc) and torch.equal(vc.to(dt).float(), vc)
+    kc, vc = kc.to(dt), vc.to(dt)
+    table = torch.full((1, W), -1, dtype=torch.int32)
+    table[0, 0] = 1
+    n = torch.tensor([2 + m], dtype=torch.int32)
+    meta = tuple(t.to(dev) for t in _page_meta(kc, table, [2 + m], bs))
+    want, mag, _ = O.attend(q, kc, vc, 0.5, 1.0, 1.0, table, n)
+    own = torch.arange(D)[None, None] % 8 == torch.arange(Hq)[None, :, None]
+    assert bool((want.abs() <= 2.0 ** -14 * mag)[own].all())
+    a, t = (q.to(dev), kc.to(dev), vc.to(dev)), (table.to(dev), n.to(dev))
+    for out in (PG.paged_decode_attn(*a, *t, 0.5), PG.paged_quest_decode(*a, meta, *t, 64, 0.5)):
+        err = (out.double().cpu().reshape(want.shape) - want).abs()
+        bad = ~(err <= 2.0 ** -8 * want.abs() + 2.0 ** -19 * mag)
+        assert not bool(bad.any()), float((err / mag)[bad].max())
