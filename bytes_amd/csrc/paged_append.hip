@@ -442,7 +442,8 @@ int bytes_paged_kv_append(const void* k, int64_t k_st, int64_t k_sh, const void*
                           int64_t cos_st, const void* sin, int64_t sin_st, int positions, int rot, int interleaved,
                           float k_scale, float v_scale, int T, int B, int Hq, int Hk, int D, int block_size,
                           int num_blocks, int max_blocks, void* stream) {
-  if (!k || !v || !k_paged || !v_paged || !block_table || !context_lens || T < 0 || B <= 0 || Hk <= 0 || Hq < 0)
+  if (!k || !v || !k_paged || !v_paged || !block_table || !context_lens || T < 0 || B <= 0 || Hk <= 0 || Hq < 0 ||
+      max_blocks <= 0)                             // (a table's first column is read for every token)
     return (int)hipErrorInvalidValue;
   if ((D != 64 && D != 128) || rot < 0 || rot > D || rot % 16 != 0 || (!cu_seqlens && T != B))
     return (int)hipErrorInvalidValue;

@@ -256,3 +256,13 @@ def test_c_entries_refuse(monkeypatch):
         return lib.bytes_paged_page_scores(q, 64, 64, p, p, p, W, p, p, 64, 64, B, Hq, Hk, D, bs, N, W, local, -1, 1.0, None)
     for bad in (dict(q=None), dict(B=0), dict(B=70000), dict(Hq=9), dict(D=100), dict(bs=0), dict(W=0), dict(local=-1)):
         assert scores(**bad), bad
+
+
+def test_append_entry_refuses_tables_without_columns():
+    """The append reads a table's first column also for tokens that have no position."""
+    lib, p = _lib.lib(), 64                           # never dereferenced: refused before a launch
+    c4 = (p, 64, 64, 64)
+    for W in (0, -1):
+        for cu, rot in ((None, 0), (p, 0), (None, 64), (p, 64)):
+            assert lib.bytes_paged_kv_append(p, 64, 64, p, 64, 64, p, 64, 64, p, 64, 64, *c4, *c4, 0, p, p, p, W, p, cu, p,
+                                             32, p, 32, 64, rot, 0, 1.0, 1.0, 3, 3, 8, 2, 64, 16, 12, W, None) == 1
