@@ -575,6 +575,13 @@ Tensor paged_quest(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   return out;
 }
 
+// Two tensors that are written: no two elements in one place.
+void written(const Tensor& a, const Tensor& b) {
+  for (const Tensor* t : {&a, &b})
+    for (int64_t d = 0; d < t->dim(); ++d) need(t->size(d) <= 1 || t->stride(d) != 0);
+  need(addr(a) != addr(b));
+}
+
 // The rotated queries, or True without any.
 PyObject* paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const Tensor& vp, const Tensor& bt,
                        const Tensor& cl, const Tensor* cu, const Tensor* q, const Tensor* cos, const Tensor* sin,
@@ -587,6 +594,7 @@ PyObject* paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const
   rows(k);
   rows(v);
   same_device(kp, {&k, &v});
+  written(kp, vp);
   if (cu) {
     need(shape(*cu, {B + 1}) && cu->scalar_type() == at::kInt && cu->is_contiguous());
     same_device(kp, {cu});
@@ -616,6 +624,7 @@ PyObject* paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const
       need(t->scalar_type() == at::kBFloat16 && shape(*t, {p.N, p.Hk, p.D}) && t->is_contiguous() && addr(*t) % 16 == 0);
       same_device(kp, {t});
     }
+    written(*kmin, *kmax);
   }
   c10::DeviceGuard guard(kp.device());
   Tensor out;

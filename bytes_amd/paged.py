@@ -95,6 +95,15 @@ def _meta(meta: Meta, N: int, Hk: int, D: int) -> Meta:
     return kmin, kmax
 
 
+def _written(a: torch.Tensor, b: torch.Tensor, names: Tuple[str, str]) -> None:
+    """Refuses two tensors that are written if two of their elements are in one place."""
+    for t, n in zip((a, b), names):
+        if any(t.size(d) > 1 and t.stride(d) == 0 for d in range(t.dim())):
+            raise ValueError(f"{n} is written: an expanded view, with several elements in one place, is not supported")
+    if a.data_ptr() == b.data_ptr():
+        raise ValueError(f"{names[0]} and {names[1]} are written and must not be the same memory")
+
+
 def _query(q: torch.Tensor, Hk: int, D: int):
     C.ndim(q, 4, "q")
     C.dtype_in(q, "q", torch.bfloat16)
@@ -141,8 +150,9 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
     q_rot.unsqueeze(2) is paged_decode_attn's query); zeros in rows that have no
     position.  Without q the result is None.
 
-    Blocks that receive tokens must belong to one sequence each (blocks of a
-    shared prefix are only read)."""
+    Blocks that receive tokens must belong to one sequence each, and be named once
+    in its table row (blocks of a shared prefix are only read).  The caches and
+    min / max must be memory of their own, without expanded dims."""
     kmin, kmax = meta if meta is not None else (None, None)
     out = native().paged_append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin,
                                 bool(interleaved), kmin, kmax, k_scale, v_scale)
@@ -185,8 +195,10 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
         if P < bt.shape[1] * bs:
             raise ValueError(f"cos, sin hold {P} positions, the block table {bt.shape[1] * bs}")
         cos, sin = C.rows16(cos), C.rows16(sin)
+    _written(k_paged, v_paged, ("k_paged", "v_paged"))
     if meta is not None:
         kmin, kmax = _meta(meta, N, Hk, D)
+        _written(kmin, kmax, ("kmin", "kmax"))
     k, v = C.rows16(k), C.rows16(v)
     out = None
     if q is not None:

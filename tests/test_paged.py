@@ -266,3 +266,28 @@ def test_append_entry_refuses_tables_without_columns():
         for cu, rot in ((None, 0), (p, 0), (None, 64), (p, 64)):
             assert lib.bytes_paged_kv_append(p, 64, 64, p, 64, 64, p, 64, 64, p, 64, 64, *c4, *c4, 0, p, p, p, W, p, cu, p,
                                              32, p, 32, 64, rot, 0, 1.0, 1.0, 3, 3, 8, 2, 64, 16, 12, W, None) == 1
+
+
+@pytest.mark.parametrize("change", [
+    _bad("blocks in one place", kc=lambda t: t[:1].expand(12, 2, 16, 64)),
+    _bad("heads in one place", vc=lambda t: t[:, :1].expand(12, 2, 16, 64)),
+    _bad("rows in one place", vc=lambda t: t[:, :, :1].expand(12, 2, 16, 64)),
+])
+def test_append_refuses_caches_that_overlap_themselves(calls, change):
+    """Two writes of one call to the same place; decode only reads and takes them."""
+    x = _inputs()
+    for n, f in change.items():
+        x[n] = f(x[n])
+    with pytest.raises(ValueError, match="expanded"):
+        _append(x)
+    assert not calls
+    assert _decode(x).shape == (3, 8, 1, 64)
+
+
+def test_append_refuses_one_tensor_for_two(calls):
+    x = _inputs()
+    for a, b in (("kc", "vc"), ("kmin", "kmax")):
+        with pytest.raises(ValueError, match="same memory"):
+            _append({**x, b: x[a]})
+    assert not calls
+    assert _decode({**x, "vc": x["kc"]}).shape == (3, 8, 1, 64)

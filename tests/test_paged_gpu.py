@@ -833,3 +833,16 @@ def test_weights_are_fp32(dev, fp8, W, D):
         err = (out.double().cpu().reshape(want.shape) - want).abs()
         bad = ~(err <= 2.0 ** -8 * want.abs() + 2.0 ** -19 * mag)
         assert not bool(bad.any()), float((err / mag)[bad].max())
+
+
+def test_append_refuses_memory_written_twice(dev):
+    """Expanded caches and one tensor for two, through the native call path and the wrapper."""
+    bf = lambda *s: torch.zeros(*s, dtype=BF16, device=dev)                  # noqa: E731
+    kc, vc, new = bf(4, 2, 16, 64), bf(4, 2, 16, 64), bf(1, 2, 64)
+    t, n = torch.zeros(1, 2, dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    mn, mx = bf(4, 2, 64), bf(4, 2, 64)
+    for k, v, m in ((kc[:1].expand(4, 2, 16, 64), vc, None), (kc, vc[:, :1].expand(4, 2, 16, 64), None), (kc, kc, None),
+                    (kc, vc, (mn, mn))):
+        with pytest.raises(ValueError):
+            PG.paged_kv_append(new, new, k, v, t, n, meta=m)
+    assert PG.paged_kv_append(new, new, kc, vc, t, n, meta=(mn, mx)) is None
