@@ -187,7 +187,10 @@ __device__ __forceinline__ uint32_t upper16(uint32_t lo, uint32_t hi) { return _
 // infinite value that takes part gives that infinity and not the NaN that 0 or a
 // negative number times it would add.  (What the first leaves is at most a whole step
 // of it, 2^16 units of the weight's last place, the second's remainder then one of
-// 2^8: either fits.)  Caches of e4m3, which has no infinities, need no such care.
+// 2^8: either fits.)  That holds down to weights of 2^-100 of the row's largest; where
+// one underflows fp32, here or as the factor of a rescaled or joined part, 0 times the
+// infinity is NaN, as in any fp32 evaluation.  Caches of e4m3, which has no infinities,
+// need no such care.
 template <int D, bool INF>
 __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int lane, const bf16x8 (&qb)[D / 32],
                                            const char* kst, const char* vst, float& m_run, float& l_run,

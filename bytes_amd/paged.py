@@ -226,8 +226,9 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
 
     q [B,H_q,1,D] bf16; `scale` as in decode_attn_bf16 (default 1.0; pass
     1/sqrt(D) for standard attention).  For fp8 caches the rows stand for
-    k * k_scale and v * v_scale.  fp32 scores, softmax and sums.  Returns
-    [B,H_q,1,D] bf16."""
+    k * k_scale and v * v_scale.  fp32 scores, softmax and sums.  An infinite value
+    that takes part gives that infinity, unless its weight underflows fp32 (below
+    2^-100 of the row's largest it may give NaN).  Returns [B,H_q,1,D] bf16."""
     out = native().paged_decode(q, k_paged, v_paged, block_table, context_lens, scale, k_scale, v_scale)
     if out is not None:
         return out

@@ -846,3 +846,30 @@ def test_append_refuses_memory_written_twice(dev):
         with pytest.raises(ValueError):
             PG.paged_kv_append(new, new, k, v, t, n, meta=m)
     assert PG.paged_kv_append(new, new, kc, vc, t, n, meta=(mn, mx)) is None
+
+
+@pytest.mark.parametrize("gap", [0, 40, 100])
+@pytest.mark.parametrize("L,W", [(40, 10), (600, 40), (3000, 300)])
+def test_infinite_values_of_small_weights(dev, gap, L, W):
+    """An infinite value stays one while its weight is at least 2^-100 of the largest, which
+    a token of the same tile, another wave's or a later part has."""
+    g = torch.Generator().manual_seed(gap + L)
+    Hq, Hk, D, bs = 2, 1, 64, 16
+    table, N = _table(g, [L, L], bs, slack=max(0, W - -(-L // bs)))
+    kc, vc = _make_cache(g, N, Hk, bs, D, False)
+    kc[..., 0] = -1.0                                     # every score is minus half the gap ..
+    q = torch.zeros(2, Hq, 1, D, dtype=BF16)
+    q[..., 0] = 1.0
+    for b, p in enumerate((20, L - 1)):                   # .. but one token's
+        kc[int(table[b, p // bs]), 0, p % bs, 0] = 1.0
+    for b in range(2):
+        vc[int(table[b, 0]), 0, 3, 5], vc[int(table[b, (L - 3) // bs]), 0, (L - 3) % bs, 6] = INF, -INF
+    scale = gap / 2 * math.log(2)
+    n = torch.tensor([L, L], dtype=torch.int32)
+    meta = tuple(t.to(dev) for t in _page_meta(kc, table, [L, L], bs))
+    a = (q.to(dev), kc.to(dev), vc.to(dev))
+    t = (table.to(dev), n.to(dev))
+    for out in (PG.paged_decode_attn(*a, *t, scale), PG.paged_quest_decode(*a, meta, *t, L + bs, scale)):
+        out = out.float().cpu()
+        assert bool((out[..., 5] == INF).all()) and bool((out[..., 6] == -INF).all())
+        assert int((~torch.isfinite(out)).sum()) == 2 * 2 * Hq
