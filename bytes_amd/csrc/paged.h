@@ -28,10 +28,6 @@ __device__ __forceinline__ int paged_len(const PagedKv& c, int b) {
   return n < 0 ? 0 : min(n, c.width * c.bs);
 }
 
-// NaN-propagating minimum and maximum (the page metadata's rule).
-__device__ __forceinline__ float nan_min(float a, float b) { return (a < b || a != a) ? a : b; }
-__device__ __forceinline__ float nan_max(float a, float b) { return (a > b || a != a) ? a : b; }
-
 // Folds v over the lanes that hold the same part of other rows, LPR lanes to a row:
 // rotations within the rows of 16, then the row and half swaps.  Every lane of the
 // wave takes part and receives the result.
