@@ -122,13 +122,15 @@ __device__ __forceinline__ void load_turn(const AppendArgs& a, const AppendItem&
     for (int e = 0; e < 4; ++e) r.c[4 * j + e] = x[e], r.s[4 * j + e] = y[e];
   }
 }
-// x0 c - x1 s from its exact products (8 by 24 bits), rounded to fp32 once.
+// x0 c - x1 s from its exact products (8 by 24 bits), rounded to fp32.
 __device__ __forceinline__ float turned_exact(double x0, double c, double x1, double s) {
   return (float)__builtin_fma(x0, c, -(x1 * s));
 }
-// EXACT for keys, which stay in the cache and in its min / max: with the products
-// rounded to fp32 one in some 2^16 came out on the other side of a bf16 step.
-// Queries, most of a prompt's rows, take fp32.
+// EXACT for keys, which stay in the cache and in its min / max.  The second rounding,
+// to bf16, takes one in some 2^17 of them to the other side of a bf16 step than one
+// rounding of the exact value would (those within half an fp32 step of a midpoint);
+// with the products rounded to fp32 too it is one in some 2^15.  Queries, most of a
+// prompt's rows, take fp32.
 template <bool EXACT>
 __device__ __forceinline__ void turn_item(const AppendArgs& a, const Turn& r, float* x) {
   float y[16];

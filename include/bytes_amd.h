@@ -491,7 +491,8 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  *   1.  The first rot dims (a multiple of 16) of keys and queries are rotated
  *   with row p of cos, sin (fp32 rows of rot / 2, row strides cos_st, sin_st;
  *   positions >= max_blocks * block_size rows): pairs (j, j + rot / 2), or
- *   (2j, 2j + 1) if interleaved; keys from the exact products.  fp8 rows hold
+ *   (2j, 2j + 1) if interleaved; keys from the exact products, rounded to fp32
+ *   and then to the cache's type.  fp8 rows hold
  *   k / k_scale and v / v_scale, held to +-448 (NaN stays NaN).  kmin, kmax
  *   [num_blocks, Hk, D] bf16 (or NULL): min / max of each block's stored keys,
  *   started anew where a token enters a block at its first row, else folded

@@ -873,3 +873,41 @@ def test_infinite_values_of_small_weights(dev, gap, L, W):
         out = out.float().cpu()
         assert bool((out[..., 5] == INF).all()) and bool((out[..., 6] == -INF).all())
         assert int((~torch.isfinite(out)).sum()) == 2 * 2 * Hq
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("single", [False, True])
+def test_stored_keys_are_the_exact_rotation(dev, single, interleaved):
+    """Keys in a bf16 cache bit for bit: the exact sum of the exact products, rounded to
+    fp32 and from there to bf16 (with the products rounded to fp32 some differ); their
+    min / max with them."""
+    g = torch.Generator().manual_seed(91 + single)
+    T, Hk, D, bs = 2048, 4, 128, 16
+    k = _rand(g, T, Hk, D)
+    W = 1 if single else T // bs
+    cos, sin = _cos_sin(W * bs, D, base=37.0)
+    if single:                                            # a token each, at every row of a block
+        table, n, cu = torch.arange(T, dtype=torch.int32)[:, None], torch.arange(T, dtype=torch.int32) % bs + 1, None
+        p = torch.arange(T) % bs
+    else:
+        table, n, cu = torch.randperm(W, generator=g).to(torch.int32)[None], torch.tensor([T], dtype=torch.int32), [0, T]
+        p = torch.arange(T)
+    N = table.numel()
+    kc, vc = (torch.zeros(N, Hk, bs, D, dtype=BF16, device=dev) for _ in range(2))
+    meta = tuple(torch.zeros(N, Hk, D, dtype=BF16, device=dev) for _ in range(2))
+    PG.paged_kv_append(k.to(dev), k.to(dev), kc, vc, table.to(dev), n.to(dev), cos=cos.to(dev), sin=sin.to(dev), meta=meta,
+                       cu_seqlens=None if cu is None else torch.tensor(cu, dtype=torch.int32, device=dev),
+                       interleaved=interleaved)
+    x, c, s = k.double(), cos.double()[p][:, None], sin.double()[p][:, None]
+    i = torch.arange(D // 2)
+    lo, hi = (2 * i, 2 * i + 1) if interleaved else (i, i + D // 2)
+    y = x.clone()
+    y[..., lo], y[..., hi] = x[..., lo] * c - x[..., hi] * s, x[..., hi] * c + x[..., lo] * s
+    want = y.float().to(BF16)
+    b = torch.arange(T) if single else torch.zeros(T, dtype=torch.long)
+    got = kc.cpu()[table[b, p // bs].long(), :, p % bs]
+    assert torch.equal(got, want)
+    if not single:
+        pages = want.reshape(W, bs, Hk, D).float()
+        assert torch.equal(meta[0].cpu()[table[0].long()].float(), pages.amin(1))
+        assert torch.equal(meta[1].cpu()[table[0].long()].float(), pages.amax(1))
