@@ -911,3 +911,112 @@ def test_stored_keys_are_the_exact_rotation(dev, single, interleaved):
         pages = want.reshape(W, bs, Hk, D).float()
         assert torch.equal(meta[0].cpu()[table[0].long()].float(), pages.amin(1))
         assert torch.equal(meta[1].cpu()[table[0].long()].float(), pages.amax(1))
+
+
+# ---------------------------------------------------------------------------
+# selection and page-sparse attention: every size of the selection, other layouts
+# ---------------------------------------------------------------------------
+def _want_pages(q, meta, table, n, bs, scale, npick):
+    """The best npick places per head by (bound descending, place ascending), ascending; from
+    sums of bf16 products in fp64."""
+    B, Hq, _, D = q.shape
+    Hk = meta[0].shape[1]
+    qd = q.double().reshape(B, Hk, Hq // Hk, D)
+    ids = table.clamp(min=0).long()
+    lo, hi = (m.double()[ids].permute(0, 2, 3, 1).nan_to_num(0) for m in meta)
+    b = (torch.matmul(qd.clamp(min=0), hi) + torch.matmul(qd.clamp(max=0), lo)).reshape(B, Hq, -1) * scale
+    b = b.float().masked_fill((torch.arange(table.shape[1]) * bs >= n[:, None])[:, None], -INF)
+    return b.argsort(dim=-1, descending=True, stable=True)[..., :npick].sort(-1).values
+
+
+@pytest.mark.parametrize("ties", [False, True])
+@pytest.mark.parametrize("npick", [1, 300, 1023, 1024, 2047, 2048, 4095])
+def test_quest_selection_sizes(dev, npick, ties):
+    """Sequences of 1023 to 4096 pages, at both ends of every size of the selection in the
+    attention kernel; ties: bounds of a few values only."""
+    g = torch.Generator().manual_seed(npick)
+    Hq, Hk, D = 4, 2, 64
+    lens = [1023, 1024, 1025, 2047, 2048, 2049, 4096, 3001]
+    table, N = _table(g, lens, 1, slack=0)
+    kc, vc = _make_cache(g, N, Hk, 1, D, False)
+    q = _rand(g, len(lens), Hq, 1, D)
+    if ties:
+        kc, q = (torch.randint(0, 2, x.shape, generator=g).to(BF16) for x in (kc, q))
+    n = torch.tensor(lens, dtype=torch.int32)
+    meta = (kc[:, :, 0].contiguous(), kc[:, :, 0].contiguous().clone())      # pages of one token
+    a = (q.to(dev), kc.to(dev), vc.to(dev), tuple(m.to(dev) for m in meta), table.to(dev), n.to(dev), npick, 0.125)
+    alone = PG.paged_quest_decode(*a)                     # selects in the attention kernel
+    out, pages = PG.paged_quest_decode(*a, return_pages=True)
+    want = _want_pages(q, meta, table, n, 1, 0.125, npick)
+    assert torch.equal(pages.cpu().long(), want) and torch.equal(alone, out)
+    _check_decode(dev, alone, q, kc, vc, 0.125, 1.0, 1.0, table, n,
+                  [[set(want[b, h].tolist()) for h in range(Hq)] for b in range(len(lens))])
+
+
+@pytest.mark.parametrize("W,L,npick", [(4096, 4096, 4095), (5000, 4990, 4980)])
+def test_quest_runs_of_as_many_pages_as_a_list_holds(dev, W, L, npick):
+    """So many heads and pages of one token that a run of a head's picks is bounded by the
+    kernel's list and not by the grid."""
+    g = torch.Generator().manual_seed(W)
+    B, Hq, Hk, D = 16, 64, 1, 64
+    table = torch.randperm(W, generator=g).to(torch.int32)[None].expand(B, W).contiguous()
+    kc, vc = _make_cache(g, W, Hk, 1, D, False)
+    q = _rand(g, B, Hq, 1, D)
+    n = torch.tensor([L - 2 * b for b in range(B)], dtype=torch.int32)
+    meta = (kc[:, :, 0].contiguous(), kc[:, :, 0].contiguous().clone())
+    a = (q.to(dev), kc.to(dev), vc.to(dev), tuple(m.to(dev) for m in meta), table.to(dev), n.to(dev), npick, 0.125)
+    alone = PG.paged_quest_decode(*a)
+    out, pages = PG.paged_quest_decode(*a, return_pages=True)
+    assert torch.equal(alone, out)
+    some, heads = [0, 7, 15], [0, 9, 63]
+    sub = q[some][:, heads]
+    want = _want_pages(sub, meta, table[some], n[some], 1, 0.125, npick)
+    assert torch.equal(pages.cpu().long()[some][:, heads], want)
+    _check_decode(dev, alone[some][:, heads], sub, kc, vc, 0.125, 1.0, 1.0, table[some], n[some],
+                  [[set(want[b, h].tolist()) for h in range(3)] for b in range(3)])
+
+
+@pytest.mark.parametrize("pages,npick", [(1001, 7), (2047, 500), (4093, 4000)])
+def test_quest_c_entries_with_unpadded_bounds(dev, pages, npick):
+    """The C entries on bounds whose rows are not whole 16-byte chunks: the wrapper's bits."""
+    g = torch.Generator().manual_seed(pages)
+    B, Hq, Hk, D, bs = 2, 6, 2, 64, 1
+    table, N = _table(g, [pages, pages - 1], bs, slack=0)
+    kc, vc = (c.to(dev) for c in _make_cache(g, N, Hk, bs, D, False))
+    q = _rand(g, B, Hq, 1, D).to(dev)
+    table, n = table.to(dev), torch.tensor([pages, pages - 1], dtype=torch.int32, device=dev)
+    meta = (kc[:, :, 0].contiguous(), kc[:, :, 0].contiguous().clone())
+    want = PG.paged_quest_decode(q, kc, vc, meta, table, n, npick, 0.125)
+    bound = PG.paged_page_scores(q, meta, table, n, bs, 0.125)
+    assert bound.shape[-1] % 4 and bound.stride(1) == pages
+    size = _lib.size_query("bytes_paged_quest_workspace_size", B, Hq, Hk, D, 0, bs, pages, npick)
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+    out = torch.empty(B, Hq, D, dtype=BF16, device=dev)
+    p = _lib.ptr
+    _lib.call("bytes_paged_quest_attn", p(q), q.stride(0), q.stride(1), p(kc), kc.stride(0), kc.stride(1), kc.stride(2),
+              p(vc), vc.stride(0), vc.stride(1), vc.stride(2), 0, p(bound), bound.stride(0), bound.stride(1), None, 0, 0,
+              npick, p(table), table.stride(0), p(n), p(out), out.stride(0), out.stride(1), B, Hq, Hk, D, bs, N, pages,
+              0.125, 1.0, p(ws), ws.numel(), _lib.stream_of(q))
+    assert torch.equal(out.unsqueeze(2), want)
+
+
+@pytest.mark.parametrize("layout", ["nshd", "pair"])
+@pytest.mark.parametrize("Hq,Hk,D,bs,fp8", [(14, 2, 64, 16, False), (7, 1, 128, 32, True), (6, 3, 128, 5, False),
+                                            (8, 8, 64, 64, True)])
+def test_quest_decode_of_strided_caches(dev, Hq, Hk, D, bs, fp8, layout):
+    g = torch.Generator().manual_seed(bs + D)
+    lens = [700, 0, 333]
+    table, N = _table(g, lens, bs)
+    kc, vc = _make_cache(g, N, Hk, bs, D, fp8, layout)
+    q, n = _rand(g, 3, Hq, 1, D), torch.tensor(lens, dtype=torch.int32)
+    meta = _page_meta(kc, table, lens, bs)
+    ks, vs = (0.03, 0.05) if fp8 else (1.0, 1.0)
+    for kb in (128, 10 ** 5):
+        out, pages = PG.paged_quest_decode(q.to(dev), _keep_storage(kc, dev), _keep_storage(vc, dev),
+                                           tuple(m.to(dev) for m in meta), table.to(dev), n.to(dev), kb, D ** -0.5,
+                                           k_scale=ks, v_scale=vs, return_pages=True)
+        npick = min(-(-kb // bs), table.shape[1])
+        want = _want_pages(q, meta, table, n, bs, D ** -0.5 * ks, npick)
+        assert torch.equal(pages.cpu().long(), want)
+        _check_decode(dev, out, q, kc, vc, D ** -0.5, ks, vs, table, n,
+                      [[set(want[b, h].tolist()) for h in range(Hq)] for b in range(3)])
