@@ -22,6 +22,12 @@
 //    without atomics or a second read.  Spans are numbered over the batch; every
 //    wave finds its own from a prefix sum over the sequences, rows past the last
 //    sequence being one more.
+//    Made for blocks of 8 to 64 rows where min / max are kept: of smaller ones a wave
+//    has few rows, of larger ones many in turn (us, four chunks of 1 to 2K tokens of
+//    28 + 2 x 4 heads of 128 and of 14 + 2 x 2 of 64, from a graph: without min / max 25
+//    and 10 with any block; with them, blocks of 1 row 59 and 33, of 2 40 and 21, of 4
+//    31 and 14, of 8 27 and 12, of 16 26 and 12, of 64 26 and 13, of 128 35 and 18, of
+//    256 55 and 27, of 1024 172 and 86).
 // Bound by memory: a 32K-token prompt of 32 query and 8 KV heads (0.4 GB read, 0.4
 // GB written) takes 160 us, 5.1 TB/s; a plain copy of 2 GiB runs at 4.9.
 #include "paged.h"

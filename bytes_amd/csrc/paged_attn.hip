@@ -21,7 +21,7 @@
 // launch (short_waves).
 // Bound by memory: four sequences of 64K to 128K (8 KV heads of 128, 1.6 GB) take 245
 // us, 6.6 TB/s, where streaming reads reach 7.1; 29 of 6.6K to 16K over an fp8 cache (0.68
-// GB) 116, 5.9 TB/s.  Eight of 3.4K to 8K (95 MB) take 22, six tiles per wave between a
+// GB) 116, 5.9 TB/s.  Eight of 3.4K to 8K (95 MB) take 23, six tiles per wave between a
 // start and an end that stream nothing, and the join.
 #include "paged.h"
 
@@ -221,7 +221,8 @@ static int decode_grid(int64_t units, int64_t granules_max) {
 
 // Waves of a workgroup that does a whole unit by itself (one launch, no parts to
 // join), or 0 for the even split.  By the bytes of a full table row, which one CU
-// reads at about 50 GB/s: up to 256 KB (us, whole unit and split: one sequence of
+// reads at about 50 GB/s: up to 256 KB (us from a graph, so without what a second
+// launch costs the host; whole unit and split: one sequence of
 // 2 KV heads of 64, 500 tokens 5.7 and 7.1, 1000 tokens 8.0 and 7.1; of 4 heads of
 // 128, 500 tokens 7.8 and 8.3, 1000 tokens 13.4 and 8.9), twice that where the
 // units keep half the CUs busy anyway (64 sequences of 4 heads of 128, 500 tokens

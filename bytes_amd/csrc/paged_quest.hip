@@ -53,10 +53,12 @@ __device__ __forceinline__ double bound_literal(const uint16_t* q, const uint16_
 // A and B agree); q's parts are widened once per workgroup, in LDS.  The result is
 // at lane: head l / 16, block l % 16.  A tile with an infinite or NaN entry, where
 // the part of q that is 0 would give NaN, takes the literal sum.
-// Bound by memory for large batches: 44 MB of min / max (seven sequences of 32K to 64K,
-// 8 KV heads of 128, blocks of 32) take 16.5 us from a graph, 12.4 of them the loads
-// alone; with the sums on the vector unit 24.  One sequence of 32K (4.2 MB): 5.2, launch and round trips; two tiles per wave,
-// half the waves, 7.7 (and 17.2 for the 44 MB).
+// Bound by its loads and then its products for large batches: 44 MB of min / max (seven
+// sequences of 32K to 64K, 8 KV heads of 128, blocks of 32) take 16.5 us from a graph,
+// 12.4 of them the loads alone (3.5 TB/s, in pieces of 256 bytes: the heads of a block
+// are different workgroups'); with the sums on the vector unit 24.  One sequence of
+// 32K (4.2 MB): 5.2, launch and round trips; two tiles per wave, half the waves, 7.7
+// (and 17.2 for the 44 MB).
 template <int D, int NG>
 __global__ __launch_bounds__(kBoundWaves * 64, 4) void page_bound_kernel(PageBoundArgs a) {
   PREFETCH_ARGS(a);
@@ -253,10 +255,13 @@ __device__ __forceinline__ void add_chunk(const u32x4& v, float p, float (&acc)[
 // throughout), and groups and waves are merged at the end.  No LDS stage, so
 // registers alone bound the waves in flight.  RUNS: block sizes that are multiples of
 // RPI, whose instructions' rows lie in one block and start at a scalar address.
-// Bound by reads of short runs of rows anywhere in the cache: 2048 of 32K to 64K
-// fp8 tokens of 7 x 24 heads (84 MB of distinct rows) take 24 us, 3.5 TB/s, 4 of
-// them the selection; 2048 of 32K bf16 tokens of 28 heads (24 MB) 10.5.  With two tiles
-// in flight per wave a whole call takes 53 for 46.5 and 22 for 20.
+// Bound by what a run does besides streaming: every run of a head begins with the
+// selection, while no row is in flight, and has few tiles per wave, each issued when
+// the one before is done.  2048 of 32K to 64K fp8 tokens of 7 x 24 heads (84 MB of
+// distinct rows) take 24 us, 3.5 TB/s, 4 of them the selection; 2048 of 32K bf16 tokens
+// of 28 heads (24 MB) 10.5.  (That blocks lie anywhere is not it: the decode reads
+// blocks of 16 rows in the same order at 6.6.)  With two tiles in flight per wave a
+// whole call takes 53 for 46.5 and 22 for 20.
 template <int D, bool FP8, bool RUNS>
 __global__ __launch_bounds__(kPickThreads, 4) void paged_quest_kernel(PagedQuestArgs a) {
   using P = PickCfg<D, FP8>;

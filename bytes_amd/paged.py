@@ -12,8 +12,9 @@ sequence b is row p % block_size of block block_table[b, p // block_size].
 operator here: the append takes it with the new tokens counted, so one tensor
 serves a whole decode step.  Lengths, block tables and cu_seqlens stay on the
 device; nothing here synchronises, and every call can be captured in a graph
-(lengths and tables are read at replay).  Lengths are held to 0 .. max_blocks *
-block_size.  A block id outside [0, num_blocks) names no block (-1 past a
+(lengths and tables are read at replay).  The decodes hold lengths to 0 .. max_blocks *
+block_size; the append takes them as they are, and new tokens at positions outside
+that range are not written.  A block id outside [0, num_blocks) names no block (-1 past a
 sequence's blocks, or a hole where a block was evicted): nothing is written for
 its tokens and they take no part in attention.  A sequence none of whose tokens
 take part (length 0, as in the padding rows of a batch) gets zeros.
@@ -294,9 +295,11 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     """quest_decode over a paged cache whose blocks are the pages: the
     ceil(kb / block_size) blocks of the highest bounds per query head
     (paged_page_scores; the lowest block first on equal bounds), exact attention over
-    their tokens.  A sequence of fewer blocks is attended over whole.  q
-    [B,H_q,1,D] bf16; meta as paged_kv_append keeps it.  Returns out [B,H_q,1,D]
-    bf16 (and the selected blocks' places in the table, int32
+    their tokens.  A sequence of fewer blocks is attended over whole.  The blocks of
+    the last local_w tokens are all equally best, so a window of more blocks than are
+    picked loses its newest ones, as in quest_decode: take kb of at least local_w +
+    block_size.  q [B,H_q,1,D] bf16; meta as paged_kv_append keeps it.  Returns out
+    [B,H_q,1,D] bf16 (and the selected blocks' places in the table, int32
     [B,H_q,min(ceil(kb / block_size), max_blocks)] ascending, if return_pages;
     places past a short sequence's blocks stand for nothing)."""
     if not return_pages:

@@ -479,11 +479,12 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  * value * k_scale (v_scale); strides *_sb, *_sh, *_ss per block, KV head and
  * row.  Token p of sequence b is row p % block_size of block
  * block_table[b * bt_sb + p / block_size] (int32, max_blocks columns);
- * sequence b holds context_lens[b] tokens (int32), held to 0 .. max_blocks *
- * block_size.  Block ids outside [0, num_blocks) name no block: nothing is
+ * sequence b holds context_lens[b] tokens (int32; the decodes hold them to 0 ..
+ * max_blocks * block_size, new tokens at positions outside that range are not
+ * written).  Block ids outside [0, num_blocks) name no block: nothing is
  * written for their tokens, and they take no part.  Lengths, tables and
  * cu_seqlens are device memory, read when the kernels run.  D in {64, 128};
- * max_blocks * block_size <= 2^30.
+ * max_blocks >= 1, max_blocks * block_size <= 2^30.
  *
  * bytes_paged_kv_append: k, v [T, Hk, D] bf16 (strides *_st, *_sh), the new
  *   tokens of B sequences: rows cu_seqlens[b] .. cu_seqlens[b + 1], or row b
@@ -497,7 +498,9 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  *   [num_blocks, Hk, D] bf16 (or NULL): min / max of each block's stored keys,
  *   started anew where a token enters a block at its first row, else folded
  *   into.  q [T, Hq, D] bf16 (or NULL with Hq = 0): rotated into q_out; rows
- *   without a position get zeros.
+ *   without a position get zeros.  What is written (caches, kmin, kmax, q_out)
+ *   overlaps neither itself nor another argument, and a block that receives tokens
+ *   is named once.
  * bytes_paged_decode_attn: out [B, Hq, D] bf16 (strides o_sb, o_sh) =
  *   v_scale * softmax(scale * q . K^T) V over the tokens that take part, zeros
  *   where none does; q [B, Hq, D] bf16.  (scale includes the cache's k_scale.)
@@ -510,7 +513,8 @@ int bytes_pq_kmeans_update(const void* x, int heads, int64_t n, int D, int K, co
  *   not written).
  * bytes_paged_quest_attn: bytes_paged_decode_attn over the tokens of npick
  *   blocks per query head: the best of bound (as bytes_paged_page_scores gives
- *   them, skip <= npick; bound descending, lowest place first on equal bounds;
+ *   them, skip <= npick; bound descending, lowest place first on equal bounds, so
+ *   also among the +inf of a window of more than npick blocks;
  *   max_blocks <= 16384, hipErrorNotSupported above; sequences of at most npick
  *   blocks whole; where b_sb, b_sh are multiples of 4 and b_sh at least
  *   max_blocks rounded up to one, rows are read in whole 16-byte chunks), or,

@@ -1020,3 +1020,23 @@ def test_quest_decode_of_strided_caches(dev, Hq, Hk, D, bs, fp8, layout):
         assert torch.equal(pages.cpu().long(), want)
         _check_decode(dev, out, q, kc, vc, D ** -0.5, ks, vs, table, n,
                       [[set(want[b, h].tolist()) for h in range(Hq)] for b in range(3)])
+
+
+def test_window_of_more_blocks_than_are_picked(dev):
+    """All blocks of the window are equally best, the lowest first; kb of local_w +
+    block_size tokens always reaches the newest."""
+    g = torch.Generator().manual_seed(61)
+    Hq, Hk, D, bs, lens = 4, 2, 64, 16, [1000, 993, 992, 40]
+    table, N = _table(g, lens, bs)
+    kc, vc = _make_cache(g, N, Hk, bs, D, False)
+    q, n = _rand(g, 4, Hq, 1, D).to(dev), torch.tensor(lens, dtype=torch.int32)
+    meta = tuple(m.to(dev) for m in _page_meta(kc, table, n, bs))
+    a = (q, kc.to(dev), vc.to(dev), meta, table.to(dev), n.to(dev))
+    w = 100
+    _, pages = PG.paged_quest_decode(*a, 64, 0.125, local_w=w, return_pages=True)
+    for b in range(3):
+        first = (lens[b] - w) // bs
+        assert bool((pages[b].cpu() == torch.arange(first, first + 4)).all())
+    _, pages = PG.paged_quest_decode(*a, w + bs, 0.125, local_w=w, return_pages=True)
+    for b in range(3):
+        assert bool((pages[b, :, -1] == (lens[b] - 1) // bs).all())
