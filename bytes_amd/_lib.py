@@ -176,6 +176,37 @@ SIGNATURES: Dict[str, Tuple] = {
         c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,                   # block table, row stride, lengths, out + strides
         c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, Hq, Hk, D, block size, blocks, max blocks
         c_f32, c_f32, c_vp, c_sz, c_vp),                         # scale, v_scale, workspace, bytes, stream
+    "bytes_paged_kv_append_blocks": (
+        c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,                  # k, v + strides (token, head)
+        c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,                  # q, q_out + strides (token, head)
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)
+        c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,           # cache type, scales + strides (block, head)
+        c_vp, c_i64, c_vp, c_vp,                                 # block table, row stride, lengths, cu_seqlens
+        c_vp, c_i64, c_vp, c_i64, c_int, c_int, c_int,           # cos, sin + row strides, positions, rot, interleaved
+        c_int, c_int, c_int, c_int, c_int,                       # T, B, Hq, Hk, D
+        c_int, c_int, c_int, c_vp),                              # block size, blocks, max blocks, stream
+    "bytes_paged_window_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
+    "bytes_paged_window_attn": (
+        c_vp, c_i64, c_i64,                                      # q, strides (b, h)
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)
+        c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,           # cache type, scales + strides (block, head)
+        c_vp, c_i64, c_vp, c_vp, c_i64, c_i64,                   # block table, row stride, lengths, out, strides (b, h)
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, Hq, Hk, D, block size, blocks, max blocks
+        c_int, c_int, c_f32, c_f32, c_vp, c_sz, c_vp),           # window, sinks, scale, v_scale, workspace, bytes, stream
+    "bytes_paged_prompt_workspace_size": (c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_szp),
+    "bytes_paged_prompt_attn": (
+        c_vp, c_i64, c_i64,                                      # q, strides (token, head)
+        c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_i64, c_i64,    # k_paged, v_paged + strides (block, head, row)
+        c_int, c_vp, c_i64, c_i64, c_vp, c_i64, c_i64,           # cache type, scales + strides (block, head)
+        c_vp, c_i64, c_vp, c_vp, c_vp, c_i64, c_i64,             # table, row stride, lengths, cu_seqlens, out, strides
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,  # T, B, Hq, Hk, D, block size, blocks, max blocks
+        c_int, c_int, c_f32, c_f32, c_vp, c_sz, c_vp),           # window, sinks, scale, v_scale, workspace, bytes, stream
+    "bytes_paged_resize_workspace_size": (c_int, c_szp),
+    "bytes_paged_resize": (
+        c_vp, c_i64, c_vp, c_vp, c_vp,                           # block table, row stride, lengths, free blocks, free range
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,                # keep, new, cu_seqlens, granted, seqs, positions, slots
+        c_int, c_int, c_int, c_int, c_int, c_int, c_int,         # B, max blocks, blocks, T, block size, window, sinks
+        c_vp, c_sz, c_vp),                                       # workspace, bytes, stream
 }
 _RESTYPES = {"bytes_error_string": ctypes.c_char_p}
 

@@ -23,8 +23,10 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <utility>
 
 #include "../../../include/bytes_amd.h"
 
@@ -642,6 +644,196 @@ PyObject* paged_append(const Tensor& k, const Tensor& v, const Tensor& kp, const
   return THPVariable_Wrap(out);
 }
 
+// A cache of any kind: a scale for the tensor, or one for each block and KV head.
+struct TypedPaged {
+  Paged p;
+  int type;                              // as the C ABI's kv_type
+  const Tensor *ks, *vs;                 // tensors of scales, or null
+  double k_scale, v_scale;               // else these
+
+  const void* kptr() const { return ks ? ks->const_data_ptr() : nullptr; }
+  const void* vptr() const { return vs ? vs->const_data_ptr() : nullptr; }
+  int64_t kst(int d) const { return ks ? ks->stride(d) : 0; }
+  int64_t vst(int d) const { return vs ? vs->stride(d) : 0; }
+};
+TypedPaged typed_paged(const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& cl, int64_t B, PyObject* ks,
+                       PyObject* vs) {
+  TypedPaged t{};
+  t.k_scale = t.v_scale = 1.0;
+  if (!THPVariable_Check(ks) && !THPVariable_Check(vs)) {
+    t.k_scale = number(ks), t.v_scale = number(vs);
+    t.p = paged(k, v, bt, cl, B, t.k_scale, t.v_scale);
+    t.type = t.p.f8 ? 1 : 0;
+    return t;
+  }
+  t.ks = &tensor(ks), t.vs = &tensor(vs);
+  const bool i8 = k.scalar_type() == at::kChar;
+  need((i8 || k.scalar_type() == kF8) && v.scalar_type() == k.scalar_type() && k.dim() == 4 && v.sizes() == k.sizes());
+  t.p = Paged{k.size(0), k.size(1), k.size(2), k.size(3), !i8, bt.dim() == 2 ? bt.size(1) : 0};
+  const Paged& p = t.p;
+  need(p.N > 0 && p.N <= 0x7FFFFFFF && p.Hk > 0 && p.bs > 0 && head_dim(p.D));
+  rows(k);
+  rows(v);
+  need(bt.dim() == 2 && bt.size(0) == B && bt.scalar_type() == at::kInt && (bt.stride(1) == 1 || p.W == 1) && p.W > 0);
+  need(shape(cl, {B}) && cl.scalar_type() == at::kInt && cl.is_contiguous());
+  need(p.bs <= (1 << 30) && p.W * p.bs <= (1 << 30));
+  for (const Tensor* s : {t.ks, t.vs}) need(s->scalar_type() == at::kFloat && shape(*s, {p.N, p.Hk}));
+  same_device(k, {&v, &bt, &cl, t.ks, t.vs});
+  t.type = i8 ? 3 : 2;
+  return t;
+}
+// (window, sinks) as the C ABI takes them.
+std::pair<int, int> window_of(PyObject* window, PyObject* sinks) {
+  const long s = integer(sinks);
+  if (window == Py_None) {
+    need(s == 0);
+    return {1 << 30, 0};
+  }
+  const long w = integer(window);
+  need(w >= 1 && s >= 0);
+  return {(int)std::min(w, 1L << 30), (int)std::min(s, 1L << 30)};
+}
+
+Tensor paged_window(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& cl, double scale,
+                    PyObject* window, PyObject* sinks, PyObject* ks, PyObject* vs) {
+  paged_query(q, k);
+  const int64_t B = q.size(0), Hq = q.size(1);
+  const TypedPaged t = typed_paged(k, v, bt, cl, B, ks, vs);
+  const Paged& p = t.p;
+  const auto [w, s] = window_of(window, sinks);
+  c10::DeviceGuard guard(q.device());
+  size_t n = 0;
+  need(bytes_paged_window_workspace_size(B, Hq, p.Hk, p.D, t.type, p.bs, p.W, w, s, &n) == 0);
+  Tensor ws;                                             // the call's own: calls on other streams share nothing
+  if (n) ws = empty(q, {(int64_t)n}, at::kByte);
+  Tensor out = empty(q, {B, Hq, 1, p.D}, at::kBFloat16);
+  void* st = stream_of(q);
+  launch("bytes_paged_window_attn", bytes_paged_window_attn, data(q), q.stride(0), q.stride(1), data(k), k.stride(0),
+         k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), t.type, t.kptr(), t.kst(0), t.kst(1),
+         t.vptr(), t.vst(0), t.vst(1), data(bt), bt.stride(0), data(cl), out.mutable_data_ptr(), out.stride(0),
+         out.stride(1), B, Hq, p.Hk, p.D, p.bs, p.N, p.W, w, s, (float)(scale * t.k_scale), (float)t.v_scale,
+         n ? ws.mutable_data_ptr() : nullptr, n, st);
+  return out;
+}
+
+Tensor paged_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& bt, const Tensor& cl,
+                    const Tensor& cu, double scale, PyObject* window, PyObject* sinks, PyObject* ks, PyObject* vs) {
+  need(q.dim() == 3 && q.scalar_type() == at::kBFloat16 && q.size(0) > 0 && q.size(0) <= (1 << 30) && q.size(1) > 0 &&
+       k.dim() == 4 && q.size(2) == k.size(3) && k.size(1) > 0 && q.size(1) % k.size(1) == 0);
+  need(bt.dim() == 2 && bt.size(0) > 0);
+  rows(q);
+  const int64_t T = q.size(0), Hq = q.size(1), B = bt.size(0);
+  const TypedPaged t = typed_paged(k, v, bt, cl, B, ks, vs);
+  const Paged& p = t.p;
+  need(shape(cu, {B + 1}) && cu.scalar_type() == at::kInt && cu.is_contiguous());
+  same_device(k, {&q, &cu});
+  const auto [w, s] = window_of(window, sinks);
+  c10::DeviceGuard guard(q.device());
+  size_t n = 0;
+  need(bytes_paged_prompt_workspace_size(T, B, Hq, p.Hk, p.D, p.bs, p.W, w, s, &n) == 0);
+  Tensor ws;
+  if (n) ws = empty(q, {(int64_t)n}, at::kByte);
+  Tensor out = empty(q, {T, Hq, p.D}, at::kBFloat16);
+  void* st = stream_of(q);
+  launch("bytes_paged_prompt_attn", bytes_paged_prompt_attn, data(q), q.stride(0), q.stride(1), data(k), k.stride(0),
+         k.stride(1), k.stride(2), data(v), v.stride(0), v.stride(1), v.stride(2), t.type, t.kptr(), t.kst(0), t.kst(1),
+         t.vptr(), t.vst(0), t.vst(1), data(bt), bt.stride(0), data(cl), data(cu), out.mutable_data_ptr(), out.stride(0),
+         out.stride(1), T, B, Hq, p.Hk, p.D, p.bs, p.N, p.W, w, s, (float)(scale * t.k_scale), (float)t.v_scale,
+         n ? ws.mutable_data_ptr() : nullptr, n, st);
+  return out;
+}
+
+// The rotated queries, or True without any.
+PyObject* paged_append_blocks(const Tensor& k, const Tensor& v, const Tensor& kp, const Tensor& vp, const Tensor& bt,
+                              const Tensor& cl, const Tensor* cu, const Tensor* q, const Tensor* cos, const Tensor* sin,
+                              bool interleaved, PyObject* ks, PyObject* vs) {
+  need(THPVariable_Check(ks) && THPVariable_Check(vs));
+  need(k.dim() == 3 && v.sizes() == k.sizes() && k.scalar_type() == at::kBFloat16 && v.scalar_type() == at::kBFloat16);
+  need(bt.dim() == 2 && bt.size(0) > 0);
+  const int64_t T = k.size(0), B = bt.size(0);
+  const TypedPaged t = typed_paged(kp, vp, bt, cl, B, ks, vs);
+  const Paged& p = t.p;
+  need(T > 0 && T <= 0x7FFFFFFF && k.size(1) == p.Hk && k.size(2) == p.D);
+  rows(k);
+  rows(v);
+  same_device(kp, {&k, &v});
+  written(kp, vp);
+  written(*t.ks, *t.vs);
+  if (cu) {
+    need(shape(*cu, {B + 1}) && cu->scalar_type() == at::kInt && cu->is_contiguous());
+    same_device(kp, {cu});
+  } else {
+    need(T == B);
+  }
+  int64_t Hq = 0, rot = 0, P = 0;
+  if (q) {
+    need(q->dim() == 3 && q->scalar_type() == at::kBFloat16);
+    Hq = q->size(1);
+    need(shape(*q, {T, Hq, p.D}) && Hq > 0);
+    rows(*q);
+    same_device(kp, {q});
+  }
+  need(!cos == !sin);
+  if (cos) {
+    need(cos->dim() == 2 && sin->sizes() == cos->sizes() && cos->scalar_type() == at::kFloat &&
+         sin->scalar_type() == at::kFloat);
+    P = cos->size(0), rot = 2 * cos->size(1);
+    need(rot > 0 && rot % 16 == 0 && rot <= p.D && P >= p.W * p.bs && P <= 0x7FFFFFFF);
+    rows(*cos);
+    rows(*sin);
+    same_device(kp, {cos, sin});
+  }
+  c10::DeviceGuard guard(kp.device());
+  Tensor out;
+  if (q) out = empty(*q, {T, Hq, p.D}, at::kBFloat16);
+  void* st = stream_of(kp);
+  launch("bytes_paged_kv_append_blocks", bytes_paged_kv_append_blocks, data(k), k.stride(0), k.stride(1), data(v),
+         v.stride(0), v.stride(1), q ? data(*q) : nullptr, q ? q->stride(0) : 0, q ? q->stride(1) : 0,
+         q ? out.mutable_data_ptr() : nullptr, q ? out.stride(0) : 0, q ? out.stride(1) : 0, kp.mutable_data_ptr(),
+         kp.stride(0), kp.stride(1), kp.stride(2), vp.mutable_data_ptr(), vp.stride(0), vp.stride(1), vp.stride(2), t.type,
+         t.ks->mutable_data_ptr(), t.kst(0), t.kst(1), t.vs->mutable_data_ptr(), t.vst(0), t.vst(1), data(bt),
+         bt.stride(0), data(cl), cu ? data(*cu) : nullptr, cos ? data(*cos) : nullptr, cos ? cos->stride(0) : 0,
+         sin ? data(*sin) : nullptr, sin ? sin->stride(0) : 0, (int)P, (int)rot, interleaved, (int)T, (int)B, (int)Hq,
+         (int)p.Hk, (int)p.D, (int)p.bs, (int)p.N, (int)p.W, st);
+  if (!q) Py_RETURN_TRUE;
+  return THPVariable_Wrap(out);
+}
+
+// (cu_seqlens, granted, seqs, positions, slots)
+PyObject* paged_resize(const Tensor& bt, const Tensor& cl, const Tensor& ring, const Tensor& range, const Tensor& fresh,
+                       const Tensor* keep, long T, long bs, long window, long sinks) {
+  need(bt.dim() == 2 && bt.size(0) > 0 && bt.size(1) > 0 && ring.dim() == 1 && ring.size(0) > 0);
+  const int64_t B = bt.size(0), W = bt.size(1), N = ring.size(0);
+  need((W == 1 || bt.stride(1) == 1) && (B == 1 || bt.stride(0) >= W));
+  need(T >= 0 && bs >= 1 && bs <= (1 << 30) && W * bs <= (1 << 30) && T <= (1 << 30) && N <= (1 << 30) && B <= (1 << 24));
+  need(window >= 0 && sinks >= 0);
+  need(shape(cl, {B}) && shape(range, {2}) && shape(fresh, {B}) && (!keep || shape(*keep, {B})));
+  const Tensor* mine[] = {&bt, &cl, &ring, &range};
+  for (const Tensor* t : mine) {
+    need(t->scalar_type() == at::kInt && (t == &bt || t->is_contiguous()) && addr(*t) != addr(fresh) &&
+         (!keep || addr(*t) != addr(*keep)));
+    for (const Tensor* o : mine) need(o == t || addr(*o) != addr(*t));
+  }
+  need(fresh.scalar_type() == at::kInt && fresh.is_contiguous());
+  if (keep) need(keep->scalar_type() == at::kInt && keep->is_contiguous());
+  same_device(bt, {&cl, &ring, &range, &fresh});
+  if (keep) same_device(bt, {keep});
+  c10::DeviceGuard guard(bt.device());
+  size_t n = 0;
+  need(bytes_paged_resize_workspace_size((int)B, &n) == 0);
+  Tensor ws = empty(bt, {(int64_t)n}, at::kByte);
+  Tensor cu = empty(bt, {B + 1}, at::kInt), granted = empty(bt, {B}, at::kInt), seqs = empty(bt, {T}, at::kInt),
+         positions = empty(bt, {T}, at::kInt), slots = empty(bt, {T}, at::kLong);
+  void* st = stream_of(bt);
+  launch("bytes_paged_resize", bytes_paged_resize, bt.mutable_data_ptr(), bt.stride(0), cl.mutable_data_ptr(),
+         ring.mutable_data_ptr(), range.mutable_data_ptr(), keep ? data(*keep) : nullptr, data(fresh),
+         cu.mutable_data_ptr(), granted.mutable_data_ptr(), seqs.mutable_data_ptr(), positions.mutable_data_ptr(),
+         slots.mutable_data_ptr(), (int)B, (int)W, (int)N, (int)T, (int)bs, (int)window, (int)sinks, ws.mutable_data_ptr(),
+         n, st);
+  return Py_BuildValue("(NNNNN)", THPVariable_Wrap(cu), THPVariable_Wrap(granted), THPVariable_Wrap(seqs),
+                       THPVariable_Wrap(positions), THPVariable_Wrap(slots));
+}
+
 // ---- bindings ----
 
 template <class F>
@@ -708,6 +900,15 @@ BIND(paged_append, 15, paged_append(tensor(a[0]), tensor(a[1]), tensor(a[2]), te
                                     optional(a[11]), optional(a[12]), number(a[13]), number(a[14])))
 BIND(paged_decode, 8, WRAP(paged_decode(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), number(a[5]),
                                         number(a[6]), number(a[7]))))
+BIND(paged_window, 10, WRAP(paged_window(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]),
+                                         number(a[5]), a[6], a[7], a[8], a[9])))
+BIND(paged_prompt, 11, WRAP(paged_prompt(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]),
+                                         tensor(a[5]), number(a[6]), a[7], a[8], a[9], a[10])))
+BIND(paged_append_blocks, 13, paged_append_blocks(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]),
+                                                  tensor(a[5]), optional(a[6]), optional(a[7]), optional(a[8]),
+                                                  optional(a[9]), a[10] == Py_True, a[11], a[12]))
+BIND(paged_resize, 10, paged_resize(tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), optional(a[5]),
+                                    integer(a[6]), integer(a[7]), integer(a[8]), integer(a[9])))
 
 PyObject* py_set_workspaces(PyObject*, PyObject* d) {
   if (!PyDict_Check(d)) {
@@ -724,6 +925,7 @@ PyMethodDef methods[] = {METHOD(dense),     METHOD(kivi),   METHOD(kivi_pack), M
                          METHOD(pq_asym),   METHOD(pq_paged), METHOD(pq_encode), METHOD(score_into), METHOD(topk),
                          METHOD(gather),    METHOD(sparse_decode), METHOD(token_topk), METHOD(quest),
                          METHOD(paged_append), METHOD(paged_decode), METHOD(paged_quest),
+                         METHOD(paged_append_blocks), METHOD(paged_window), METHOD(paged_prompt), METHOD(paged_resize),
                          {"set_workspaces", py_set_workspaces, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native call path of the operators.", -1, methods};

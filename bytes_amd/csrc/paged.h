@@ -22,6 +22,10 @@ struct PagedKv {
   FastDiv dbs;                       // division by bs
 };
 
+// How a cache's rows are held: bf16, e4m3 with one scale for the tensor, e4m3 or int8 with
+// a scale for each block and KV head.
+enum PagedType : int { kBf16Cache = 0, kFp8Cache = 1, kE4m3Blocks = 2, kInt8Blocks = 3 };
+
 // Tokens of sequence b: negative lengths count as 0, lengths past the table row as its capacity.
 __device__ __forceinline__ int paged_len(const PagedKv& c, int b) {
   const int n = c.lens[b];
@@ -69,9 +73,9 @@ struct PagedIds {
   bool ok;
 };
 
-// fp8 rows of a tile into its bf16 LDS tile, as dense_stage_fp8 places them, two
-// values an instruction (exact: every e4m3 value is a bf16 value).  A batch of 32
-// sequences of up to 16K: 138 us with fp32 in between, 114 so.
+// Rows of bytes into the bf16 LDS tile, as dense_stage_fp8 places them; e4m3 two
+// values an instruction (exact: every e4m3 value is a bf16 value, as is every int8 one).
+// A batch of 32 sequences of up to 16K: 138 us with fp32 in between, 114 so.
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void fp8x16_to_bf16_direct(const u32x4& in, u32x4& lo, u32x4& hi) {
 #pragma unroll
@@ -82,15 +86,29 @@ __device__ __forceinline__ void fp8x16_to_bf16_direct(const u32x4& in, u32x4& lo
     hi[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[2 + j], 1.0f, true));
   }
 }
-template <int D>
-__device__ __forceinline__ void paged_stage_fp8(int lane, const DenseRegs8<D>& r, char* kst, char* vst) {
+__device__ __forceinline__ void int8x16_to_bf16(const u32x4& in, u32x4& lo, u32x4& hi) {
+  auto pair = [&](int j) {                         // values 2 j and 2 j + 1 (exact in fp32's upper half)
+    const uint32_t w = in[j >> 1] >> (16 * (j & 1));
+    const float a = (float)(int8_t)w, b = (float)(int8_t)(w >> 8);
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  };
+#pragma unroll
+  for (int j = 0; j < 4; ++j) lo[j] = pair(j), hi[j] = pair(4 + j);
+}
+template <bool INT8>
+__device__ __forceinline__ void bytes16_to_bf16(const u32x4& in, u32x4& lo, u32x4& hi) {
+  if constexpr (INT8) int8x16_to_bf16(in, lo, hi);
+  else fp8x16_to_bf16_direct(in, lo, hi);
+}
+template <int D, bool INT8>
+__device__ __forceinline__ void paged_stage_bytes(int lane, const DenseRegs8<D>& r, char* kst, char* vst) {
   using R = DenseRegs8<D>;
 #pragma unroll
   for (int i = 0; i < R::CPL8; ++i) {
     const int p = lane + 64 * i, rr = p / R::CPR8, pos = p - rr * R::CPR8;
     u32x4 k0, k1, v0, v1;
-    fp8x16_to_bf16_direct(r.k[i], k0, k1);
-    fp8x16_to_bf16_direct(r.v[i], v0, v1);
+    bytes16_to_bf16<INT8>(r.k[i], k0, k1);
+    bytes16_to_bf16<INT8>(r.v[i], v0, v1);
     *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * pos) * 16) = k0;
     *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * pos + 1) * 16) = k1;
     *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * pos) * 16) = v0;
@@ -103,8 +121,9 @@ __device__ __forceinline__ void paged_stage_fp8(int lane, const DenseRegs8<D>& r
 // from the lane that holds it.  A tile past the end (live false) reads the first
 // bytes of the cache, the same on every lane, so that every iteration issues the
 // same instructions.
-template <int D, bool FP8, bool HALVES>
+template <int D, int TYPE, bool HALVES>
 struct PagedRows {
+  static constexpr bool FP8 = TYPE != kBf16Cache;         // rows of bytes
   using Elem = typename std::conditional<FP8, uint8_t, uint16_t>::type;
   using Regs = typename std::conditional<FP8, DenseRegs8<D>, DenseRegs<D>>::type;
   static constexpr int EPC = 16 / (int)sizeof(Elem);      // elements per 16-byte chunk
@@ -158,7 +177,7 @@ struct PagedRows {
       for (int i = 0; i < CPL; ++i)
         if (!((vmask >> (r0 + i * RPI)) & 1u)) r.v[i] = u32x4{0, 0, 0, 0};
     }
-    if constexpr (FP8) paged_stage_fp8<D>(lane, r, kst, vst);
+    if constexpr (FP8) paged_stage_bytes<D, TYPE == kInt8Blocks>(lane, r, kst, vst);
     else dense_stage<D>(lane, r, kst, vst);
   }
 };
@@ -187,10 +206,12 @@ __device__ __forceinline__ uint32_t upper16(uint32_t lo, uint32_t hi) { return _
 // one underflows fp32, here or as the factor of a rescaled or joined part, 0 times the
 // infinity is NaN, as in any fp32 evaluation.  Caches of e4m3, which has no infinities,
 // need no such care.
-template <int D, bool INF>
+// Scales of blocks (sc: 32 of the slots' keys, 32 of their values, in LDS) multiply the
+// scores, and the weights before they are split; 0 for slots that are no token.
+template <int D, bool INF, bool SCALED = false>
 __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int lane, const bf16x8 (&qb)[D / 32],
                                            const char* kst, const char* vst, float& m_run, float& l_run,
-                                           f32x4 (&acc)[D / 16]) {
+                                           f32x4 (&acc)[D / 16], const float* sc = nullptr) {
   using C = DenseCfg<D>;
   const int l16 = lane & 15, lg = lane >> 4;
   f32x4 s[2];
@@ -203,6 +224,14 @@ __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int
       const bf16x8 ka = __builtin_bit_cast(
           bf16x8, *reinterpret_cast<const u32x4*>(kst + row * (D * 2) + kswz<D>(row, kk * 4 + lg) * 16));
       s[blk] = mfma_bf16(ka, qb[kk], s[blk]);
+    }
+  }
+  f32x4 vs[2];
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+      s[blk] *= *reinterpret_cast<const f32x4*>(sc + blk * 16 + lg * 4);
+      vs[blk] = *reinterpret_cast<const f32x4*>(sc + 32 + blk * 16 + lg * 4);
     }
   }
   float x[8], mx = kNegInf;
@@ -220,8 +249,9 @@ __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int
   uint32_t even[3];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float p = fast_exp2(x[j] - m_use);
+    float p = fast_exp2(x[j] - m_use);
     psum += p;
+    if constexpr (SCALED) p *= vs[j >> 2][j & 3];
     uint32_t u[3];
     u[0] = leading8<INF>(p);
     const float r1 = p - __uint_as_float(u[0]);    // (exact, as is the next)
@@ -259,17 +289,25 @@ __device__ __forceinline__ void paged_tile(uint32_t vmask, float scale_log2, int
   }
 }
 
+// A KV head's scales by block, and 64 floats of LDS of the wave's own.
+struct PagedScales {
+  const float *k, *v;
+  int64_t k_sb, v_sb;
+  float* lds;
+};
+
 // Slots [s, s_end) in steps of `step` (s a multiple of 32 from the first slot):
 // online softmax over them into m_run, l_run, acc.
-template <int D, bool FP8, bool HALVES, class FIND>
+template <int D, int TYPE, bool HALVES, class FIND>
 __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t* table, int hk, int s, int s_end,
                                                 int step, int lane, float scale_log2, const bf16x8 (&qb)[D / 32],
                                                 char* wbuf, const FIND& find, float& m_run, float& l_run,
-                                                f32x4 (&acc)[D / 16]) {
+                                                f32x4 (&acc)[D / 16], const PagedScales& sc = PagedScales{}) {
+  constexpr bool SCALED = TYPE >= kE4m3Blocks;
   if (s >= s_end) return;
   char* kst = wbuf;
   char* vst = wbuf + DenseCfg<D>::VT;
-  PagedRows<D, FP8, HALVES> rows(c, hk, lane);
+  PagedRows<D, TYPE, HALVES> rows(c, hk, lane);
   // entries of the tile at s0: loaded well before they are used
   auto fetch = [&](int s0) {
     PagedIds t;
@@ -286,19 +324,28 @@ __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t*
     t.ok = t.ok && in;
     t.id = in ? t.id : 0;
   };
+  // lanes 0 to 31 their slot's key scale, the others its value scale
+  auto scale = [&](const PagedIds& t) {
+    if constexpr (!SCALED) return 0.f;
+    const float x = *(lane < 32 ? sc.k + t.id * sc.k_sb : sc.v + t.id * sc.v_sb);
+    return t.ok ? x : 0.f;
+  };
   PagedIds now = fetch(s), next = fetch(s + step);
   settle(now);
+  float scaled = scale(now);
   rows.issue(now, true);
   for (; s < s_end; s += step) {
     const uint32_t vmask = (uint32_t)__ballot(now.ok);
     wave_lds_sync();
     rows.stage(vmask, kst, vst);
+    if constexpr (SCALED) sc.lds[lane] = scaled;
     settle(next);
     now = next;
     next = fetch(s + 2 * step);
+    scaled = scale(now);
     rows.issue(now, s + step < s_end);
     wave_lds_sync();
-    paged_tile<D, !FP8>(vmask, scale_log2, lane, qb, kst, vst, m_run, l_run, acc);
+    paged_tile<D, TYPE == kBf16Cache, SCALED>(vmask, scale_log2, lane, qb, kst, vst, m_run, l_run, acc, sc.lds);
   }
 }
 

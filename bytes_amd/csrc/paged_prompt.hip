@@ -1,0 +1,566 @@
+// Causal attention of several new tokens per sequence over a paged cache, whole or
+// within a sliding window and the first tokens (sinks).
+//
+//   out[i, h] = sum_t p_t vs_t v_t / sum_t p_t,  p_t = exp(scale * ks_t * (q . k_t) - max)
+//
+// for the query at position p = n - m + i of a sequence of n tokens, m of them new, over
+// the tokens t <= p whose block exists and, with a window w and s sinks, t > p - w or
+// t < s.  ks_t, vs_t: the scales of token t's block (or one for the tensor).
+//
+// Rows: the G query heads of a KV head read the same keys, so a workgroup's rows are
+// (token, head of the group) pairs, token major: 32 to a wave.  Keys come in tiles of 64,
+// staged through LDS for the workgroup.
+//   S^T[t][row] = K[t][:] . Q[row][:]   32x32x16 MFMA; A = K rows from LDS, B = Q in registers
+//   softmax per row: a lane has half of a row's keys, its partner lane + 32 the others
+//   O^T[d][row] += V^T[d][t] P^T[t][row]  A = V read transposed (ds_read_b64_tr_b16)
+// The output registers of S^T hold, for lane half e, the keys 8 g + 4 e .. + 3: the second
+// product takes its keys in that order, so P goes from one to the other without leaving
+// the lane.  P is rounded to bf16 (nearest even, 2^-8 of a weight at most, as much as the
+// result's own rounding: error against 64 bits 0.0023 of the norm, 0.0017 of it the
+// result's rounding; a second bf16 part would make three products of two); its sum stays in fp32.
+// The running maximum moves only where a score passes it by 2^8, so most tiles leave the
+// accumulators as they are; weights are then up to 2^8, which changes no relative error.
+#include "paged.h"
+
+namespace bytes_amd {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kPromptWaves = 4;
+constexpr int kPromptRows = kPromptWaves * 32;
+constexpr int kKeys = 64;            // of a tile
+constexpr float kSlack = 8.f;        // log2 of how far weights may pass 1
+
+struct PromptArgs {
+  PagedKv c;
+  const uint16_t* q;
+  int64_t q_st, q_sh;
+  uint16_t* out;
+  int64_t o_st, o_sh;
+  const int32_t* cu;                 // [B + 1]
+  const float *ks, *vs;              // [num_blocks, Hk], or null
+  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
+  float* part_acc;                   // [unit][split][row][D]
+  float* part_ml;                    // [unit][split][row][2]
+  int T, B, Hk, G, D;
+  int cap, window, sinks;            // no window: 2^30
+  int nsplit, tiles;                 // parts of a unit's keys; row tiles at most
+  int flip, pad;                     // the scale is negative: queries change sign
+  float scale_log2, v_scale;
+  FastDiv dHk, dG, dsplit;
+};
+
+// Row tile number r of the batch: rows r0 .. of sequence b, whose new tokens are rows
+// t0 .. t0 + n - 1 of q (b = B: the rows past the last sequence).  False past the last.
+struct RowTile {
+  int b, t0, n, r0;
+};
+template <int ROWS>
+__device__ __forceinline__ bool find_tile(const PromptArgs& a, int r, int lane, RowTile& x) {
+  for (int b0 = 0; b0 <= a.B; b0 += 64) {
+    const int b = b0 + lane, bc = min(b, a.B);
+    const int c0 = min(max(a.cu[bc], 0), a.T), c1 = b < a.B ? min(max(a.cu[bc + 1], 0), a.T) : a.T;
+    const int n = b <= a.B ? max(c1 - c0, 0) : 0;
+    const uint32_t mine = (uint32_t)((n * a.G + ROWS - 1) / ROWS);
+    const uint32_t incl = wave_prefix_sum(mine);
+    const int total = __builtin_amdgcn_readlane((int)incl, 63);
+    if (r < total) {
+      const int l = __ffsll((unsigned long long)__ballot((int)incl > r)) - 1;
+      x.b = b0 + l;
+      x.t0 = __builtin_amdgcn_readlane(c0, l);
+      x.n = __builtin_amdgcn_readlane(n, l);
+      x.r0 = (r - __builtin_amdgcn_readlane((int)(incl - mine), l)) * ROWS;
+      return true;
+    }
+    r -= total;
+  }
+  return false;
+}
+
+// The first n of 64 bits.
+__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+// The largest exponent fields of bf16 pairs so far and of eight more; an infinity or NaN has all ones there.
+__device__ __forceinline__ u16x2 exponents(u16x2 m, const u32x4& x) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[j] & 0x7F807F80u));
+  return m;
+}
+
+__device__ __forceinline__ float half_max(float v) {   // of a lane and its partner lane ^ 32
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Four consecutive results; zeros where nothing was seen.
+__device__ __forceinline__ void store_bf16x4(uint16_t* out, const f32x16& x, int at, float by) {
+  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+  bf16x4 r;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) r[u] = (__bf16)(by == 0.f ? 0.f : x[at + u] * by);
+  *reinterpret_cast<u32x2*>(out) = __builtin_bit_cast(u32x2, r);
+}
+
+template <int D, int TYPE, bool HALVES>
+__global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 1 : 2) void paged_prompt_kernel(PromptArgs a) {
+  constexpr bool BYTES = TYPE != kBf16Cache, SCALED = TYPE >= kE4m3Blocks;
+  using Elem = typename std::conditional<BYTES, uint8_t, uint16_t>::type;
+  constexpr int EPC = 16 / (int)sizeof(Elem), CPR = D / EPC;         // elements per chunk, chunks per row
+  constexpr int RPW = 64 / CPR, RPI = kPromptWaves * RPW, NI = kKeys / RPI;
+  static_assert(RPW <= 16 && NI >= 1, "a wave's rows of one instruction lie in 16 of a block");
+  constexpr int KK = D / 16, DB = D / 32, VT = kKeys * D * 2;
+  __shared__ __attribute__((aligned(16))) char smem[2][2 * VT];      // [buffer][K, V]
+  // scales of a tile's tokens: in scalar registers where 16 of them share a block, else in LDS
+  constexpr bool SCALES_LDS = SCALED && !HALVES;
+  __shared__ float sc[2][SCALES_LDS ? 128 : 1];
+  __shared__ int bad[2];
+
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l32 = lane & 31, e = lane >> 5;
+  const int per = a.Hk * a.nsplit;
+  const int tile = a.tiles - 1 - (int)blockIdx.x / per;              // the last rows, which see most, first
+  const int rest = (int)blockIdx.x % per, split = fast_div(rest, a.dHk), hk = rest - split * a.Hk;
+  RowTile x;
+  if (!find_tile<kPromptRows>(a, tile, lane, x)) return;
+  const int row = x.r0 + w * 32 + l32, rows = x.n * a.G;
+  const bool exists = row < rows;
+  const int i = fast_div(exists ? row : 0, a.dG), h = hk * a.G + (exists ? row : 0) - i * a.G;
+  uint16_t* out = a.out + (int64_t)(x.t0 + i) * a.o_st + (int64_t)h * a.o_sh;
+  if (x.b == a.B) {                                // rows of no sequence
+    if (exists && split == 0) {
+      for (int d = e * (D / 2); d < (e + 1) * (D / 2); d += 8) *reinterpret_cast<u32x4*>(out + d) = u32x4{0, 0, 0, 0};
+    }
+    return;
+  }
+  const int p0 = a.c.lens[x.b] - x.n;              // the first new token's position
+  const int p = p0 + i;
+  const bool placed = exists && p >= 0 && p < a.cap;
+  const int first = fast_div(x.r0, a.dG), last = min(fast_div(x.r0 + kPromptRows - 1, a.dG), x.n - 1);
+  const int p_lo = max(p0 + first, 0), p_hi = min(p0 + last, a.cap - 1);
+  // this wave's positions
+  const int wl = fast_div(min(x.r0 + w * 32, rows - 1), a.dG), wh = fast_div(min(x.r0 + w * 32 + 31, rows - 1), a.dG);
+  const bool wave_any = x.r0 + w * 32 < rows;
+  const int w_lo = max(p0 + wl, 0), w_hi = wave_any ? min(p0 + wh, a.cap - 1) : -1;
+  // keys: tiles of the sinks, then from the window's first one on
+  const int end = max(p_hi + 1, 0), lo_key = max(p_lo - a.window + 1, 0);
+  const int near_tiles = (min(a.sinks, end) + kKeys - 1) / kKeys * kKeys;
+  const int gap = max(lo_key / kKeys * kKeys - near_tiles, 0);
+  const int ntiles = p_lo > p_hi ? 0 : (end - gap + kKeys - 1) / kKeys;
+  const int j0 = (int)((int64_t)ntiles * split / a.nsplit), j1 = (int)((int64_t)ntiles * (split + 1) / a.nsplit);
+
+  bf16x8 qb[KK];
+  {
+    const uint16_t* qp = a.q + (int64_t)(x.t0 + i) * a.q_st + (int64_t)h * a.q_sh + e * 8;
+    const uint32_t sign = a.flip ? 0x80008000u : 0u;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      u32x4 raw = ld16_live(qp + kk * 16, placed);
+      raw ^= u32x4{sign, sign, sign, sign};
+      qb[kk] = __builtin_bit_cast(bf16x8, raw);
+    }
+  }
+  float m_run = kNegInf, l_run = 0.f;
+  f32x16 acc[DB];
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int u = 0; u < 16; ++u) acc[db][u] = 0.f;
+
+  const int32_t* table = a.c.table + (int64_t)x.b * a.c.bt_sb;
+  const Elem* kb = static_cast<const Elem*>(a.c.k) + hk * a.c.k_sh;
+  const Elem* vb = static_cast<const Elem*>(a.c.v) + hk * a.c.v_sh;
+  const int r_in = lane / CPR, col = lane % CPR;
+  auto start = [&](int j) { return j * kKeys < near_tiles ? j * kKeys : j * kKeys + gap; };
+  // tile j's table entries: lane l's token is start(j) + l
+  auto fetch = [&](int j) {
+    PagedIds t;
+    const int s = start(j) + lane, sc_ = min(s, end - 1);
+    const int place = fast_div(max(sc_, 0), a.c.dbs);
+    t.ok = j < j1 && s < end;
+    t.off = t.ok ? s - place * a.c.bs : 0;
+    t.id = table[place];
+    return t;
+  };
+  auto settle = [&](PagedIds& t) {
+    const bool in = t.id >= 0 && t.id < a.c.nblocks;
+    t.ok = t.ok && in;
+    t.id = in ? t.id : 0;
+  };
+  u32x4 kr[NI], vr[NI];
+  auto issue = [&](const PagedIds& t) {
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int base = u * RPI + w * RPW;          // this wave's rows of the instruction
+      int id, off;
+      if constexpr (HALVES) {
+        const int g = base & ~15;
+        id = __builtin_amdgcn_readlane(t.id, g);
+        off = __builtin_amdgcn_readlane(t.off, g) + (base - g) + r_in;
+      } else {
+        id = __shfl(t.id, base + r_in, 64);
+        off = __shfl(t.off, base + r_in, 64);
+      }
+      kr[u] = ld16(kb + (int64_t)id * a.c.k_sb + (int64_t)off * a.c.k_ss + col * EPC);
+      vr[u] = ld16(vb + (int64_t)id * a.c.v_sb + (int64_t)off * a.c.v_ss + col * EPC);
+      if constexpr (!HALVES) asm volatile("" ::: "memory");          // (one row's addresses in registers at a time)
+    }
+  };
+  float kscale = 0.f, vscale = 0.f, kg[4], vg[4];
+  auto scales = [&](const PagedIds& t) {
+    if constexpr (SCALED) {
+      const float x = a.ks[t.id * a.ks_sb + hk * a.ks_sh], y = a.vs[t.id * a.vs_sb + hk * a.vs_sh];
+      kscale = t.ok ? x : 0.f;
+      vscale = t.ok ? y : 0.f;
+    }
+  };
+  // Into buffer `to`; values of slots that are no token become 0.  Returns whether values
+  // of this lane's are infinite or NaN.
+  auto stage = [&](int to, uint64_t named) {
+    char *kst = smem[to], *vst = kst + VT;
+    u16x2 ex = {0, 0};
+#pragma unroll
+    for (int u = 0; u < NI; ++u) {
+      const int rr = u * RPI + w * RPW + r_in;
+      const uint32_t keep = (named >> rr) & 1 ? ~0u : 0u;
+      vr[u] &= u32x4{keep, keep, keep, keep};
+      if constexpr (BYTES) {
+        u32x4 k0, k1, v0, v1;
+        bytes16_to_bf16<TYPE == kInt8Blocks>(kr[u], k0, k1);
+        bytes16_to_bf16<TYPE == kInt8Blocks>(vr[u], v0, v1);
+        if (TYPE != kInt8Blocks) ex = exponents(exponents(ex, v0), v1);
+        *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * col) * 16) = k0;
+        *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * col + 1) * 16) = k1;
+        *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * col) * 16) = v0;
+        *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * col + 1) * 16) = v1;
+        asm volatile("" ::: "memory");
+      } else {
+        ex = exponents(ex, vr[u]);
+        *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, col) * 16) = kr[u];
+        *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, col) * 16) = vr[u];
+      }
+    }
+    if constexpr (SCALES_LDS) {
+      if (w == 0) sc[to][lane] = kscale, sc[to][64 + lane] = vscale;
+    }
+    if constexpr (SCALED && HALVES) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        kg[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kscale), 16 * g));
+        vg[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vscale), 16 * g));
+      }
+    }
+    return ex[0] == 0x7F80 || ex[1] == 0x7F80;
+  };
+
+  // One staged tile.
+  auto compute = [&](int from, int t0, uint64_t named, bool infinite) {
+    const char *kst = smem[from], *vst = kst + VT;
+    // keys that all of the wave's rows see
+    const bool whole = named == ~0ull && t0 + kKeys - 1 <= w_lo && (t0 > w_hi - a.window || t0 + kKeys <= a.sinks);
+    f32x16 s[2];
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk) {
+#pragma unroll
+      for (int u = 0; u < 16; ++u) s[blk][u] = 0.f;
+      const int rr = blk * 32 + l32;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const bf16x8 ka = __builtin_bit_cast(
+            bf16x8, *reinterpret_cast<const u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, kk * 2 + e) * 16));
+        s[blk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[kk], s[blk], 0, 0, 0);
+      }
+    }
+    if constexpr (SCALED) {
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          s[blk][u] *= SCALES_LDS ? sc[from][blk * 32 + (u >> 2) * 8 + e * 4 + (u & 3)] : kg[2 * blk + (u >> 3)];
+    }
+    uint64_t see = ~0ull;
+    if (!whole) {
+      see = placed ? named & low_bits(p - t0 + 1) & (~low_bits(p - a.window + 1 - t0) | low_bits(a.sinks - t0)) : 0ull;
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        const uint32_t m = (uint32_t)(see >> (32 * blk)) >> (4 * e);
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          if (!((m >> (8 * (u >> 2) + (u & 3))) & 1u)) s[blk][u] = kNegInf;
+      }
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+      for (int u = 0; u < 16; ++u) mx = __builtin_elementwise_maximum(mx, s[blk][u]);
+    mx = half_max(mx);
+    if (__any((mx - m_run) * a.scale_log2 > kSlack)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float alpha = m_new == kNegInf ? 0.f : fast_exp2((m_run - m_new) * a.scale_log2);
+      m_run = m_new;
+      l_run *= alpha;
+#pragma unroll
+      for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int u = 0; u < 16; ++u) acc[db][u] *= alpha;
+    }
+    const float mc = m_run == kNegInf ? 0.f : m_run * a.scale_log2;
+    auto weight = [&](float x) { return fast_exp2(__builtin_fmaf(x, a.scale_log2, -mc)); };
+    if (TYPE != kInt8Blocks && !whole && infinite) {
+      // A weight of 0 times an infinite value is not 0: one key at a time, rows that do not
+      // see it leaving their sums as they are.
+#pragma unroll 1
+      for (int k = 0; k < kKeys; ++k) {
+        const int in = k & 31, u_of = (in >> 3) * 4 + (in & 3), half = (in >> 2) & 1;
+        float mine = 0.f;
+#pragma unroll
+        for (int u = 0; u < 16; ++u) mine = u == u_of ? (k < 32 ? s[0][u] : s[1][u]) : mine;
+        float pk = weight(__shfl(mine, l32 + 32 * half, 64));
+        l_run += e == half ? pk : 0.f;
+        if constexpr (SCALES_LDS) pk *= sc[from][64 + k];
+        else if constexpr (SCALED) pk *= k < 32 ? (k < 16 ? vg[0] : vg[1]) : (k < 48 ? vg[2] : vg[3]);
+        const bool sees = (see >> k) & 1;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int d = db * 32 + 8 * g + 4 * e;
+            const u32x2 v = *reinterpret_cast<const u32x2*>(vst + k * (D * 2) + vswz<D>(k, d >> 3) * 16 + (d & 7) * 2);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const float vv = __uint_as_float(u & 1 ? v[u >> 1] & 0xFFFF0000u : v[u >> 1] << 16);
+              acc[db][4 * g + u] = sees ? __builtin_fmaf(pk, vv, acc[db][4 * g + u]) : acc[db][4 * g + u];
+            }
+            asm volatile("" ::: "memory");         // (few registers for a path that is hardly taken)
+          }
+      }
+      return;
+    }
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      bf16x8 pb;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        float pk = weight(s[kk >> 1][(kk & 1) * 8 + u]);
+        l_run += pk;
+        if constexpr (SCALES_LDS) pk *= sc[from][64 + kk * 16 + (u >> 2) * 8 + e * 4 + (u & 3)];
+        else if constexpr (SCALED) pk *= vg[kk];
+        pb[u] = (__bf16)pk;
+      }
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        u32x2 t[2];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int rr = kk * 16 + hf * 8 + e * 4 + ((lane >> 2) & 3), d = db * 32 + (lane & 16) + (lane & 3) * 4;
+          t[hf] = tr16(vst + rr * (D * 2) + vswz<D>(rr, d >> 3) * 16 + (d & 7) * 2);
+        }
+        acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, u32x4{t[0][0], t[0][1], t[1][0], t[1][1]}), pb, acc[db], 0, 0, 0);
+      }
+    }
+  };
+
+  if (j0 < j1) {
+    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
+    PagedIds now = fetch(j0), next = fetch(j0 + 1);
+    settle(now);
+    scales(now);
+    issue(now);
+    __syncthreads();
+    for (int j = j0; j < j1; ++j) {
+      const int buf = j & 1, t0 = start(j);
+      const uint64_t named = __ballot(now.ok);
+      // (buffer `buf` was last read two tiles ago, before the barrier of the last one)
+      const bool odd = stage(buf, named);
+      if (__any(odd) && lane == 0) bad[buf] = j + 1;
+      settle(next);
+      now = next;
+      next = fetch(j + 2);
+      scales(now);
+      if (j + 1 < j1) issue(now);
+      __syncthreads();
+      if (t0 <= w_hi) compute(buf, t0, named, bad[buf] == j + 1);
+    }
+  }
+
+  l_run = half_sum(l_run);
+  if (!placed) l_run = 0.f;                        // a row without a position gets zeros
+  if (a.nsplit > 1) {
+    const size_t slot = (((size_t)tile * a.Hk + hk) * a.nsplit + split) * kPromptRows + w * 32 + l32;
+    if (!exists) return;
+    float* pa = a.part_acc + slot * D;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(pa + db * 32 + 8 * g + 4 * e) =
+            f32x4{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+    if (e == 0)
+      reinterpret_cast<float2*>(a.part_ml)[slot] = make_float2(m_run == kNegInf ? kNegInf : m_run * a.scale_log2, l_run);
+    return;
+  }
+  if (!exists) return;
+  const float by = l_run == 0.f ? 0.f : a.v_scale / l_run;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) store_bf16x4(out + db * 32 + 8 * g + 4 * e, acc[db], 4 * g, by);
+}
+
+// Joins the parts of a row's keys: one wave per (row of q, query head, 64 dims).
+template <int D>
+__global__ __launch_bounds__(64) void paged_prompt_join_kernel(PromptArgs a) {
+  constexpr int NSL = D / 64;
+  const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
+  const int slice = blockIdx.y % NSL, h = blockIdx.y / NSL, t = blockIdx.x;
+  // the sequence of row t and its first row tile
+  int tiles = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane, bc = min(b, a.B - 1);
+    const int c0 = min(max(a.cu[bc], 0), a.T), c1 = min(max(a.cu[bc + 1], 0), a.T);
+    const int n = b < a.B ? max(c1 - c0, 0) : 0;
+    const uint32_t mine = (uint32_t)((n * a.G + kPromptRows - 1) / kPromptRows);
+    const uint32_t incl = wave_prefix_sum(mine);
+    const unsigned long long in = __ballot(n > 0 && t >= c0 && t < c0 + n);
+    if (in) {
+      const int l = __ffsll(in) - 1;
+      const int i = t - __builtin_amdgcn_readlane(c0, l), hk = fast_div(h, a.dG);
+      const int row = i * a.G + h - hk * a.G, tile = tiles + __builtin_amdgcn_readlane((int)(incl - mine), l) + row / kPromptRows;
+      const size_t base = ((size_t)tile * a.Hk + hk) * a.nsplit * kPromptRows + row % kPromptRows;
+      auto slot = [&](int u) { return base + (size_t)u * kPromptRows; };
+      paged_join<4>(a.nsplit, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
+                    reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4,
+                    [&](const f32x4& A, float L) {
+                      if (grp == 0)
+                        paged_store(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
+                    });
+      return;
+    }
+    tiles += __builtin_amdgcn_readlane((int)incl, 63);
+  }
+}
+
+// Row tiles of a batch, at most: whole ones, and one that is not full per sequence (and
+// of the rows past the last); none without rows.
+static int64_t prompt_tiles(int64_t T, int64_t B, int64_t G) {
+  const int64_t n = T * G / kPromptRows + B + 1, most = T;
+  return n < most ? n : most;
+}
+// Parts that a unit's keys are cut into: enough that two workgroups come to each CU, none
+// of fewer than 8 key tiles of a full table row.
+static int prompt_split(int64_t units, int64_t cap) {
+  const int64_t cus = device_cu_count(), want = (2 * cus + units - 1) / units, most = cap / (8 * kKeys);
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+static int64_t prompt_slots(int64_t cap, int window, int sinks) {
+  const int64_t most = (int64_t)window + sinks + kPromptRows + 2 * kKeys;
+  return cap < most ? cap : most;
+}
+static size_t prompt_workspace(int64_t units, int nsplit, int D) {
+  return nsplit < 2 ? 0 : (size_t)units * nsplit * kPromptRows * (D + 2) * 4;
+}
+
+template <int TYPE>
+static int launch_prompt(const PromptArgs& a, dim3 grid, hipStream_t st) {
+  const bool halves = paged_halves(a.c);
+  const dim3 block(kPromptWaves * 64);
+#define PP(DD, H) hipLaunchKernelGGL((paged_prompt_kernel<DD, TYPE, H>), grid, block, 0, st, a)
+  if (a.D == 128) {
+    if (halves) PP(128, true);
+    else PP(128, false);
+  } else {
+    if (halves) PP(64, true);
+    else PP(64, false);
+  }
+#undef PP
+  return (int)hipGetLastError();
+}
+
+}  // namespace bytes_amd
+
+using namespace bytes_amd;
+
+extern "C" {
+
+int bytes_paged_prompt_workspace_size(int T, int B, int Hq, int Hk, int D, int block_size, int max_blocks, int window,
+                                      int sinks, size_t* bytes) {
+  if (!bytes || T < 0 || B <= 0 || Hk <= 0 || Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128) || window <= 0 || sinks < 0)
+    return (int)hipErrorInvalidValue;
+  const int rc = paged_check(block_size, 1, max_blocks);
+  if (rc) return rc;
+  if (T == 0) {
+    *bytes = 0;
+    return 0;
+  }
+  const int64_t units = prompt_tiles(T, B, Hq / Hk) * Hk;
+  const int64_t slots = prompt_slots((int64_t)max_blocks * block_size, window, sinks);
+  *bytes = prompt_workspace(units, prompt_split(units, slots), D);
+  return 0;
+}
+
+int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
+                            int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_type,
+                            const void* k_scales, int64_t ks_sb, int64_t ks_sh, const void* v_scales, int64_t vs_sb,
+                            int64_t vs_sh, const void* block_table, int64_t bt_sb, const void* context_lens,
+                            const void* cu_seqlens, void* out, int64_t o_st, int64_t o_sh, int T, int B, int Hq, int Hk,
+                            int D, int block_size, int num_blocks, int max_blocks, int window, int sinks, float scale,
+                            float v_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k_paged || !v_paged || !block_table || !context_lens || !cu_seqlens || !out || T < 0 || B <= 0 || Hk <= 0 ||
+      Hq <= 0 || Hq % Hk != 0 || (D != 64 && D != 128) || max_blocks <= 0 || window <= 0 || sinks < 0 ||
+      kv_type < kBf16Cache || kv_type > kInt8Blocks || (kv_type >= kE4m3Blocks && (!k_scales || !v_scales)))
+    return (int)hipErrorInvalidValue;
+  const int rc0 = paged_check(block_size, num_blocks, max_blocks);
+  if (rc0) return rc0;
+  if (T == 0) return 0;
+  const int64_t G = Hq / Hk, tiles = prompt_tiles(T, B, G), units = tiles * Hk;
+  PromptArgs a = {};
+  a.window = window < (1 << 30) ? window : (1 << 30), a.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
+  a.nsplit = prompt_split(units, prompt_slots((int64_t)max_blocks * block_size, window, sinks));
+  if ((int64_t)T * G + kPromptRows > 0x7FFFFFFF || units * a.nsplit > 0x7FFFFFFF || T > (1 << 30) ||
+      (int64_t)Hq * (D / 64) > 65535)
+    return (int)hipErrorInvalidConfiguration;
+  if (a.nsplit > 1 && (!workspace || workspace_bytes < prompt_workspace(units, a.nsplit, D))) return (int)hipErrorInvalidValue;
+  a.c.k = k_paged, a.c.k_sb = k_sb, a.c.k_sh = k_sh, a.c.k_ss = k_ss;
+  a.c.v = v_paged, a.c.v_sb = v_sb, a.c.v_sh = v_sh, a.c.v_ss = v_ss;
+  a.c.table = static_cast<const int32_t*>(block_table), a.c.bt_sb = bt_sb;
+  a.c.lens = static_cast<const int32_t*>(context_lens);
+  a.c.bs = block_size, a.c.nblocks = num_blocks, a.c.width = max_blocks;
+  a.c.dbs = make_fastdiv((uint32_t)block_size);
+  a.q = static_cast<const uint16_t*>(q), a.q_st = q_st, a.q_sh = q_sh;
+  a.out = static_cast<uint16_t*>(out), a.o_st = o_st, a.o_sh = o_sh;
+  a.cu = static_cast<const int32_t*>(cu_seqlens);
+  a.ks = static_cast<const float*>(k_scales), a.ks_sb = ks_sb, a.ks_sh = ks_sh;
+  a.vs = static_cast<const float*>(v_scales), a.vs_sb = vs_sb, a.vs_sh = vs_sh;
+  a.part_ml = static_cast<float*>(workspace);
+  a.part_acc = a.part_ml + (size_t)units * a.nsplit * kPromptRows * 2;
+  a.T = T, a.B = B, a.Hk = Hk, a.G = (int)G, a.D = D;
+  a.cap = max_blocks * block_size;
+  a.tiles = (int)tiles;
+  a.flip = scale < 0.f ? 1 : 0;
+  // (at least the smallest normal number: times -inf, a masked score, it is -inf)
+  a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f), a.v_scale = v_scale;
+  a.dHk = make_fastdiv((uint32_t)Hk), a.dG = make_fastdiv((uint32_t)G), a.dsplit = make_fastdiv((uint32_t)a.nsplit);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(units * a.nsplit));
+  int rc = 0;
+  switch (kv_type) {
+    case kBf16Cache: rc = launch_prompt<kBf16Cache>(a, grid, st); break;
+    case kFp8Cache: rc = launch_prompt<kFp8Cache>(a, grid, st); break;
+    case kE4m3Blocks: rc = launch_prompt<kE4m3Blocks>(a, grid, st); break;
+    default: rc = launch_prompt<kInt8Blocks>(a, grid, st);
+  }
+  if (rc || a.nsplit < 2) return rc;
+  const dim3 jgrid((unsigned)T, (unsigned)(Hq * (D / 64)));
+  if (D == 128) hipLaunchKernelGGL(paged_prompt_join_kernel<128>, jgrid, dim3(64), 0, st, a);
+  else hipLaunchKernelGGL(paged_prompt_join_kernel<64>, jgrid, dim3(64), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+}  // extern "C"

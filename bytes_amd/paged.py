@@ -1,9 +1,12 @@
-"""Paged dense KV caches: append with rotation, decode, page-sparse decode.
+"""Paged dense KV caches: append with rotation, decode, page-sparse decode, prompts.
 
 A cache is a pair k_paged, v_paged [num_blocks, H_k, block_size, D] of bf16, or
 of float8_e4m3fn whose values stand for value * k_scale (v_scale): the layout of
 the paged product-quantized operators (src/attention_kernels.py:588-622,
-:858-906), with dense rows.  Any strides are taken as long as rows have unit
+:858-906), with dense rows.  Where k_scale and v_scale are tensors [num_blocks, H_k]
+fp32 (finite, not negative), the cache is float8_e4m3fn or int8 with a scale for each
+block and KV head: the append writes them, the attention operators read them (the
+page-sparse decode takes no such caches).  Any strides are taken as long as rows have unit
 stride along D and start on 16-byte boundaries (a [.., block_size, H_k, D]
 storage as well); caches are never copied, other layouts are refused.  Token p of
 sequence b is row p % block_size of block block_table[b, p // block_size].
@@ -23,7 +26,7 @@ Results carry no autograd graph.  H_q must be a multiple of H_k and D 64 or 128.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 
@@ -33,6 +36,8 @@ from .sparse import _topk
 
 _F8 = torch.float8_e4m3fn
 Meta = Tuple[torch.Tensor, torch.Tensor]
+Scale = Union[float, torch.Tensor]
+_NO_WINDOW = 2 ** 30
 
 
 def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
@@ -44,10 +49,60 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _cache(k_paged: torch.Tensor, v_paged: torch.Tensor, k_scale: float, v_scale: float):
+def _by_block(k_scale: Scale, v_scale: Scale) -> bool:
+    """Whether the scales are tensors, one for each block and KV head (one of one element
+    without two dims is a number)."""
+    a, b = (isinstance(s, torch.Tensor) and (s.dim() == 2 or s.numel() > 1) for s in (k_scale, v_scale))
+    if a != b:
+        raise ValueError("k_scale and v_scale are both numbers or both tensors [num_blocks, H_k]")
+    return a
+
+
+def _tensors(k_scale: Scale, v_scale: Scale) -> list:
+    return [k_scale, v_scale] if _by_block(k_scale, v_scale) else []
+
+
+def _block_scales(k_scale: torch.Tensor, v_scale: torch.Tensor, N: int, Hk: int) -> None:
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        C.dtype_in(t, n, torch.float32)
+        if tuple(t.shape) != (N, Hk):
+            raise ValueError(f"{n} must be [num_blocks, H_k] = {(N, Hk)}; got {tuple(t.shape)}")
+
+
+def _window(window: Optional[int], sinks: int) -> Tuple[int, int]:
+    """-> (window, sinks) as the C ABI takes them."""
+    if window is None:
+        if int(sinks) != 0:
+            raise ValueError(f"sinks={sinks}: without a window every token is seen")
+        return _NO_WINDOW, 0
+    if int(window) < 1 or int(sinks) < 0:
+        raise ValueError(f"window={window}, sinks={sinks}: a window has at least one token, sinks are none or more")
+    return min(int(window), _NO_WINDOW), min(int(sinks), _NO_WINDOW)
+
+
+def _typed_cache(k_paged, v_paged, k_scale: Scale, v_scale: Scale):
+    """-> (num_blocks, H_k, block_size, D, cache type of the C ABI), for caches of every kind."""
+    if not _by_block(k_scale, v_scale):
+        N, Hk, bs, D, fp8 = _cache(k_paged, v_paged, k_scale, v_scale)
+        return N, Hk, bs, D, int(fp8)
+    N, Hk, bs, D, _ = _cache(k_paged, v_paged, 1.0, 1.0, (_F8, torch.int8))
+    _block_scales(k_scale, v_scale, N, Hk)
+    return N, Hk, bs, D, 2 if k_paged.dtype == _F8 else 3
+
+
+def _scale_args(k_scale: Scale, v_scale: Scale, typ: int, scale: float):
+    """-> the C ABI's (scales and strides), (scale, v_scale)."""
+    if typ < 2:
+        return (None, 0, 0, None, 0, 0), (float(scale) * float(k_scale), float(v_scale))
+    return ((ptr(k_scale), k_scale.stride(0), k_scale.stride(1), ptr(v_scale), v_scale.stride(0), v_scale.stride(1)),
+            (float(scale), 1.0))
+
+
+def _cache(k_paged: torch.Tensor, v_paged: torch.Tensor, k_scale: float, v_scale: float,
+           dtypes: Tuple[torch.dtype, ...] = (torch.bfloat16, _F8)):
     """-> (num_blocks, H_k, block_size, D, the cache is fp8)."""
     C.ndim(k_paged, 4, "k_paged"), C.ndim(v_paged, 4, "v_paged")
-    C.dtype_in(k_paged, "k_paged", torch.bfloat16, _F8)
+    C.dtype_in(k_paged, "k_paged", *dtypes)
     C.dtype_in(v_paged, "v_paged", k_paged.dtype)
     if tuple(v_paged.shape) != tuple(k_paged.shape):
         raise ValueError(f"shape mismatch: k_paged {tuple(k_paged.shape)}, v_paged {tuple(v_paged.shape)}")
@@ -120,8 +175,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
                     block_table: torch.Tensor, context_lens: torch.Tensor, *,
                     cu_seqlens: Optional[torch.Tensor] = None, q: Optional[torch.Tensor] = None,
                     cos: Optional[torch.Tensor] = None, sin: Optional[torch.Tensor] = None, interleaved: bool = False,
-                    meta: Optional[Meta] = None, k_scale: float = 1.0,
-                    v_scale: float = 1.0) -> Optional[torch.Tensor]:
+                    meta: Optional[Meta] = None, k_scale: Scale = 1.0,
+                    v_scale: Scale = 1.0) -> Optional[torch.Tensor]:
     """Write new tokens' keys and values into the cache, keys rotated by their
     position, in place.
 
@@ -147,6 +202,16 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
     (For a cache filled otherwise, quest_page_minmax(k_paged, block_size) gives
     them where all blocks are full.)
 
+    k_scale, v_scale [num_blocks, H_k] fp32 tensors (memory of their own, any strides):
+    float8_e4m3fn or int8 caches with a scale for each block and KV head, written here
+    (meta is not taken).  For every block that receives tokens, with a the largest |x|
+    of its new rows (infinities as the largest bf16 number) and c = a / 127 (int8) or
+    the smallest power of two of at least a / 448 (e4m3): the scale becomes c where a
+    sequence enters the block at its first row, else the larger of c and what it was;
+    where it grows, the rows before the new ones are rounded again to the new scale.
+    New rows hold round(x / scale), NaN 0 in int8.  What int8 rows lose so: half a step of
+    their scale at first, and up to another half each time that it grows.
+
     q [T, H_q, D] bf16: returned rotated, [T, H_q, D] bf16 (with T = B,
     q_rot.unsqueeze(2) is paged_decode_attn's query); zeros in rows that have no
     position.  Without q the result is None.
@@ -154,14 +219,29 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
     Blocks that receive tokens must belong to one sequence each, and be named once
     in its table row (blocks of a shared prefix are only read).  The caches and
     min / max must be memory of their own, without expanded dims."""
+    if _by_block(k_scale, v_scale):
+        out = None if meta is not None else native().paged_append_blocks(
+            k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, bool(interleaved), k_scale, v_scale)
+        if out is not None:
+            return out if q is not None else None
+        if meta is not None:
+            raise ValueError("meta is not kept for caches with a scale for each block")
+        return _append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, interleaved, None,
+                       k_scale, v_scale)
     kmin, kmax = meta if meta is not None else (None, None)
     out = native().paged_append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin,
                                 bool(interleaved), kmin, kmax, k_scale, v_scale)
     if out is not None:
         return out if q is not None else None
-    C.cuda_tensors(k, v, k_paged, v_paged, block_table, context_lens,
+    return _append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, interleaved, meta, k_scale,
+                   v_scale)
+
+
+def _append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, interleaved, meta, k_scale, v_scale):
+    """paged_kv_append where the native path does not take the call."""
+    C.cuda_tensors(k, v, k_paged, v_paged, block_table, context_lens, *_tensors(k_scale, v_scale),
                    *(t for t in (cu_seqlens, q, cos, sin, *(meta or ())) if t is not None))
-    N, Hk, bs, D, fp8 = _cache(k_paged, v_paged, k_scale, v_scale)
+    N, Hk, bs, D, typ = _typed_cache(k_paged, v_paged, k_scale, v_scale)
     C.ndim(k, 3, "k"), C.ndim(v, 3, "v")
     C.dtype_in(k, "k", torch.bfloat16), C.dtype_in(v, "v", torch.bfloat16)
     T = k.shape[0]
@@ -197,6 +277,9 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
             raise ValueError(f"cos, sin hold {P} positions, the block table {bt.shape[1] * bs}")
         cos, sin = C.rows16(cos), C.rows16(sin)
     _written(k_paged, v_paged, ("k_paged", "v_paged"))
+    if typ >= 2:
+        _written(k_scale, v_scale, ("k_scale", "v_scale"))
+    kmin = kmax = None
     if meta is not None:
         kmin, kmax = _meta(meta, N, Hk, D)
         _written(kmin, kmax, ("kmin", "kmax"))
@@ -209,11 +292,21 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
         return out.zero_() if out is not None else None
     z = lambda t, i: t.stride(i) if t is not None else 0    # noqa: E731
     p = lambda t: ptr(t) if t is not None else None          # noqa: E731
+    if typ >= 2:
+        scales, _ = _scale_args(k_scale, v_scale, typ, 1.0)
+        with torch.cuda.device(k_paged.device):
+            call("bytes_paged_kv_append_blocks", ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1),
+                 p(q), z(q, 0), z(q, 1), p(out), z(out, 0), z(out, 1),
+                 ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),
+                 ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), typ, *scales,
+                 ptr(bt), bt.stride(0), ptr(cl), p(cu_seqlens), p(cos), z(cos, 0), p(sin), z(sin, 0), int(P), int(rot),
+                 int(bool(interleaved)), T, B, Hq, Hk, D, bs, N, bt.shape[1], stream_of(k_paged))
+        return out
     with torch.cuda.device(k_paged.device):
         call("bytes_paged_kv_append", ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1),
              p(q), z(q, 0), z(q, 1), p(out), z(out, 0), z(out, 1),
              ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),
-             ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), int(fp8), p(kmin), p(kmax),
+             ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), typ, p(kmin), p(kmax),
              ptr(bt), bt.stride(0), ptr(cl), p(cu_seqlens), p(cos), z(cos, 0), p(sin), z(sin, 0), int(P), int(rot),
              int(bool(interleaved)), float(k_scale), float(v_scale), T, B, Hq, Hk, D, bs, N, bt.shape[1],
              stream_of(k_paged))
@@ -221,15 +314,20 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
 
 
 def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Tensor, block_table: torch.Tensor,
-                      context_lens: torch.Tensor, scale: float = 1.0, *, k_scale: float = 1.0,
-                      v_scale: float = 1.0) -> torch.Tensor:
+                      context_lens: torch.Tensor, scale: float = 1.0, *, window: Optional[int] = None, sinks: int = 0,
+                      k_scale: Scale = 1.0, v_scale: Scale = 1.0) -> torch.Tensor:
     """softmax(scale * q.K^T) V of one new token per sequence over the cache.
 
     q [B,H_q,1,D] bf16; `scale` as in decode_attn_bf16 (default 1.0; pass
     1/sqrt(D) for standard attention).  For fp8 caches the rows stand for
-    k * k_scale and v * v_scale.  fp32 scores, softmax and sums.  An infinite value
+    k * k_scale and v * v_scale, with scales for the tensor, or for each block and KV
+    head.  With a window the token sees the latest `window` tokens (itself among
+    them) and the first `sinks`; what lies between is not read, and its blocks
+    may be gone from the table.  fp32 scores, softmax and sums.  An infinite value
     that takes part gives that infinity, unless its weight underflows fp32 (below
     2^-100 of the row's largest it may give NaN).  Returns [B,H_q,1,D] bf16."""
+    if window is not None or sinks or _by_block(k_scale, v_scale):
+        return _window_attn(q, k_paged, v_paged, block_table, context_lens, scale, window, sinks, k_scale, v_scale)
     out = native().paged_decode(q, k_paged, v_paged, block_table, context_lens, scale, k_scale, v_scale)
     if out is not None:
         return out
@@ -249,6 +347,84 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
              ptr(cl), ptr(out), out.stride(0), out.stride(1), B, Hq, Hk, D, bs, N, W, float(scale) * float(k_scale),
              float(v_scale), ptr(ws), ws.numel(), stream_of(q))
     return out.unsqueeze(2)
+
+
+def _window_attn(q, k_paged, v_paged, block_table, context_lens, scale, window, sinks, k_scale, v_scale):
+    out = native().paged_window(q, k_paged, v_paged, block_table, context_lens, scale, window, sinks, k_scale, v_scale)
+    if out is not None:
+        return out
+    C.cuda_tensors(q, k_paged, v_paged, block_table, context_lens,
+                   *_tensors(k_scale, v_scale))
+    N, Hk, bs, D, typ = _typed_cache(k_paged, v_paged, k_scale, v_scale)
+    window, sinks = _window(window, sinks)
+    qs, B, Hq = _query(q, Hk, D)
+    bt, cl = _tables(block_table, context_lens, B, bs)
+    W = bt.shape[1]
+    scales, factors = _scale_args(k_scale, v_scale, typ, scale)
+    with torch.cuda.device(q.device):
+        out = torch.empty((B, Hq, D), dtype=torch.bfloat16, device=q.device)
+        n = size_query("bytes_paged_window_workspace_size", B, Hq, Hk, D, typ, bs, W, window, sinks)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+        call("bytes_paged_window_attn", ptr(qs), qs.stride(0), qs.stride(1),
+             ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),
+             ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), typ, *scales, ptr(bt), bt.stride(0),
+             ptr(cl), ptr(out), out.stride(0), out.stride(1), B, Hq, Hk, D, bs, N, W, window, sinks, *factors, ptr(ws),
+             ws.numel(), stream_of(q))
+    return out.unsqueeze(2)
+
+
+def paged_prompt_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Tensor, block_table: torch.Tensor,
+                      context_lens: torch.Tensor, cu_seqlens: torch.Tensor, scale: float = 1.0, *,
+                      window: Optional[int] = None, sinks: int = 0, k_scale: Scale = 1.0,
+                      v_scale: Scale = 1.0) -> torch.Tensor:
+    """Causal attention of several new tokens per sequence over the cache that holds
+    them: whole prompts, chunks of them, draft tokens.
+
+    q [T,H_q,D] bf16, as paged_kv_append returns it: sequence b's new tokens are rows
+    cu_seqlens[b] .. cu_seqlens[b+1] (int32 [B+1], ascending from 0) and end at
+    position context_lens[b] - 1.  The token at position p attends over the tokens
+    t <= p of its sequence that take part; with a window, over those with
+    t > p - window or t < sinks.  Caches, scales and `scale` as in paged_decode_attn.
+    fp32 scores, softmax and sums; weights rounded to bf16 for the value product.
+    An infinite or NaN value reaches the rows that see its token only; one that takes
+    part gives that infinity, unless its weight underflows (NaN then).  Rows without a
+    position, without a token to see, and past cu_seqlens[B] get zeros.  Returns
+    [T,H_q,D] bf16."""
+    out = native().paged_prompt(q, k_paged, v_paged, block_table, context_lens, cu_seqlens, scale, window, sinks, k_scale,
+                                v_scale)
+    if out is not None:
+        return out
+    C.cuda_tensors(q, k_paged, v_paged, block_table, context_lens, cu_seqlens,
+                   *_tensors(k_scale, v_scale))
+    N, Hk, bs, D, typ = _typed_cache(k_paged, v_paged, k_scale, v_scale)
+    window, sinks = _window(window, sinks)
+    C.ndim(q, 3, "q")
+    C.dtype_in(q, "q", torch.bfloat16)
+    T, Hq, Dq = q.shape
+    if Dq != D or Hq == 0:
+        raise ValueError(f"q must be [T, H_q, D] with D={D}; got {tuple(q.shape)}")
+    if Hq % Hk != 0:
+        raise ValueError(f"H_q={Hq} is not a multiple of H_k={Hk}")
+    B = block_table.shape[0] if block_table.dim() == 2 else 0
+    bt, cl = _tables(block_table, context_lens, B, bs)
+    if tuple(cu_seqlens.shape) != (B + 1,):
+        raise ValueError(f"cu_seqlens must be [B + 1] = [{B + 1}]; got {tuple(cu_seqlens.shape)}")
+    cu = _int32(cu_seqlens, "cu_seqlens").contiguous()
+    q = C.rows16(q)
+    W = bt.shape[1]
+    scales, factors = _scale_args(k_scale, v_scale, typ, scale)
+    with torch.cuda.device(q.device):
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+        if T == 0 or B == 0:
+            return out.zero_()
+        n = size_query("bytes_paged_prompt_workspace_size", T, B, Hq, Hk, D, bs, W, window, sinks)
+        ws = torch.empty(max(n, 16), dtype=torch.uint8, device=q.device)
+        call("bytes_paged_prompt_attn", ptr(q), q.stride(0), q.stride(1),
+             ptr(k_paged), k_paged.stride(0), k_paged.stride(1), k_paged.stride(2),
+             ptr(v_paged), v_paged.stride(0), v_paged.stride(1), v_paged.stride(2), typ, *scales, ptr(bt), bt.stride(0),
+             ptr(cl), ptr(cu), ptr(out), out.stride(0), out.stride(1), T, B, Hq, Hk, D, bs, N, W, window, sinks, *factors,
+             ptr(ws), ws.numel(), stream_of(q))
+    return out
 
 
 def paged_page_scores(q: torch.Tensor, meta: Meta, block_table: torch.Tensor, context_lens: torch.Tensor,
@@ -302,6 +478,8 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     [B,H_q,1,D] bf16 (and the selected blocks' places in the table, int32
     [B,H_q,min(ceil(kb / block_size), max_blocks)] ascending, if return_pages;
     places past a short sequence's blocks stand for nothing)."""
+    if _by_block(k_scale, v_scale):
+        raise ValueError("page-sparse decode takes caches with one scale for the tensor")
     if not return_pages:
         out = native().paged_quest(q, k_paged, v_paged, *meta, block_table, context_lens, kb, scaling, local_w, k_scale,
                                    v_scale)

@@ -552,6 +552,81 @@ int bytes_paged_quest_attn(const void* q, int64_t q_sb, int64_t q_sh, const void
                            int max_blocks, float scale, float v_scale, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* ---------------------------------------------------------------------------
+ * More of the paged dense caches: scales by block, windows, prompts, tables.
+ * kv_type: 0 bf16, 1 e4m3 with one scale for the tensor (part of scale, and
+ * v_scale), 2 e4m3 and 3 int8 with a scale for each block and KV head: k_scales,
+ * v_scales fp32 [num_blocks, Hk] (strides *_sb, *_sh; NULL for types 0 and 1),
+ * finite and not negative, a row standing for code * scale.  window: 1 or more
+ * tokens, 2^30 or more for none; sinks: the first tokens, which stay visible.
+ * The rest as above.
+ *
+ * bytes_paged_kv_append_blocks: bytes_paged_kv_append into caches of kv_type 2
+ *   or 3 (no kmin, kmax).  For every block that receives tokens and every head,
+ *   with a = max |x| over its new rows (infinities as the largest bf16 number,
+ *   NaN not counted) and c = a / 127 (int8) or the smallest power of two of at
+ *   least a / 448 (e4m3, at least 2^-126; 0 for a = 0): the scale becomes c
+ *   where a token enters the block at its first row, else max(scale, c); the rows
+ *   before the new ones, where it grows, become round(code * (old / new)); new
+ *   rows are round(x / scale), to nearest even (NaN: 0 in int8, NaN in e4m3).
+ * bytes_paged_window_attn: bytes_paged_decode_attn over the tokens t >=
+ *   context_lens[b] - window or t < sinks that take part.  Workspace:
+ *   bytes_paged_window_workspace_size (may be 0), contents arbitrary.
+ * bytes_paged_prompt_attn: out [T, Hq, D] bf16 (strides o_st, o_sh): attention
+ *   of the rows cu_seqlens[b] .. cu_seqlens[b + 1] of q [T, Hq, D] bf16, whose
+ *   positions p end at context_lens[b] - 1, over the tokens t <= p that take
+ *   part, t > p - window or t < sinks.  Rows without a position in 0 ..
+ *   max_blocks * block_size, without a token that takes part, and of no sequence
+ *   get zeros.  Workspace: bytes_paged_prompt_workspace_size (may be 0),
+ *   contents arbitrary.
+ * bytes_paged_resize: one step of a batch's tables.  In place: block_table
+ *   [B, max_blocks], context_lens [B], and the free blocks as a ring
+ *   free_blocks [num_blocks] with free_range = (head, count).  For b in order,
+ *   with n = context_lens[b] held to 0 .. max_blocks * block_size and kept =
+ *   min(n, max(keep[b], 0)) (keep NULL: n): blocks of places from ceil(kept /
+ *   block_size) to ceil(n / block_size) go to the ring's end, entries -1; with a
+ *   window (0: none) those of the places that name a block, going down from
+ *   (kept - window + 1) / block_size - 1 to ceil(sinks / block_size), too, up to
+ *   the first that names none.  new_lens[b] tokens are granted if they fit the
+ *   row, the ring (as it was; blocks asked for by the sequences before included)
+ *   and T (likewise), else none; their blocks leave the ring's start.  context_lens[b] =
+ *   kept + granted[b]; cu_seqlens [B + 1] sums granted; for the rows t <
+ *   cu_seqlens[B] of T: seqs, positions (int32), slots (int64: block *
+ *   block_size + row, -1 without a block); -1 in the rest.  Nothing overlaps.
+ *   Workspace: bytes_paged_resize_workspace_size, contents arbitrary.
+ * ------------------------------------------------------------------------- */
+int bytes_paged_kv_append_blocks(const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                                 const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                                 void* k_paged, int64_t kp_sb, int64_t kp_sh, int64_t kp_ss, void* v_paged, int64_t vp_sb,
+                                 int64_t vp_sh, int64_t vp_ss, int kv_type, void* k_scales, int64_t ks_sb, int64_t ks_sh,
+                                 void* v_scales, int64_t vs_sb, int64_t vs_sh, const void* block_table, int64_t bt_sb,
+                                 const void* context_lens, const void* cu_seqlens, const void* cos, int64_t cos_st,
+                                 const void* sin, int64_t sin_st, int positions, int rot, int interleaved, int T, int B,
+                                 int Hq, int Hk, int D, int block_size, int num_blocks, int max_blocks, void* stream);
+int bytes_paged_window_workspace_size(int B, int Hq, int Hk, int D, int kv_type, int block_size, int max_blocks,
+                                      int window, int sinks, size_t* bytes);
+int bytes_paged_window_attn(const void* q, int64_t q_sb, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
+                            int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_type,
+                            const void* k_scales, int64_t ks_sb, int64_t ks_sh, const void* v_scales, int64_t vs_sb,
+                            int64_t vs_sh, const void* block_table, int64_t bt_sb, const void* context_lens, void* out,
+                            int64_t o_sb, int64_t o_sh, int B, int Hq, int Hk, int D, int block_size, int num_blocks,
+                            int max_blocks, int window, int sinks, float scale, float v_scale, void* workspace,
+                            size_t workspace_bytes, void* stream);
+int bytes_paged_prompt_workspace_size(int T, int B, int Hq, int Hk, int D, int block_size, int max_blocks, int window,
+                                      int sinks, size_t* bytes);
+int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const void* k_paged, int64_t k_sb, int64_t k_sh,
+                            int64_t k_ss, const void* v_paged, int64_t v_sb, int64_t v_sh, int64_t v_ss, int kv_type,
+                            const void* k_scales, int64_t ks_sb, int64_t ks_sh, const void* v_scales, int64_t vs_sb,
+                            int64_t vs_sh, const void* block_table, int64_t bt_sb, const void* context_lens,
+                            const void* cu_seqlens, void* out, int64_t o_st, int64_t o_sh, int T, int B, int Hq, int Hk,
+                            int D, int block_size, int num_blocks, int max_blocks, int window, int sinks, float scale,
+                            float v_scale, void* workspace, size_t workspace_bytes, void* stream);
+int bytes_paged_resize_workspace_size(int B, size_t* bytes);
+int bytes_paged_resize(void* block_table, int64_t bt_sb, void* context_lens, void* free_blocks, void* free_range,
+                       const void* keep, const void* new_lens, void* cu_seqlens, void* granted, void* seqs,
+                       void* positions, void* slots, int B, int max_blocks, int num_blocks, int T, int block_size,
+                       int window, int sinks, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif
