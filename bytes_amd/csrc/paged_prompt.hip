@@ -80,12 +80,16 @@ __device__ __forceinline__ bool find_tile(const PromptArgs& a, int r, int lane, 
 // The first n of 64 bits.
 __device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
 
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-// The largest exponent fields of bf16 pairs so far and of eight more; an infinity or NaN has all ones there.
-__device__ __forceinline__ u16x2 exponents(u16x2 m, const u32x4& x) {
+// Eight bf16 numbers with infinities and NaN made 0; odd: whether there were any.
+__device__ __forceinline__ u32x4 finite_only(const u32x4& x, bool& odd) {
+  u32x4 r;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[j] & 0x7F807F80u));
-  return m;
+  for (int j = 0; j < 4; ++j) {
+    const bool lo = (x[j] & 0x7F80u) == 0x7F80u, hi = (x[j] & 0x7F800000u) == 0x7F800000u;
+    r[j] = x[j] & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
+    odd = odd | lo | hi;
+  }
+  return r;
 }
 
 __device__ __forceinline__ float half_max(float v) {   // of a lane and its partner lane ^ 32
@@ -118,7 +122,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
   // scales of a tile's tokens: in scalar registers where 16 of them share a block, else in LDS
   constexpr bool SCALES_LDS = SCALED && !HALVES;
   __shared__ float sc[2][SCALES_LDS ? 128 : 1];
-  __shared__ int bad[2];
+  __shared__ int odd_tiles;                        // some had an infinity or NaN left out
 
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l32 = lane & 31, e = lane >> 5;
@@ -137,21 +141,23 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
     }
     return;
   }
-  const int p0 = a.c.lens[x.b] - x.n;              // the first new token's position
+  // (what all lanes share goes to scalar registers)
+  auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  const int p0 = same(a.c.lens[x.b] - x.n);        // the first new token's position
   const int p = p0 + i;
   const bool placed = exists && p >= 0 && p < a.cap;
   const int first = fast_div(x.r0, a.dG), last = min(fast_div(x.r0 + kPromptRows - 1, a.dG), x.n - 1);
-  const int p_lo = max(p0 + first, 0), p_hi = min(p0 + last, a.cap - 1);
+  const int p_lo = same(max(p0 + first, 0)), p_hi = same(min(p0 + last, a.cap - 1));
   // this wave's positions
   const int wl = fast_div(min(x.r0 + w * 32, rows - 1), a.dG), wh = fast_div(min(x.r0 + w * 32 + 31, rows - 1), a.dG);
   const bool wave_any = x.r0 + w * 32 < rows;
-  const int w_lo = max(p0 + wl, 0), w_hi = wave_any ? min(p0 + wh, a.cap - 1) : -1;
+  const int w_lo = same(max(p0 + wl, 0)), w_hi = same(wave_any ? min(p0 + wh, a.cap - 1) : -1);
   // keys: tiles of the sinks, then from the window's first one on
   const int end = max(p_hi + 1, 0), lo_key = max(p_lo - a.window + 1, 0);
-  const int near_tiles = (min(a.sinks, end) + kKeys - 1) / kKeys * kKeys;
-  const int gap = max(lo_key / kKeys * kKeys - near_tiles, 0);
+  const int near_tiles = (min(a.sinks, end) + kKeys - 1) & -kKeys;
+  const int gap = max((lo_key & -kKeys) - near_tiles, 0);
   const int ntiles = p_lo > p_hi ? 0 : (end - gap + kKeys - 1) / kKeys;
-  const int j0 = (int)((int64_t)ntiles * split / a.nsplit), j1 = (int)((int64_t)ntiles * (split + 1) / a.nsplit);
+  const int j0 = same((int)((int64_t)ntiles * split / a.nsplit)), j1 = same((int)((int64_t)ntiles * (split + 1) / a.nsplit));
 
   bf16x8 qb[KK];
   {
@@ -175,6 +181,11 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
   const Elem* kb = static_cast<const Elem*>(a.c.k) + hk * a.c.k_sh;
   const Elem* vb = static_cast<const Elem*>(a.c.v) + hk * a.c.v_sh;
   const int r_in = lane / CPR, col = lane % CPR;
+  // HALVES: this lane's row among the 16 that its wave's instructions read of, and its column
+  const int row16 = (w * RPW & 15) + r_in;
+  const int kcol = BYTES ? col : kswz<D>(w * RPW + r_in, col), vcol = BYTES ? col : vswz<D>(w * RPW + r_in, col);
+  const uint32_t ko = row16 * (int)a.c.k_ss + kcol * EPC, vo = row16 * (int)a.c.v_ss + vcol * EPC;
+  static_assert(RPI % 8 == 0 && (D / 8) % 8 == 0 && (RPI % (D / 8) == 0 || BYTES), "the swizzle is that of the instruction's first row");
   auto start = [&](int j) { return j * kKeys < near_tiles ? j * kKeys : j * kKeys + gap; };
   // tile j's table entries: lane l's token is start(j) + l
   auto fetch = [&](int j) {
@@ -191,23 +202,36 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
     t.ok = t.ok && in;
     t.id = in ? t.id : 0;
   };
-  u32x4 kr[NI], vr[NI];
-  auto issue = [&](const PagedIds& t) {
+  // Tile j's rows: bf16 ones go to LDS on their own (lane l's 16 bytes to the wave's place + 16 l,
+  // so the swizzle is in the column that it reads), bytes to registers first.
+  constexpr bool DMA = !BYTES && HALVES;
+  constexpr int NR = DMA ? 1 : NI;
+  u32x4 kr[NR], vr[NR];
+  auto issue = [&](const PagedIds& t, int to) {
+    // every lane its own token's place: 64-bit products once a tile
+    const int64_t ka = t.id * a.c.k_sb + t.off * a.c.k_ss, va = t.id * a.c.v_sb + t.off * a.c.v_ss;
+    auto at = [](int64_t x, int l) {
+      return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32 |
+                       (uint32_t)__builtin_amdgcn_readlane((int)x, l));
+    };
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
       const int base = u * RPI + w * RPW;          // this wave's rows of the instruction
-      int id, off;
-      if constexpr (HALVES) {
-        const int g = base & ~15;
-        id = __builtin_amdgcn_readlane(t.id, g);
-        off = __builtin_amdgcn_readlane(t.off, g) + (base - g) + r_in;
+      if constexpr (HALVES) {                      // all in one block: one scalar base
+        const Elem *kp = kb + at(ka, base & ~15), *vp = vb + at(va, base & ~15);
+        if constexpr (DMA) {
+          char* to_k = smem[to] + base * (D * 2);
+          lds_dma16<false>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
+          lds_dma16<false>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
+        } else {
+          kr[u] = ld16(kp + ko);
+          vr[u] = ld16(vp + vo);
+        }
       } else {
-        id = __shfl(t.id, base + r_in, 64);
-        off = __shfl(t.off, base + r_in, 64);
+        kr[u] = ld16(kb + __shfl(ka, base + r_in, 64) + col * EPC);
+        vr[u] = ld16(vb + __shfl(va, base + r_in, 64) + col * EPC);
+        asm volatile("" ::: "memory");             // (one row's addresses in registers at a time)
       }
-      kr[u] = ld16(kb + (int64_t)id * a.c.k_sb + (int64_t)off * a.c.k_ss + col * EPC);
-      vr[u] = ld16(vb + (int64_t)id * a.c.v_sb + (int64_t)off * a.c.v_ss + col * EPC);
-      if constexpr (!HALVES) asm volatile("" ::: "memory");          // (one row's addresses in registers at a time)
     }
   };
   float kscale = 0.f, vscale = 0.f, kg[4], vg[4];
@@ -218,30 +242,46 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
       vscale = t.ok ? y : 0.f;
     }
   };
-  // Into buffer `to`; values of slots that are no token become 0.  Returns whether values
-  // of this lane's are infinite or NaN.
-  auto stage = [&](int to, uint64_t named) {
+  // They are in buffer `to` after this and a barrier.  CHECK, tiles that some rows do not see
+  // whole: values of slots that are no token become 0, as do infinities and NaN, which no
+  // weight of 0 would take away; returns whether this lane met any.
+  auto finish = [&](int to, uint64_t named, auto check) {
+    constexpr bool CHECK = decltype(check)::value;
     char *kst = smem[to], *vst = kst + VT;
-    u16x2 ex = {0, 0};
+    bool odd = false;
+    if constexpr (DMA) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if constexpr (CHECK) {
 #pragma unroll
-    for (int u = 0; u < NI; ++u) {
-      const int rr = u * RPI + w * RPW + r_in;
-      const uint32_t keep = (named >> rr) & 1 ? ~0u : 0u;
-      vr[u] &= u32x4{keep, keep, keep, keep};
-      if constexpr (BYTES) {
-        u32x4 k0, k1, v0, v1;
-        bytes16_to_bf16<TYPE == kInt8Blocks>(kr[u], k0, k1);
-        bytes16_to_bf16<TYPE == kInt8Blocks>(vr[u], v0, v1);
-        if (TYPE != kInt8Blocks) ex = exponents(exponents(ex, v0), v1);
-        *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * col) * 16) = k0;
-        *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * col + 1) * 16) = k1;
-        *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * col) * 16) = v0;
-        *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * col + 1) * 16) = v1;
-        asm volatile("" ::: "memory");
-      } else {
-        ex = exponents(ex, vr[u]);
-        *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, col) * 16) = kr[u];
-        *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, col) * 16) = vr[u];
+        for (int u = 0; u < NI; ++u) {
+          const int rr = u * RPI + w * RPW + r_in;
+          u32x4* at = reinterpret_cast<u32x4*>(vst + (u * RPI + w * RPW) * (D * 2) + lane * 16);
+          const u32x4 v = *at;
+          *at = (named >> rr) & 1 ? finite_only(v, odd) : u32x4{0, 0, 0, 0};
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < NI; ++u) {
+        const int rr = u * RPI + w * RPW + r_in;
+        if constexpr (CHECK) {
+          const uint32_t keep = (named >> rr) & 1 ? ~0u : 0u;
+          vr[u] &= u32x4{keep, keep, keep, keep};
+        }
+        if constexpr (BYTES) {
+          u32x4 k0, k1, v0, v1;
+          bytes16_to_bf16<TYPE == kInt8Blocks>(kr[u], k0, k1);
+          bytes16_to_bf16<TYPE == kInt8Blocks>(vr[u], v0, v1);
+          if constexpr (CHECK && TYPE != kInt8Blocks) v0 = finite_only(v0, odd), v1 = finite_only(v1, odd);
+          *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * col) * 16) = k0;
+          *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, 2 * col + 1) * 16) = k1;
+          *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * col) * 16) = v0;
+          *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, 2 * col + 1) * 16) = v1;
+        } else {
+          *reinterpret_cast<u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, col) * 16) = kr[u];
+          *reinterpret_cast<u32x4*>(vst + rr * (D * 2) + vswz<D>(rr, col) * 16) = CHECK ? finite_only(vr[u], odd) : vr[u];
+        }
+        asm volatile("" ::: "memory");             // (one row's conversion in registers at a time)
       }
     }
     if constexpr (SCALES_LDS) {
@@ -254,14 +294,22 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
         vg[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vscale), 16 * g));
       }
     }
-    return ex[0] == 0x7F80 || ex[1] == 0x7F80;
+    return odd;
+  };
+  // Whether all rows at positions lo .. hi see all of the tile at t0.
+  auto all_see = [&](int t0, int lo, int hi) {
+    return t0 + kKeys - 1 <= lo && (t0 > hi - a.window || t0 + kKeys <= a.sinks);
   };
 
+  // The tile's keys that this lane's row sees.
+  auto seen = [&](int t0, uint64_t named) {
+    return placed ? named & low_bits(p - t0 + 1) & (~low_bits(p - a.window + 1 - t0) | low_bits(a.sinks - t0)) : 0ull;
+  };
   // One staged tile.
-  auto compute = [&](int from, int t0, uint64_t named, bool infinite) {
+  auto compute = [&](int from, int t0, uint64_t named) {
     const char *kst = smem[from], *vst = kst + VT;
     // keys that all of the wave's rows see
-    const bool whole = named == ~0ull && t0 + kKeys - 1 <= w_lo && (t0 > w_hi - a.window || t0 + kKeys <= a.sinks);
+    const bool whole = named == ~0ull && all_see(t0, w_lo, w_hi);
     f32x16 s[2];
 #pragma unroll
     for (int blk = 0; blk < 2; ++blk) {
@@ -282,9 +330,8 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
         for (int u = 0; u < 16; ++u)
           s[blk][u] *= SCALES_LDS ? sc[from][blk * 32 + (u >> 2) * 8 + e * 4 + (u & 3)] : kg[2 * blk + (u >> 3)];
     }
-    uint64_t see = ~0ull;
     if (!whole) {
-      see = placed ? named & low_bits(p - t0 + 1) & (~low_bits(p - a.window + 1 - t0) | low_bits(a.sinks - t0)) : 0ull;
+      const uint64_t see = seen(t0, named);
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk) {
         const uint32_t m = (uint32_t)(see >> (32 * blk)) >> (4 * e);
@@ -311,36 +358,6 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
     }
     const float mc = m_run == kNegInf ? 0.f : m_run * a.scale_log2;
     auto weight = [&](float x) { return fast_exp2(__builtin_fmaf(x, a.scale_log2, -mc)); };
-    if (TYPE != kInt8Blocks && !whole && infinite) {
-      // A weight of 0 times an infinite value is not 0: one key at a time, rows that do not
-      // see it leaving their sums as they are.
-#pragma unroll 1
-      for (int k = 0; k < kKeys; ++k) {
-        const int in = k & 31, u_of = (in >> 3) * 4 + (in & 3), half = (in >> 2) & 1;
-        float mine = 0.f;
-#pragma unroll
-        for (int u = 0; u < 16; ++u) mine = u == u_of ? (k < 32 ? s[0][u] : s[1][u]) : mine;
-        float pk = weight(__shfl(mine, l32 + 32 * half, 64));
-        l_run += e == half ? pk : 0.f;
-        if constexpr (SCALES_LDS) pk *= sc[from][64 + k];
-        else if constexpr (SCALED) pk *= k < 32 ? (k < 16 ? vg[0] : vg[1]) : (k < 48 ? vg[2] : vg[3]);
-        const bool sees = (see >> k) & 1;
-#pragma unroll
-        for (int db = 0; db < DB; ++db)
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int d = db * 32 + 8 * g + 4 * e;
-            const u32x2 v = *reinterpret_cast<const u32x2*>(vst + k * (D * 2) + vswz<D>(k, d >> 3) * 16 + (d & 7) * 2);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const float vv = __uint_as_float(u & 1 ? v[u >> 1] & 0xFFFF0000u : v[u >> 1] << 16);
-              acc[db][4 * g + u] = sees ? __builtin_fmaf(pk, vv, acc[db][4 * g + u]) : acc[db][4 * g + u];
-            }
-            asm volatile("" ::: "memory");         // (few registers for a path that is hardly taken)
-          }
-      }
-      return;
-    }
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       bf16x8 pb;
@@ -367,25 +384,63 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
   };
 
   if (j0 < j1) {
-    if (threadIdx.x < 2) bad[threadIdx.x] = 0;
-    PagedIds now = fetch(j0), next = fetch(j0 + 1);
-    settle(now);
-    scales(now);
-    issue(now);
+    if (threadIdx.x == 0) odd_tiles = 0;
+    PagedIds next = fetch(j0);
+    settle(next);
+    uint64_t named = 0, named_next = __ballot(next.ok);
+    scales(next);
+    issue(next, j0 & 1);
+    next = fetch(j0 + 1);
     __syncthreads();
+    auto done = [&](int j) {                       // tile j is in LDS
+      const int t0 = start(j);
+      if (named_next == ~0ull && all_see(t0, p_lo, p_hi)) finish(j & 1, named_next, std::false_type{});
+      else if (__any(finish(j & 1, named_next, std::true_type{})) && lane == 0) odd_tiles = 1;
+      named = named_next;
+      lds_barrier();
+    };
+    done(j0);
     for (int j = j0; j < j1; ++j) {
-      const int buf = j & 1, t0 = start(j);
-      const uint64_t named = __ballot(now.ok);
-      // (buffer `buf` was last read two tiles ago, before the barrier of the last one)
-      const bool odd = stage(buf, named);
-      if (__any(odd) && lane == 0) bad[buf] = j + 1;
-      settle(next);
-      now = next;
-      next = fetch(j + 2);
-      scales(now);
-      if (j + 1 < j1) issue(now);
-      __syncthreads();
-      if (t0 <= w_hi) compute(buf, t0, named, bad[buf] == j + 1);
+      const bool more = j + 1 < j1;
+      if (more) {                                  // (the other buffer was last read before the barrier)
+        settle(next);
+        named_next = __ballot(next.ok);
+        scales(next);
+        issue(next, (j + 1) & 1);
+        next = fetch(j + 2);
+      }
+      const int t0 = start(j);
+      if (t0 <= w_hi) compute(j & 1, t0, named);
+      if (more) done(j + 1);
+    }
+    if (TYPE != kInt8Blocks && odd_tiles) {
+      // Infinities and NaN that were left out: rows that see them take them, others do not.
+      // Again through the tiles that some row does not see whole, without weights: any
+      // above 0 gives the same.
+      for (int j = j0; j < j1; ++j) {
+        PagedIds t = fetch(j);
+        settle(t);
+        const uint64_t there = __ballot(t.ok);
+        const int t0 = start(j);
+        if (there == ~0ull && all_see(t0, p_lo, p_hi)) continue;
+        const uint64_t see = seen(t0, there);
+        for (int k = 0; k < kKeys; ++k) {
+          if (!((there >> k) & 1)) continue;
+          const int id = __builtin_amdgcn_readlane(t.id, k), off = __builtin_amdgcn_readlane(t.off, k);
+          const Elem* vp = vb + (int64_t)id * a.c.v_sb + (int64_t)off * a.c.v_ss;
+          const bool mine = (see >> k) & 1;
+#pragma unroll
+          for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int u = 0; u < 16; ++u) {
+              const int d = db * 32 + 8 * (u >> 2) + 4 * e + (u & 3);
+              const uint32_t raw = vp[d];
+              const float v = BYTES ? ((raw & 0x7Fu) == 0x7Fu ? __builtin_nanf("") : 0.f) : __uint_as_float(raw << 16);
+              if (mine && (__float_as_uint(v) & 0x7F800000u) == 0x7F800000u) acc[db][u] += v;
+              asm volatile("" ::: "memory");       // (few registers for a path that is hardly taken)
+            }
+        }
+      }
     }
   }
 

@@ -219,7 +219,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
     Blocks that receive tokens must belong to one sequence each, and be named once
     in its table row (blocks of a shared prefix are only read).  The caches and
     min / max must be memory of their own, without expanded dims."""
-    if _by_block(k_scale, v_scale):
+    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale):
         out = None if meta is not None else native().paged_append_blocks(
             k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, bool(interleaved), k_scale, v_scale)
         if out is not None:
@@ -326,7 +326,8 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     may be gone from the table.  fp32 scores, softmax and sums.  An infinite value
     that takes part gives that infinity, unless its weight underflows fp32 (below
     2^-100 of the row's largest it may give NaN).  Returns [B,H_q,1,D] bf16."""
-    if window is not None or sinks or _by_block(k_scale, v_scale):
+    if window is not None or sinks or (
+            not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale)):
         return _window_attn(q, k_paged, v_paged, block_table, context_lens, scale, window, sinks, k_scale, v_scale)
     out = native().paged_decode(q, k_paged, v_paged, block_table, context_lens, scale, k_scale, v_scale)
     if out is not None:
@@ -478,7 +479,7 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     [B,H_q,1,D] bf16 (and the selected blocks' places in the table, int32
     [B,H_q,min(ceil(kb / block_size), max_blocks)] ascending, if return_pages;
     places past a short sequence's blocks stand for nothing)."""
-    if _by_block(k_scale, v_scale):
+    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale):
         raise ValueError("page-sparse decode takes caches with one scale for the tensor")
     if not return_pages:
         out = native().paged_quest(q, k_paged, v_paged, *meta, block_table, context_lens, kb, scaling, local_w, k_scale,
