@@ -26,8 +26,6 @@ namespace bytes_amd {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPromptWaves = 4;
-constexpr int kPromptRows = kPromptWaves * 32;
 constexpr int kKeys = 64;            // of a tile
 constexpr float kSlack = 8.f;        // log2 of how far weights may pass 1
 
@@ -45,7 +43,8 @@ struct PromptArgs {
   int T, B, Hk, G, D;
   int cap, window, sinks;            // no window: 2^30
   int nsplit, tiles;                 // parts of a unit's keys; row tiles at most
-  int flip, pad;                     // the scale is negative: queries change sign
+  int flip;                          // the scale is negative: queries change sign
+  int once;                          // a cache row is read by about one workgroup
   float scale_log2, v_scale;
   FastDiv dHk, dG, dsplit;
 };
@@ -110,13 +109,14 @@ __device__ __forceinline__ void store_bf16x4(uint16_t* out, const f32x16& x, int
   *reinterpret_cast<u32x2*>(out) = __builtin_bit_cast(u32x2, r);
 }
 
-template <int D, int TYPE, bool HALVES>
-__global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 1 : 2) void paged_prompt_kernel(PromptArgs a) {
+// NW waves of 32 rows.
+template <int D, int TYPE, bool HALVES, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 4 && D == 128 && TYPE == kBf16Cache && !HALVES ? 1 : 2) void paged_prompt_kernel(PromptArgs a) {
   constexpr bool BYTES = TYPE != kBf16Cache, SCALED = TYPE >= kE4m3Blocks;
   using Elem = typename std::conditional<BYTES, uint8_t, uint16_t>::type;
   constexpr int EPC = 16 / (int)sizeof(Elem), CPR = D / EPC;         // elements per chunk, chunks per row
-  constexpr int RPW = 64 / CPR, RPI = kPromptWaves * RPW, NI = kKeys / RPI;
-  static_assert(RPW <= 16 && NI >= 1, "a wave's rows of one instruction lie in 16 of a block");
+  constexpr int RPW = 64 / CPR, RPI = NW * RPW, NI = RPI < kKeys ? kKeys / RPI : 1;
+  static_assert(RPW <= 16, "a wave's rows of one instruction lie in 16 of a block");
   constexpr int KK = D / 16, DB = D / 32, VT = kKeys * D * 2;
   __shared__ __attribute__((aligned(16))) char smem[2][2 * VT];      // [buffer][K, V]
   // scales of a tile's tokens: in scalar registers where 16 of them share a block, else in LDS
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
   const int tile = a.tiles - 1 - (int)blockIdx.x / per;              // the last rows, which see most, first
   const int rest = (int)blockIdx.x % per, split = fast_div(rest, a.dHk), hk = rest - split * a.Hk;
   RowTile x;
-  if (!find_tile<kPromptRows>(a, tile, lane, x)) return;
+  if (!find_tile<NW * 32>(a, tile, lane, x)) return;
   const int row = x.r0 + w * 32 + l32, rows = x.n * a.G;
   const bool exists = row < rows;
   const int i = fast_div(exists ? row : 0, a.dG), h = hk * a.G + (exists ? row : 0) - i * a.G;
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
   const int p0 = same(a.c.lens[x.b] - x.n);        // the first new token's position
   const int p = p0 + i;
   const bool placed = exists && p >= 0 && p < a.cap;
-  const int first = fast_div(x.r0, a.dG), last = min(fast_div(x.r0 + kPromptRows - 1, a.dG), x.n - 1);
+  const int first = fast_div(x.r0, a.dG), last = min(fast_div(x.r0 + NW * 32 - 1, a.dG), x.n - 1);
   const int p_lo = same(max(p0 + first, 0)), p_hi = same(min(p0 + last, a.cap - 1));
   // this wave's positions
   const int wl = fast_div(min(x.r0 + w * 32, rows - 1), a.dG), wh = fast_div(min(x.r0 + w * 32 + 31, rows - 1), a.dG);
@@ -217,12 +217,18 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
 #pragma unroll
     for (int u = 0; u < NI; ++u) {
       const int base = u * RPI + w * RPW;          // this wave's rows of the instruction
+      if (RPI > kKeys && base >= kKeys) break;
       if constexpr (HALVES) {                      // all in one block: one scalar base
         const Elem *kp = kb + at(ka, base & ~15), *vp = vb + at(va, base & ~15);
         if constexpr (DMA) {
           char* to_k = smem[to] + base * (D * 2);
-          lds_dma16<false>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
-          lds_dma16<false>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
+          if (a.once) {
+            lds_dma16<true>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
+            lds_dma16<true>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
+          } else {
+            lds_dma16<false>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
+            lds_dma16<false>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
+          }
         } else {
           kr[u] = ld16(kp + ko);
           vr[u] = ld16(vp + vo);
@@ -255,6 +261,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
 #pragma unroll
         for (int u = 0; u < NI; ++u) {
           const int rr = u * RPI + w * RPW + r_in;
+          if (RPI > kKeys && rr >= kKeys) break;
           u32x4* at = reinterpret_cast<u32x4*>(vst + (u * RPI + w * RPW) * (D * 2) + lane * 16);
           const u32x4 v = *at;
           *at = (named >> rr) & 1 ? finite_only(v, odd) : u32x4{0, 0, 0, 0};
@@ -264,6 +271,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
 #pragma unroll
       for (int u = 0; u < NI; ++u) {
         const int rr = u * RPI + w * RPW + r_in;
+        if (RPI > kKeys && rr >= kKeys) break;
         if constexpr (CHECK) {
           const uint32_t keep = (named >> rr) & 1 ? ~0u : 0u;
           vr[u] &= u32x4{keep, keep, keep, keep};
@@ -312,17 +320,26 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
     const bool whole = named == ~0ull && all_see(t0, w_lo, w_hi);
     f32x16 s[2];
 #pragma unroll
-    for (int blk = 0; blk < 2; ++blk) {
+    for (int blk = 0; blk < 2; ++blk)
 #pragma unroll
       for (int u = 0; u < 16; ++u) s[blk][u] = 0.f;
-      const int rr = blk * 32 + l32;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int blk = 0; blk < 2; ++blk) {
+        const int rr = blk * 32 + l32;
         const bf16x8 ka = __builtin_bit_cast(
             bf16x8, *reinterpret_cast<const u32x4*>(kst + rr * (D * 2) + kswz<D>(rr, kk * 2 + e) * 16));
         s[blk] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qb[kk], s[blk], 0, 0, 0);
       }
+    // four reads of K ahead of the products that take them
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int z = 0; z < 2 * KK - 4; ++z) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
     }
+    __builtin_amdgcn_sched_group_barrier(0x008, 4, 0);
     if constexpr (SCALED) {
 #pragma unroll
       for (int blk = 0; blk < 2; ++blk)
@@ -447,7 +464,7 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
   l_run = half_sum(l_run);
   if (!placed) l_run = 0.f;                        // a row without a position gets zeros
   if (a.nsplit > 1) {
-    const size_t slot = (((size_t)tile * a.Hk + hk) * a.nsplit + split) * kPromptRows + w * 32 + l32;
+    const size_t slot = (((size_t)tile * a.Hk + hk) * a.nsplit + split) * (NW * 32) + w * 32 + l32;
     if (!exists) return;
     float* pa = a.part_acc + slot * D;
 #pragma unroll
@@ -469,8 +486,9 @@ __global__ __launch_bounds__(kPromptWaves * 64, TYPE == kBf16Cache && !HALVES ? 
 }
 
 // Joins the parts of a row's keys: one wave per (row of q, query head, 64 dims).
-template <int D>
+template <int D, int NW>
 __global__ __launch_bounds__(64) void paged_prompt_join_kernel(PromptArgs a) {
+  constexpr int ROWS = NW * 32;
   constexpr int NSL = D / 64;
   const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
   const int slice = blockIdx.y % NSL, h = blockIdx.y / NSL, t = blockIdx.x;
@@ -480,15 +498,15 @@ __global__ __launch_bounds__(64) void paged_prompt_join_kernel(PromptArgs a) {
     const int b = b0 + lane, bc = min(b, a.B - 1);
     const int c0 = min(max(a.cu[bc], 0), a.T), c1 = min(max(a.cu[bc + 1], 0), a.T);
     const int n = b < a.B ? max(c1 - c0, 0) : 0;
-    const uint32_t mine = (uint32_t)((n * a.G + kPromptRows - 1) / kPromptRows);
+    const uint32_t mine = (uint32_t)((n * a.G + ROWS - 1) / ROWS);
     const uint32_t incl = wave_prefix_sum(mine);
     const unsigned long long in = __ballot(n > 0 && t >= c0 && t < c0 + n);
     if (in) {
       const int l = __ffsll(in) - 1;
       const int i = t - __builtin_amdgcn_readlane(c0, l), hk = fast_div(h, a.dG);
-      const int row = i * a.G + h - hk * a.G, tile = tiles + __builtin_amdgcn_readlane((int)(incl - mine), l) + row / kPromptRows;
-      const size_t base = ((size_t)tile * a.Hk + hk) * a.nsplit * kPromptRows + row % kPromptRows;
-      auto slot = [&](int u) { return base + (size_t)u * kPromptRows; };
+      const int row = i * a.G + h - hk * a.G, tile = tiles + __builtin_amdgcn_readlane((int)(incl - mine), l) + row / ROWS;
+      const size_t base = ((size_t)tile * a.Hk + hk) * a.nsplit * ROWS + row % ROWS;
+      auto slot = [&](int u) { return base + (size_t)u * ROWS; };
       paged_join<4>(a.nsplit, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
                     reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4,
                     [&](const f32x4& A, float L) {
@@ -501,41 +519,53 @@ __global__ __launch_bounds__(64) void paged_prompt_join_kernel(PromptArgs a) {
   }
 }
 
-// Row tiles of a batch, at most: whole ones, and one that is not full per sequence (and
-// of the rows past the last); none without rows.
-static int64_t prompt_tiles(int64_t T, int64_t B, int64_t G) {
-  const int64_t n = T * G / kPromptRows + B + 1, most = T;
-  return n < most ? n : most;
-}
-// Parts that a unit's keys are cut into: enough that two workgroups come to each CU, none
-// of fewer than 8 key tiles of a full table row.
-static int prompt_split(int64_t units, int64_t cap) {
-  const int64_t cus = device_cu_count(), want = (2 * cus + units - 1) / units, most = cap / (8 * kKeys);
+// How a call is cut up.
+struct PromptPlan {
+  int waves, nsplit;                 // of a workgroup; parts of a unit's keys
+  int64_t tiles, units;              // row tiles, and (row tile, KV head) pairs, at most
+  int rows() const { return waves * 32; }
+  size_t workspace(int D) const { return nsplit < 2 ? 0 : (size_t)units * nsplit * rows() * (D + 2) * 4; }
+};
+// cap: positions that a table row holds.
+static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int64_t cap, int window, int sinks) {
+  const int64_t cus = device_cu_count();
+  PromptPlan p;
+  // whole row tiles, and one that is not full per sequence (and of the rows past the
+  // last); none without rows
+  auto cut = [&](int waves) {
+    p.waves = waves;
+    const int64_t n = T * G / p.rows() + B + 1, most = T * ((G + p.rows() - 1) / p.rows());
+    p.tiles = n < most ? n : most;
+    p.units = p.tiles * Hk;
+  };
+  cut(8);
+  if (p.units < cus) cut(4);
+  // parts: enough that two workgroups come to each CU, none of fewer than 8 key tiles of
+  // the slots that a row can see
+  const int64_t see = (int64_t)window + sinks + p.rows() + 2 * kKeys, slots = cap < see ? cap : see;
+  const int64_t want = p.units < cus ? (2 * cus + p.units - 1) / (p.units < 1 ? 1 : p.units) : 1, most = slots / (8 * kKeys);
   const int64_t n = want < most ? want : most;
-  return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
-}
-static int64_t prompt_slots(int64_t cap, int window, int sinks) {
-  const int64_t most = (int64_t)window + sinks + kPromptRows + 2 * kKeys;
-  return cap < most ? cap : most;
-}
-static size_t prompt_workspace(int64_t units, int nsplit, int D) {
-  return nsplit < 2 ? 0 : (size_t)units * nsplit * kPromptRows * (D + 2) * 4;
+  p.nsplit = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+  return p;
 }
 
-template <int TYPE>
-static int launch_prompt(const PromptArgs& a, dim3 grid, hipStream_t st) {
-  const bool halves = paged_halves(a.c);
-  const dim3 block(kPromptWaves * 64);
-#define PP(DD, H) hipLaunchKernelGGL((paged_prompt_kernel<DD, TYPE, H>), grid, block, 0, st, a)
-  if (a.D == 128) {
-    if (halves) PP(128, true);
-    else PP(128, false);
-  } else {
-    if (halves) PP(64, true);
-    else PP(64, false);
-  }
-#undef PP
+template <int D, int TYPE, bool HALVES>
+static int launch_prompt(const PromptArgs& a, const PromptPlan& plan, hipStream_t st) {
+  const dim3 grid((unsigned)(plan.units * plan.nsplit)), block(plan.waves * 64);
+  if (plan.waves == 8) hipLaunchKernelGGL((paged_prompt_kernel<D, TYPE, HALVES, 8>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((paged_prompt_kernel<D, TYPE, HALVES, 4>), grid, block, 0, st, a);
+  int rc = (int)hipGetLastError();
+  if (rc || plan.nsplit < 2) return rc;
+  const dim3 jgrid((unsigned)a.T, (unsigned)(a.Hk * a.G * (D / 64)));
+  if (plan.waves == 8) hipLaunchKernelGGL((paged_prompt_join_kernel<D, 8>), jgrid, dim3(64), 0, st, a);
+  else hipLaunchKernelGGL((paged_prompt_join_kernel<D, 4>), jgrid, dim3(64), 0, st, a);
   return (int)hipGetLastError();
+}
+template <int TYPE>
+static int launch_prompt_of(const PromptArgs& a, int D, const PromptPlan& plan, hipStream_t st) {
+  const bool halves = paged_halves(a.c);
+  if (D == 128) return halves ? launch_prompt<128, TYPE, true>(a, plan, st) : launch_prompt<128, TYPE, false>(a, plan, st);
+  return halves ? launch_prompt<64, TYPE, true>(a, plan, st) : launch_prompt<64, TYPE, false>(a, plan, st);
 }
 
 }  // namespace bytes_amd
@@ -554,9 +584,7 @@ int bytes_paged_prompt_workspace_size(int T, int B, int Hq, int Hk, int D, int b
     *bytes = 0;
     return 0;
   }
-  const int64_t units = prompt_tiles(T, B, Hq / Hk) * Hk;
-  const int64_t slots = prompt_slots((int64_t)max_blocks * block_size, window, sinks);
-  *bytes = prompt_workspace(units, prompt_split(units, slots), D);
+  *bytes = prompt_plan(T, B, Hk, Hq / Hk, (int64_t)max_blocks * block_size, window, sinks).workspace(D);
   return 0;
 }
 
@@ -574,14 +602,15 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   const int rc0 = paged_check(block_size, num_blocks, max_blocks);
   if (rc0) return rc0;
   if (T == 0) return 0;
-  const int64_t G = Hq / Hk, tiles = prompt_tiles(T, B, G), units = tiles * Hk;
+  const int64_t G = Hq / Hk;
+  const PromptPlan plan = prompt_plan(T, B, Hk, G, (int64_t)max_blocks * block_size, window, sinks);
   PromptArgs a = {};
   a.window = window < (1 << 30) ? window : (1 << 30), a.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
-  a.nsplit = prompt_split(units, prompt_slots((int64_t)max_blocks * block_size, window, sinks));
-  if ((int64_t)T * G + kPromptRows > 0x7FFFFFFF || units * a.nsplit > 0x7FFFFFFF || T > (1 << 30) ||
+  a.nsplit = plan.nsplit;
+  if ((int64_t)T * G + plan.rows() > 0x7FFFFFFF || plan.units * plan.nsplit > 0x7FFFFFFF || T > (1 << 30) ||
       (int64_t)Hq * (D / 64) > 65535)
     return (int)hipErrorInvalidConfiguration;
-  if (a.nsplit > 1 && (!workspace || workspace_bytes < prompt_workspace(units, a.nsplit, D))) return (int)hipErrorInvalidValue;
+  if (plan.nsplit > 1 && (!workspace || workspace_bytes < plan.workspace(D))) return (int)hipErrorInvalidValue;
   a.c.k = k_paged, a.c.k_sb = k_sb, a.c.k_sh = k_sh, a.c.k_ss = k_ss;
   a.c.v = v_paged, a.c.v_sb = v_sb, a.c.v_sh = v_sh, a.c.v_ss = v_ss;
   a.c.table = static_cast<const int32_t*>(block_table), a.c.bt_sb = bt_sb;
@@ -594,28 +623,22 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   a.ks = static_cast<const float*>(k_scales), a.ks_sb = ks_sb, a.ks_sh = ks_sh;
   a.vs = static_cast<const float*>(v_scales), a.vs_sb = vs_sb, a.vs_sh = vs_sh;
   a.part_ml = static_cast<float*>(workspace);
-  a.part_acc = a.part_ml + (size_t)units * a.nsplit * kPromptRows * 2;
+  a.part_acc = a.part_ml + (size_t)plan.units * plan.nsplit * plan.rows() * 2;
   a.T = T, a.B = B, a.Hk = Hk, a.G = (int)G, a.D = D;
   a.cap = max_blocks * block_size;
-  a.tiles = (int)tiles;
+  a.tiles = (int)plan.tiles;
   a.flip = scale < 0.f ? 1 : 0;
+  a.once = T * G <= (int64_t)B * plan.rows() ? 1 : 0;
   // (at least the smallest normal number: times -inf, a masked score, it is -inf)
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f), a.v_scale = v_scale;
   a.dHk = make_fastdiv((uint32_t)Hk), a.dG = make_fastdiv((uint32_t)G), a.dsplit = make_fastdiv((uint32_t)a.nsplit);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(units * a.nsplit));
-  int rc = 0;
   switch (kv_type) {
-    case kBf16Cache: rc = launch_prompt<kBf16Cache>(a, grid, st); break;
-    case kFp8Cache: rc = launch_prompt<kFp8Cache>(a, grid, st); break;
-    case kE4m3Blocks: rc = launch_prompt<kE4m3Blocks>(a, grid, st); break;
-    default: rc = launch_prompt<kInt8Blocks>(a, grid, st);
+    case kBf16Cache: return launch_prompt_of<kBf16Cache>(a, D, plan, st);
+    case kFp8Cache: return launch_prompt_of<kFp8Cache>(a, D, plan, st);
+    case kE4m3Blocks: return launch_prompt_of<kE4m3Blocks>(a, D, plan, st);
+    default: return launch_prompt_of<kInt8Blocks>(a, D, plan, st);
   }
-  if (rc || a.nsplit < 2) return rc;
-  const dim3 jgrid((unsigned)T, (unsigned)(Hq * (D / 64)));
-  if (D == 128) hipLaunchKernelGGL(paged_prompt_join_kernel<128>, jgrid, dim3(64), 0, st, a);
-  else hipLaunchKernelGGL(paged_prompt_join_kernel<64>, jgrid, dim3(64), 0, st, a);
-  return (int)hipGetLastError();
 }
 
 }  // extern "C"

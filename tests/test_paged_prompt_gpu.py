@@ -88,6 +88,15 @@ def test_few_rows_over_long_contexts(dev, kind, B, Hq, Hk, D, L, new, bs, window
     _check(out, q, kc, vc, D ** -0.5, ks, vs, table, n, cu, window, kw.get("sinks", 0), some)
 
 
+@pytest.mark.parametrize("Hq,Hk,D", [(160, 1, 64), (257, 1, 128), (384, 2, 64)])
+def test_groups_of_more_heads_than_a_workgroup_has_rows(dev, Hq, Hk, D):
+    """One token's heads are several row tiles: fewer tokens than tiles."""
+    g = torch.Generator().manual_seed(Hq)
+    for lens, new in (([1], [1]), ([40, 70], [3, 1])):
+        q, kc, vc, ks, vs, table, n, cu = _batch(g, lens, new, 16, Hq, Hk, D, "bf16")
+        _check(_run(dev, q, kc, vc, ks, vs, table, n, cu, D ** -0.5), q, kc, vc, D ** -0.5, ks, vs, table, n, cu)
+
+
 def test_long_prompt_rows(dev):
     """Rows all over a prompt of many tiles, against the decode of each as the last token."""
     g = torch.Generator().manual_seed(1)
