@@ -821,15 +821,25 @@ PyObject* paged_resize(const Tensor& bt, const Tensor& cl, const Tensor& ring, c
   c10::DeviceGuard guard(bt.device());
   size_t n = 0;
   need(bytes_paged_resize_workspace_size((int)B, &n) == 0);
-  Tensor ws = empty(bt, {(int64_t)n}, at::kByte);
-  Tensor cu = empty(bt, {B + 1}, at::kInt), granted = empty(bt, {B}, at::kInt), seqs = empty(bt, {T}, at::kInt),
-         positions = empty(bt, {T}, at::kInt), slots = empty(bt, {T}, at::kLong);
+  // the outputs and the workspace in one allocation (a step of 32 sequences, us a call: six of their own 9.0, so 6.2)
+  Tensor all = empty(bt, {8 * T + 4 * (2 * T + 2 * B + 1) + (int64_t)n}, at::kByte);
+  int64_t used = 0;
+  auto part = [&](int64_t len, at::ScalarType dt) {
+    const auto type = c10::scalarTypeToTypeMeta(dt);
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), type);
+    t.unsafeGetTensorImpl()->set_storage_offset(used / (int64_t)type.itemsize());
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({len});
+    used += len * (int64_t)type.itemsize();
+    return t;
+  };
+  Tensor slots = part(T, at::kLong), cu = part(B + 1, at::kInt), granted = part(B, at::kInt), seqs = part(T, at::kInt),
+         positions = part(T, at::kInt);
+  char* ws = static_cast<char*>(all.mutable_data_ptr()) + used;
   void* st = stream_of(bt);
   launch("bytes_paged_resize", bytes_paged_resize, bt.mutable_data_ptr(), bt.stride(0), cl.mutable_data_ptr(),
          ring.mutable_data_ptr(), range.mutable_data_ptr(), keep ? data(*keep) : nullptr, data(fresh),
          cu.mutable_data_ptr(), granted.mutable_data_ptr(), seqs.mutable_data_ptr(), positions.mutable_data_ptr(),
-         slots.mutable_data_ptr(), (int)B, (int)W, (int)N, (int)T, (int)bs, (int)window, (int)sinks, ws.mutable_data_ptr(),
-         n, st);
+         slots.mutable_data_ptr(), (int)B, (int)W, (int)N, (int)T, (int)bs, (int)window, (int)sinks, ws, n, st);
   return Py_BuildValue("(NNNNN)", THPVariable_Wrap(cu), THPVariable_Wrap(granted), THPVariable_Wrap(seqs),
                        THPVariable_Wrap(positions), THPVariable_Wrap(slots));
 }

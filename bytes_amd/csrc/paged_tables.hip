@@ -19,8 +19,10 @@
 // (waves take those with many), four prefix sums with a carry, the lengths.
 // Fill: a wave per sequence moves its blocks, a thread per token finds its sequence
 // in cu.  Small steps run both in one launch.
-// Bound by latency and launches: nothing here is read or written twice, and a step of
-// 32 sequences moves 3 KB.
+// Bound by latency and launches: nothing here is read or written twice. A step of 32
+// sequences that moves 3 KB takes 5.3 us in one launch (lengths, entries, two rounds of
+// sums, the ring and the outputs follow one another), one of 256 with 34K new tokens 7.6
+// and 3.6 in two.  (Sixteen waves to the plan: 5.8, and 7.5 and 3.6.)
 #include "common.h"
 
 namespace bytes_amd {
@@ -44,41 +46,57 @@ constexpr int kPlanWaves = 8, kPlanThreads = kPlanWaves * 64;
 constexpr int kFillThreads = 256;
 constexpr int kBySelf = 4;           // places that a thread counts alone
 constexpr int kCuLds = 4096;         // sequences whose cu fits the fill's LDS
+constexpr int kSmallB = 128, kSmallT = 1024;   // a step that one workgroup takes in one launch
 
 __device__ __forceinline__ bool names(int id, int N) { return id >= 0 && id < N; }
 __device__ __forceinline__ int places(const TablesArgs& a, int n) { return fast_div(n + a.bs - 1, a.dbs); }
 
-__device__ __forceinline__ int64_t wave_scan64(int64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
-  return v;
+// Sums that stay at the largest number once they reach it: what is asked for may be more
+// than 32 bits hold, and then is more than there is.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+// wave_prefix_sum with such sums.
+__device__ __forceinline__ uint32_t wave_prefix_sat(uint32_t x) {
+  x = add_sat(x, dpp_u32<0x111>(x));
+  x = add_sat(x, dpp_u32<0x112>(x));
+  x = add_sat(x, dpp_u32<0x114>(x));
+  x = add_sat(x, dpp_u32<0x118>(x));
+  x = add_sat(x, dpp_u32<0x142, 0xA>(x));
+  return add_sat(x, dpp_u32<0x143, 0xC>(x));
 }
-// Inclusive prefix sum over the workgroup's threads; total of all in `total`.
-__device__ __forceinline__ int64_t group_scan64(int64_t v, int64_t* sums, int64_t& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  v = wave_scan64(v, lane);
-  __syncthreads();
-  if (lane == 63) sums[w] = v;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
+// Inclusive prefix sums of N numbers over the workgroup's threads, and their totals.
+template <int N>
+__device__ __forceinline__ void group_scan(uint32_t (&v)[N], uint32_t (*sums)[N], uint32_t (&total)[N]) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-  for (int i = 0; i < kPlanWaves; ++i) {
-    if (i < w) before += sums[i];
-    total += sums[i];
+  for (int k = 0; k < N; ++k) v[k] = wave_prefix_sat(v[k]);
+  __syncthreads();
+  if (lane == 63) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) sums[w][k] = v[k];
   }
-  return v + before;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    uint32_t before = 0;
+    total[k] = 0;
+    for (int i = 0; i < kPlanWaves; ++i) {
+      if (i < w) before = add_sat(before, sums[i][k]);
+      total[k] = add_sat(total[k], sums[i][k]);
+    }
+    v[k] = add_sat(v[k], before);
+  }
 }
 
 // Places of [lo, hi) of a row that name a block.
 __device__ __forceinline__ int count_named(const int32_t* row, int lo, int hi, int N, int lane) {
+  constexpr int U = 4;                             // loads in flight
   int n = 0;
-  for (int j0 = lo; j0 < hi; j0 += 64) {
-    const int j = j0 + lane;
-    n += __popcll(__ballot(j < hi && names(row[min(j, hi - 1)], N)));
+  for (int j0 = lo; j0 < hi; j0 += U * 64) {
+    int id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = row[min(j0 + u * 64 + lane, hi - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u) n += __popcll(__ballot(j0 + u * 64 + lane < hi && names(id[u], N)));
   }
   return n;
 }
@@ -95,19 +113,20 @@ __device__ __forceinline__ int run_down(const int32_t* row, int lo, int hi, int 
 }
 
 struct PlanShared {
-  int64_t sums[kPlanWaves];
+  uint32_t asked[kPlanWaves][3], given[kPlanWaves][2];
   int big[kPlanThreads];
   int back[kPlanThreads], run[kPlanThreads];
   int nbig;
 };
 
-__device__ __forceinline__ void make_plan(const TablesArgs& a, PlanShared& sh) {
+// cu and plan: in memory, or the workgroup's own.
+__device__ __forceinline__ void make_plan(const TablesArgs& a, PlanShared& sh, int32_t* cu, int32_t* plan) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int count = min(max(a.range[1], 0), a.N);
   int head = a.range[0];
   head = head >= 0 && head < a.N ? head : 0;
   const int s_lo = fast_div(min(a.sinks, a.cap) + a.bs - 1, a.dbs);
-  int64_t asked_blocks = 0, asked_tokens = 0;      // of the sequences before these
+  uint32_t asked_blocks = 0, asked_tokens = 0;     // of the sequences before these
   int blocks = 0, tokens = 0, given = 0;
   for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
     const int b = b0 + tid;
@@ -126,14 +145,21 @@ __device__ __forceinline__ void make_plan(const TablesArgs& a, PlanShared& sh) {
     const int32_t* row = a.table + (int64_t)bc * a.bt_sb;
     int back = 0, r_lo = r_hi;
     bool big = false;
-    if (live) {
-      if (last - first <= kBySelf) {
-        for (int j = first; j < last; ++j) back += names(row[j], a.N);
-      } else {
-        big = true;
+    {                                              // (loads of a place that is there, all at once)
+      int ends[kBySelf], run[kBySelf];
+#pragma unroll
+      for (int i = 0; i < kBySelf; ++i) {
+        ends[i] = row[min(first + i, a.W - 1)];
+        run[i] = row[max(r_hi - 1 - i, 0)];
       }
-      for (int i = 0; i < kBySelf && r_lo > r_lo0 && names(row[r_lo - 1], a.N); ++i) --r_lo;
-      big = big || (r_hi - r_lo == kBySelf && r_lo > r_lo0);
+      bool on = live;
+#pragma unroll
+      for (int i = 0; i < kBySelf; ++i) {
+        back += live && first + i < last && names(ends[i], a.N) ? 1 : 0;
+        on = on && r_hi - 1 - i >= r_lo0 && names(run[i], a.N);
+        r_lo -= on ? 1 : 0;
+      }
+      big = live && (last - first > kBySelf || (on && r_lo > r_lo0));
     }
     __syncthreads();
     if (tid == 0) sh.nbig = 0;
@@ -154,38 +180,36 @@ __device__ __forceinline__ void make_plan(const TablesArgs& a, PlanShared& sh) {
     r_lo = sh.run[tid];
     back = live ? sh.back[tid] + (r_hi - r_lo) : 0;
     // what fits
-    int64_t total_b, total_t;
-    const int64_t cb = asked_blocks + group_scan64(need, sh.sums, total_b);
-    const int64_t ct = asked_tokens + group_scan64(m, sh.sums, total_t);
-    asked_blocks += total_b;
-    asked_tokens += total_t;
-    const bool ok = (need == 0 || cb <= count) && ct <= a.T;
+    uint32_t c[3] = {(uint32_t)need, (uint32_t)m, (uint32_t)back}, t[3];
+    group_scan(c, sh.asked, t);
+    const bool ok = (need == 0 || add_sat(asked_blocks, c[0]) <= (uint32_t)count) && add_sat(asked_tokens, c[1]) <= (uint32_t)a.T;
+    asked_blocks = add_sat(asked_blocks, t[0]);
+    asked_tokens = add_sat(asked_tokens, t[1]);
     const int got = ok ? m : 0, gneed = ok ? need : 0;
-    // blocks and tokens granted (each under 2^31 in all), and blocks that come back
-    int64_t t1, t2;
-    const int64_t c1 = group_scan64(((int64_t)gneed << 32) | (uint32_t)got, sh.sums, t1);
-    const int64_t c2 = group_scan64(back, sh.sums, t2);
+    uint32_t g[2] = {(uint32_t)gneed, (uint32_t)got}, tg[2];
+    group_scan(g, sh.given, tg);
     if (live) {
-      int32_t* p = a.plan + b;
-      p[kKept * (int64_t)a.B] = kept;
-      p[kLast * (int64_t)a.B] = last;
-      p[kNeed * (int64_t)a.B] = gneed;
-      p[kStart * (int64_t)a.B] = blocks + (int)(c1 >> 32) - gneed;
-      p[kBack * (int64_t)a.B] = given + (int)c2 - back;
-      p[kRunLo * (int64_t)a.B] = r_lo;
-      p[kRunHi * (int64_t)a.B] = r_hi;
+      int32_t* p = plan + b;
+      const int64_t B = a.B;
+      p[kKept * B] = kept;
+      p[kLast * B] = last;
+      p[kNeed * B] = gneed;
+      p[kStart * B] = blocks + (int)g[0] - gneed;
+      p[kBack * B] = given + (int)c[2] - back;
+      p[kRunLo * B] = r_lo;
+      p[kRunHi * B] = r_hi;
       a.granted[b] = got;
       a.lens[b] = kept + got;
-      a.cu[b] = tokens + (int)(uint32_t)c1 - got;
+      cu[b] = a.cu[b] = tokens + (int)g[1] - got;
     }
-    blocks += (int)(t1 >> 32);
-    tokens += (int)(uint32_t)t1;
-    given += (int)t2;
+    blocks += (int)tg[0];
+    tokens += (int)tg[1];
+    given += (int)t[2];
   }
   __syncthreads();                                 // (range has been read by all)
   if (tid == 0) {
-    a.cu[a.B] = tokens;
-    int32_t* was = a.plan + (int64_t)kPlanRows * a.B;
+    cu[a.B] = a.cu[a.B] = tokens;
+    int32_t* was = plan + (int64_t)kPlanRows * a.B;
     was[0] = head;
     was[1] = count;
     int next = head + blocks;                      // (below 2 N, held to 31 bits by the host's check)
@@ -194,15 +218,18 @@ __device__ __forceinline__ void make_plan(const TablesArgs& a, PlanShared& sh) {
   }
 }
 
-__device__ __forceinline__ int ring_at(const TablesArgs& a, int head, int64_t i) { return (int)((head + i) % a.N); }
+__device__ __forceinline__ int ring_at(const TablesArgs& a, int head, int64_t i) {
+  const int64_t x = head + i;                      // below 2 N in a pool that is one
+  return (int)(x < a.N ? x : x < 2 * (int64_t)a.N ? x - a.N : x % a.N);
+}
 
 // One wave: the blocks of sequence b that go back and come.
-__device__ __forceinline__ void move_blocks(const TablesArgs& a, int b, int lane) {
-  const int32_t* p = a.plan + b;
+__device__ __forceinline__ void move_blocks(const TablesArgs& a, const int32_t* plan, int b, int lane) {
+  const int32_t* p = plan + b;
   const int64_t B = a.B;
   const int kept = p[kKept * B], last = p[kLast * B], need = p[kNeed * B], start = p[kStart * B];
   const int r_lo = p[kRunLo * B], r_hi = p[kRunHi * B];
-  const int head = a.plan[kPlanRows * B], count = a.plan[kPlanRows * B + 1];
+  const int head = plan[kPlanRows * B], count = plan[kPlanRows * B + 1];
   int64_t to = (int64_t)count + p[kBack * B];
   int32_t* row = a.table + (int64_t)b * a.bt_sb;
   for (int j = r_lo + lane; j < r_hi; j += 64) {
@@ -224,24 +251,23 @@ __device__ __forceinline__ void move_blocks(const TablesArgs& a, int b, int lane
 }
 
 // Token t of the step: its sequence (the one whose cu range holds it), position and slot.
-template <class CU>
-__device__ __forceinline__ void place_token(const TablesArgs& a, int t, const CU& cu) {
+__device__ __forceinline__ void place_token(const TablesArgs& a, const int32_t* plan, int t, const int32_t* cu) {
   int b = -1, p = -1;
   int64_t slot = -1;
-  if (t < cu(a.B)) {
-    int lo = 0, hi = a.B - 1;                      // the last b with cu(b) <= t
+  if (t < cu[a.B]) {
+    int lo = 0, hi = a.B - 1;                      // the last b with cu[b] <= t
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (cu(mid) <= t) lo = mid;
+      if (cu[mid] <= t) lo = mid;
       else hi = mid - 1;
     }
     b = lo;
     const int64_t B = a.B;
-    const int kept = a.plan[kKept * B + b];
-    p = kept + t - cu(b);
+    const int kept = plan[kKept * B + b];
+    p = kept + t - cu[b];
     const int j = fast_div(p, a.dbs), first = places(a, kept);
     const int id = j < first ? a.table[b * a.bt_sb + j]
-                             : a.ring[ring_at(a, a.plan[kPlanRows * B], a.plan[kStart * B + b] + (j - first))];
+                             : a.ring[ring_at(a, plan[kPlanRows * B], plan[kStart * B + b] + (j - first))];
     if (names(id, a.N)) slot = (int64_t)id * a.bs + (p - j * a.bs);
   }
   a.seqs[t] = b;
@@ -251,17 +277,18 @@ __device__ __forceinline__ void place_token(const TablesArgs& a, int t, const CU
 
 __global__ __launch_bounds__(kPlanThreads) void paged_tables_plan_kernel(TablesArgs a) {
   __shared__ PlanShared sh;
-  make_plan(a, sh);
+  make_plan(a, sh, a.cu, a.plan);
 }
 
+// A step of few sequences and tokens, by one workgroup that keeps the plan to itself.
 __global__ __launch_bounds__(kPlanThreads) void paged_tables_small_kernel(TablesArgs a) {
   __shared__ PlanShared sh;
-  make_plan(a, sh);
+  __shared__ int32_t cu[kSmallB + 1], plan[kPlanRows * kSmallB + 2];
+  make_plan(a, sh, cu, plan);
   __syncthreads();
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  auto cu = [&](int b) { return a.cu[b]; };
-  for (int t = threadIdx.x; t < a.T; t += kPlanThreads) place_token(a, t, cu);
-  for (int b = w; b < a.B; b += kPlanWaves) move_blocks(a, b, lane);
+  for (int t = threadIdx.x; t < a.T; t += kPlanThreads) place_token(a, plan, t, cu);
+  for (int b = w; b < a.B; b += kPlanWaves) move_blocks(a, plan, b, lane);
 }
 
 __global__ __launch_bounds__(kFillThreads) void paged_tables_fill_kernel(TablesArgs a, int seq_wgs) {
@@ -269,16 +296,16 @@ __global__ __launch_bounds__(kFillThreads) void paged_tables_fill_kernel(TablesA
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   if ((int)blockIdx.x < seq_wgs) {
     const int b = blockIdx.x * (kFillThreads / 64) + w;
-    if (b < a.B) move_blocks(a, b, lane);
+    if (b < a.B) move_blocks(a, a.plan, b, lane);
     return;
   }
   const int64_t t = ((int64_t)blockIdx.x - seq_wgs) * kFillThreads + tid;
   if (a.B <= kCuLds) {
     for (int i = tid; i <= a.B; i += kFillThreads) lcu[i] = a.cu[i];
     __syncthreads();
-    if (t < a.T) place_token(a, (int)t, [&](int b) { return lcu[b]; });
+    if (t < a.T) place_token(a, a.plan, (int)t, lcu);
   } else if (t < a.T) {
-    place_token(a, (int)t, [&](int b) { return a.cu[b]; });
+    place_token(a, a.plan, (int)t, a.cu);
   }
 }
 
@@ -320,7 +347,7 @@ int bytes_paged_resize(void* block_table, int64_t bt_sb, void* context_lens, voi
   a.window = window < (1 << 30) ? window : (1 << 30), a.sinks = sinks;
   a.dbs = make_fastdiv((uint32_t)block_size);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (B <= 64 && T <= 2048) {
+  if (B <= kSmallB && T <= kSmallT) {
     hipLaunchKernelGGL(paged_tables_small_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
     return (int)hipGetLastError();
   }
