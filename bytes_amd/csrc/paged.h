@@ -296,13 +296,13 @@ struct PagedScales {
   float* lds;
 };
 
-// Slots [s, s_end) in steps of `step` (s a multiple of 32 from the first slot):
-// online softmax over them into m_run, l_run, acc.
-template <int D, int TYPE, bool HALVES, class FIND>
-__device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t* table, int hk, int s, int s_end,
-                                                int step, int lane, float scale_log2, const bf16x8 (&qb)[D / 32],
-                                                char* wbuf, const FIND& find, float& m_run, float& l_run,
-                                                f32x4 (&acc)[D / 16], const PagedScales& sc = PagedScales{}) {
+// Slots [s, s_end) in steps of `step` (s a multiple of 32 from the first slot), 32 at a time:
+// compute(first slot, which of them are tokens) with their rows staged in wbuf, keys and then
+// values; ready(first slot, rows) before that may change the values in registers.
+template <int D, int TYPE, bool HALVES, class FIND, class READY, class COMPUTE>
+__device__ __forceinline__ void paged_wave_tiles(const PagedKv& c, const int32_t* table, int hk, int s, int s_end,
+                                                 int step, int lane, char* wbuf, const FIND& find,
+                                                 const PagedScales& sc, const READY& ready, const COMPUTE& compute) {
   constexpr bool SCALED = TYPE >= kE4m3Blocks;
   if (s >= s_end) return;
   char* kst = wbuf;
@@ -337,6 +337,7 @@ __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t*
   for (; s < s_end; s += step) {
     const uint32_t vmask = (uint32_t)__ballot(now.ok);
     wave_lds_sync();
+    ready(s, rows);
     rows.stage(vmask, kst, vst);
     if constexpr (SCALED) sc.lds[lane] = scaled;
     settle(next);
@@ -345,8 +346,23 @@ __device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t*
     scaled = scale(now);
     rows.issue(now, s + step < s_end);
     wave_lds_sync();
-    paged_tile<D, TYPE == kBf16Cache, SCALED>(vmask, scale_log2, lane, qb, kst, vst, m_run, l_run, acc, sc.lds);
+    compute(s, vmask);
   }
+}
+
+// The same with the online softmax of up to 16 query heads over them, into m_run, l_run, acc.
+template <int D, int TYPE, bool HALVES, class FIND>
+__device__ __forceinline__ void paged_wave_loop(const PagedKv& c, const int32_t* table, int hk, int s, int s_end,
+                                                int step, int lane, float scale_log2, const bf16x8 (&qb)[D / 32],
+                                                char* wbuf, const FIND& find, float& m_run, float& l_run,
+                                                f32x4 (&acc)[D / 16], const PagedScales& sc = PagedScales{}) {
+  constexpr bool SCALED = TYPE >= kE4m3Blocks;
+  paged_wave_tiles<D, TYPE, HALVES>(
+      c, table, hk, s, s_end, step, lane, wbuf, find, sc, [](int, PagedRows<D, TYPE, HALVES>&) {},
+      [&](int, uint32_t vmask) {
+        paged_tile<D, TYPE == kBf16Cache, SCALED>(vmask, scale_log2, lane, qb, wbuf, wbuf + DenseCfg<D>::VT, m_run, l_run,
+                                                  acc, sc.lds);
+      });
 }
 
 // Merge of the workgroup's waves through LDS, in wave order: put(h, d4, A, M, L)

@@ -20,94 +20,11 @@
 // result's rounding; a second bf16 part would make three products of two); its sum stays in fp32.
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
-#include "paged.h"
+#include "paged_prompt.h"
 
 namespace bytes_amd {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-
 constexpr int kKeys = 64;            // of a tile
-constexpr float kSlack = 8.f;        // log2 of how far weights may pass 1
-
-struct PromptArgs {
-  PagedKv c;
-  const uint16_t* q;
-  int64_t q_st, q_sh;
-  uint16_t* out;
-  int64_t o_st, o_sh;
-  const int32_t* cu;                 // [B + 1]
-  const float *ks, *vs;              // [num_blocks, Hk], or null
-  int64_t ks_sb, ks_sh, vs_sb, vs_sh;
-  float* part_acc;                   // [unit][split][row][D]
-  float* part_ml;                    // [unit][split][row][2]
-  int T, B, Hk, G, D;
-  int cap, window, sinks;            // no window: 2^30
-  int nsplit, tiles;                 // parts of a unit's keys; row tiles at most
-  int flip;                          // the scale is negative: queries change sign
-  int once;                          // a cache row is read by about one workgroup
-  float scale_log2, v_scale;
-  FastDiv dHk, dG, dsplit;
-};
-
-// Row tile number r of the batch: rows r0 .. of sequence b, whose new tokens are rows
-// t0 .. t0 + n - 1 of q (b = B: the rows past the last sequence).  False past the last.
-struct RowTile {
-  int b, t0, n, r0;
-};
-template <int ROWS>
-__device__ __forceinline__ bool find_tile(const PromptArgs& a, int r, int lane, RowTile& x) {
-  for (int b0 = 0; b0 <= a.B; b0 += 64) {
-    const int b = b0 + lane, bc = min(b, a.B);
-    const int c0 = min(max(a.cu[bc], 0), a.T), c1 = b < a.B ? min(max(a.cu[bc + 1], 0), a.T) : a.T;
-    const int n = b <= a.B ? max(c1 - c0, 0) : 0;
-    const uint32_t mine = (uint32_t)((n * a.G + ROWS - 1) / ROWS);
-    const uint32_t incl = wave_prefix_sum(mine);
-    const int total = __builtin_amdgcn_readlane((int)incl, 63);
-    if (r < total) {
-      const int l = __ffsll((unsigned long long)__ballot((int)incl > r)) - 1;
-      x.b = b0 + l;
-      x.t0 = __builtin_amdgcn_readlane(c0, l);
-      x.n = __builtin_amdgcn_readlane(n, l);
-      x.r0 = (r - __builtin_amdgcn_readlane((int)(incl - mine), l)) * ROWS;
-      return true;
-    }
-    r -= total;
-  }
-  return false;
-}
-
-// The first n of 64 bits.
-__device__ __forceinline__ uint64_t low_bits(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; }
-
-// Eight bf16 numbers with infinities and NaN made 0; odd: whether there were any.
-__device__ __forceinline__ u32x4 finite_only(const u32x4& x, bool& odd) {
-  u32x4 r;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const bool lo = (x[j] & 0x7F80u) == 0x7F80u, hi = (x[j] & 0x7F800000u) == 0x7F800000u;
-    r[j] = x[j] & ((lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u));
-    odd = odd | lo | hi;
-  }
-  return r;
-}
-
-__device__ __forceinline__ float half_max(float v) {   // of a lane and its partner lane ^ 32
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ __forceinline__ float half_sum(float v) {
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
-// Four consecutive results; zeros where nothing was seen.
-__device__ __forceinline__ void store_bf16x4(uint16_t* out, const f32x16& x, int at, float by) {
-  typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-  bf16x4 r;
-#pragma unroll
-  for (int u = 0; u < 4; ++u) r[u] = (__bf16)(by == 0.f ? 0.f : x[at + u] * by);
-  *reinterpret_cast<u32x2*>(out) = __builtin_bit_cast(u32x2, r);
-}
 
 // NW waves of 32 rows.
 template <int D, int TYPE, bool HALVES, int NW>
@@ -143,7 +60,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && D == 128 && TYPE == kBf16Cache 
   }
   // (what all lanes share goes to scalar registers)
   auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const int p0 = same(a.c.lens[x.b] - x.n);        // the first new token's position
+  const int p0 = same(x.len - x.n);                // the first new token's position
   const int p = p0 + i;
   const bool placed = exists && p >= 0 && p < a.cap;
   const int first = fast_div(x.r0, a.dG), last = min(fast_div(x.r0 + NW * 32 - 1, a.dG), x.n - 1);
@@ -519,17 +436,12 @@ __global__ __launch_bounds__(64) void paged_prompt_join_kernel(PromptArgs a) {
   }
 }
 
-// How a call is cut up.
-struct PromptPlan {
-  int waves, nsplit;                 // of a workgroup; parts of a unit's keys
-  int64_t tiles, units;              // row tiles, and (row tile, KV head) pairs, at most
-  int rows() const { return waves * 32; }
-  size_t workspace(int D) const { return nsplit < 2 ? 0 : (size_t)units * nsplit * rows() * (D + 2) * 4; }
-};
 // cap: positions that a table row holds.
-static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int64_t cap, int window, int sinks) {
+static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int D, int64_t cap, int window, int sinks) {
   const int64_t cus = device_cu_count();
   PromptPlan p;
+  p.nwg = 0, p.nsplit = 1;
+  int64_t slots;                                   // that a row tile can see
   // whole row tiles, and one that is not full per sequence (and of the rows past the
   // last); none without rows
   auto cut = [&](int waves) {
@@ -537,13 +449,33 @@ static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int64
     const int64_t n = T * G / p.rows() + B + 1, most = T * ((G + p.rows() - 1) / p.rows());
     p.tiles = n < most ? n : most;
     p.units = p.tiles * Hk;
+    const int64_t see = (int64_t)window + sinks + row_span(p.rows(), G) + 2 * kKeys;
+    slots = cap < see ? cap : see;
   };
+  cut(1);
+  // Up to 32 rows of a sequence read its cache once as one tile (eight sequences of 22K to 64K,
+  // 8 KV heads of 128, 24 rows: 248 us, 289 in tiles of 128; 33 rows, two tiles: 472 and 348).
+  // Where contexts are short, and as many tiles of 32 rows as the CUs hold at once, they take
+  // fewer steps one after another (one prompt, 32 heads over 8 of 128, 500 tokens: 18.6 and 21.6 us,
+  // 300 after 1200 32.8 and 38.4, 300 after 2700 57.9 and 44.6; 14 heads over 2 of 64,
+  // 1500 tokens 19.9 and 36.5).
+  const bool lone = T * G <= 32 * B, fits = T * G * Hk / 32 <= cus * (D == 64 ? 4 : 2) && slots <= 2048;
+  if (lone || fits) {
+    // Dealt by the bytes of what a tile sees, which one workgroup reads alone: over 128 KB (one
+    // sequence, 8 heads of 128, 256 tokens: whole units 11.4 us, dealt 12.4; 512 tokens 14.7 and
+    // 12.3), over 512 KB where the units keep half the CUs busy anyway (16 sequences, 1000 tokens:
+    // 22.5 and 24.0; 2000: 38.3 and 36.9), over 2 MB where there are enough for all (60 sequences
+    // of 1200 to 2400 tokens: 81 and 91; 30 of 800 to 8000: 118 and 105).
+    const int64_t granules = p.units * ((slots + 127) / 128), bytes = slots * D * 4;
+    const int64_t alone = p.units >= cus ? 2 << 20 : 2 * p.units >= cus ? 512 << 10 : 128 << 10;
+    if (lone && bytes > alone && granules <= 1 << 24) p.nwg = few_grid(granules);
+    return p;
+  }
   cut(8);
   if (p.units < cus) cut(4);
-  // parts: enough that two workgroups come to each CU, none of fewer than 8 key tiles of
-  // the slots that a row can see
-  const int64_t see = (int64_t)window + sinks + p.rows() + 2 * kKeys, slots = cap < see ? cap : see;
-  const int64_t want = p.units < cus ? (2 * cus + p.units - 1) / (p.units < 1 ? 1 : p.units) : 1, most = slots / (8 * kKeys);
+  if (p.units >= cus) return p;
+  // parts: enough that two workgroups come to each CU, none of fewer than 8 key tiles
+  const int64_t want = (2 * cus + p.units - 1) / (p.units < 1 ? 1 : p.units), most = slots / (8 * kKeys);
   const int64_t n = want < most ? want : most;
   p.nsplit = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
   return p;
@@ -584,7 +516,7 @@ int bytes_paged_prompt_workspace_size(int T, int B, int Hq, int Hk, int D, int b
     *bytes = 0;
     return 0;
   }
-  *bytes = prompt_plan(T, B, Hk, Hq / Hk, (int64_t)max_blocks * block_size, window, sinks).workspace(D);
+  *bytes = prompt_plan(T, B, Hk, Hq / Hk, D, (int64_t)max_blocks * block_size, window, sinks).workspace(D);
   return 0;
 }
 
@@ -603,14 +535,14 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   if (rc0) return rc0;
   if (T == 0) return 0;
   const int64_t G = Hq / Hk;
-  const PromptPlan plan = prompt_plan(T, B, Hk, G, (int64_t)max_blocks * block_size, window, sinks);
+  const PromptPlan plan = prompt_plan(T, B, Hk, G, D, (int64_t)max_blocks * block_size, window, sinks);
   PromptArgs a = {};
   a.window = window < (1 << 30) ? window : (1 << 30), a.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
   a.nsplit = plan.nsplit;
   if ((int64_t)T * G + plan.rows() > 0x7FFFFFFF || plan.units * plan.nsplit > 0x7FFFFFFF || T > (1 << 30) ||
       (int64_t)Hq * (D / 64) > 65535)
     return (int)hipErrorInvalidConfiguration;
-  if (plan.nsplit > 1 && (!workspace || workspace_bytes < plan.workspace(D))) return (int)hipErrorInvalidValue;
+  if (plan.workspace(D) && (!workspace || workspace_bytes < plan.workspace(D))) return (int)hipErrorInvalidValue;
   a.c.k = k_paged, a.c.k_sb = k_sb, a.c.k_sh = k_sh, a.c.k_ss = k_ss;
   a.c.v = v_paged, a.c.v_sb = v_sb, a.c.v_sh = v_sh, a.c.v_ss = v_ss;
   a.c.table = static_cast<const int32_t*>(block_table), a.c.bt_sb = bt_sb;
@@ -623,7 +555,8 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   a.ks = static_cast<const float*>(k_scales), a.ks_sb = ks_sb, a.ks_sh = ks_sh;
   a.vs = static_cast<const float*>(v_scales), a.vs_sb = vs_sb, a.vs_sh = vs_sh;
   a.part_ml = static_cast<float*>(workspace);
-  a.part_acc = a.part_ml + (size_t)plan.units * plan.nsplit * plan.rows() * 2;
+  a.part_acc = a.part_ml + (plan.nwg ? (size_t)plan.nwg * 2 : (size_t)plan.units * plan.nsplit) * plan.rows() * 2;
+  a.nwg = plan.nwg, a.span = (int)row_span(32, G);
   a.T = T, a.B = B, a.Hk = Hk, a.G = (int)G, a.D = D;
   a.cap = max_blocks * block_size;
   a.tiles = (int)plan.tiles;
@@ -632,7 +565,9 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   // (at least the smallest normal number: times -inf, a masked score, it is -inf)
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f), a.v_scale = v_scale;
   a.dHk = make_fastdiv((uint32_t)Hk), a.dG = make_fastdiv((uint32_t)G), a.dsplit = make_fastdiv((uint32_t)a.nsplit);
+  a.dnwg = make_fastdiv((uint32_t)(a.nwg ? a.nwg : 1));
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (plan.waves == 1) return launch_prompt_few(a, kv_type, plan, st);
   switch (kv_type) {
     case kBf16Cache: return launch_prompt_of<kBf16Cache>(a, D, plan, st);
     case kFp8Cache: return launch_prompt_of<kFp8Cache>(a, D, plan, st);

@@ -45,6 +45,11 @@ def _run(dev, q, kc, vc, ks, vs, table, n, cu, scale, **kw):
                                 k_scale=_dev(ks, dev), v_scale=_dev(vs, dev), **kw)
 
 
+def _wide(table, bs):
+    """The table with entries for 2200 tokens more: what a row may see decides how a call is cut up."""
+    return torch.cat([table, table.new_full((table.shape[0], 2200 // bs + 1), -1)], 1)
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("Hq,Hk,D", [(14, 2, 64), (28, 4, 128), (5, 5, 64), (40, 1, 128)])
 @pytest.mark.parametrize("bs,layout", [(16, "nhsd"), (64, "nshd"), (1, "nhsd"), (24, "pair"), (48, "nhsd"), (200, "nhsd")])
@@ -58,6 +63,23 @@ def test_prompts(dev, kind, Hq, Hk, D, bs, layout):
         out = _run(dev, q, kc, vc, ks, vs, table, n, cu, D ** -0.5)
         assert out.shape == q.shape and out.dtype == BF16
         _check(out, q, kc, vc, D ** -0.5, ks, vs, table, n, cu)
+        out = _run(dev, q, kc, vc, ks, vs, _wide(table, bs), n, cu, D ** -0.5)
+        _check(out, q, kc, vc, D ** -0.5, ks, vs, table, n, cu)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("Hq,Hk,D,bs", [(160, 2, 64, 16), (160, 2, 64, 20), (256, 8, 64, 200), (80, 2, 128, 24), (256, 8, 128, 16)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 2), (65, 1), (40, 65), (130, 4)])
+def test_many_rows(dev, kind, Hq, Hk, D, bs, window, sinks):
+    """Rows enough for tiles of 128 and of 256 that no one shares."""
+    g = torch.Generator().manual_seed(Hq + bs)
+    lens, new = [300, 90, 257, 40], [210, 90, 3, 1]
+    q, kc, vc, ks, vs, table, n, cu = _batch(g, lens, new, bs, Hq, Hk, D, kind, extra=2)
+    kw = dict(window=window, sinks=sinks) if window else {}
+    print(f"many rows {kind} Hq{Hq} D{D} bs{bs} {kw}", flush=True)
+    out = _run(dev, q, kc, vc, ks, vs, table, n, cu, D ** -0.5, **kw)
+    rows = list(range(0, q.shape[0], 11)) + list(range(207, 212)) + list(range(298, q.shape[0]))
+    _check(out, q, kc, vc, D ** -0.5, ks, vs, table, n, cu, window, sinks, rows)
 
 
 @pytest.mark.parametrize("kind", ["bf16", I8])
@@ -114,7 +136,8 @@ def test_long_prompt_rows(dev):
 
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("bs", [16, 20])
-def test_holes_garbage_and_lengths(dev, kind, bs):
+@pytest.mark.parametrize("wide", [False, True])
+def test_holes_garbage_and_lengths(dev, kind, bs, wide):
     """Blocks that are gone or do not exist, sequences without any, lengths past the table and below
     their new tokens; NaN and infinities in every row that no sequence holds."""
     g = torch.Generator().manual_seed(bs)
@@ -124,6 +147,8 @@ def test_holes_garbage_and_lengths(dev, kind, bs):
     table[0, 1], table[1, 3], table[1, 4] = -1, kc.shape[0], 2 ** 31 - 1
     table[2] = -1
     table[3, 0] = -2 ** 31
+    if wide:
+        table = _wide(table, bs)
     n[4] = table.shape[1] * bs + 30                  # the last 30 have no position
     held = torch.zeros(kc.shape[0], bs, dtype=torch.bool)
     for b in range(6):
@@ -153,14 +178,15 @@ def test_holes_garbage_and_lengths(dev, kind, bs):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8", F8])
-@pytest.mark.parametrize("D,split", [(64, False), (128, False), (128, True)])
-def test_infinite_and_nan_values_reach_the_rows_that_see_them(dev, kind, D, split):
+@pytest.mark.parametrize("D,split,Hq,Hk", [(64, False, 4, 2), (128, False, 4, 2), (128, True, 4, 2), (128, True, 12, 2),
+                                           (64, False, 256, 2), (128, False, 448, 8)])
+def test_infinite_and_nan_values_reach_the_rows_that_see_them(dev, kind, D, split, Hq, Hk):
     """Values and keys that are infinite or NaN, in tiles that some rows see and others do not."""
     g = torch.Generator().manual_seed(D)
-    Hq, Hk, bs = 4, 2, 16
-    L, m = (6000, 20) if split else (150, 150)
+    bs = 16
+    L, m = (6000, 15 if Hq == 4 else 20) if split else (150, 150)
     q, kc, vc, ks, vs, table, n, cu = _batch(g, [L], [m], bs, Hq, Hk, D, kind)
-    bad = {L - m + 5: 3, L - m + 13: 40, L - 1: 63}   # position: dim
+    bad = {L - m + 5: 3, L - m + 12: 40, L - 1: 63}   # position: dim
     at = lambda p: (int(table[0, p // bs]), p % bs)                          # noqa: E731
     f = vc.float()
     for i, (p, d) in enumerate(bad.items()):
@@ -168,7 +194,7 @@ def test_infinite_and_nan_values_reach_the_rows_that_see_them(dev, kind, D, spli
     dirty = f.to(vc.dtype)
     for kw in ({}, dict(window=9, sinks=2)):
         out = _run(dev, q, kc, dirty, ks, vs, table, n, cu, 0.1, **kw).double().cpu()
-        rows = list(range(m)) if not split else list(range(0, m, 3)) + [m - 1]
+        rows = list(range(0, m, 3 if split or Hq > 4 else 1)) + [m - 1]
         pos = S.positions(m, table, n, cu, bs)
         w, s = kw.get("window"), kw.get("sinks", 0)
         want, mag, dots = S.attend_rows(q[rows], [pos[r] for r in rows], kc, vc, 0.1, ks, vs, table, n, w, s)
@@ -201,8 +227,24 @@ def test_large_scores(dev):
             for p in range(L):                       # keys that grow: the maximum moves on
                 kc[int(table[0, p // bs]), :, p % bs] *= 0.05 * p ** 0.5
         for scale in (1.0, -0.7, 0.0, 1e-30, 8.0):
-            out = _run(dev, q, kc, vc, ks, vs, table, n, cu, scale)
-            _check(out, q, kc, vc, scale, ks, vs, table, n, cu, rows=list(range(0, L, 7)) + [L - 1])
+            for t in (table, _wide(table, bs)):
+                out = _run(dev, q, kc, vc, ks, vs, t, n, cu, scale)
+                _check(out, q, kc, vc, scale, ks, vs, table, n, cu, rows=list(range(0, L, 7)) + [L - 1])
+
+
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("cu", [[0, 40, 10, 64, 64], [5, 5, 9, 64, 70], [-3, 20, 2 ** 31 - 1, -2 ** 31, 30], [64, 64, 64, 64, 64],
+                                [0, 10 ** 6, 0, 10 ** 6, 0]])
+def test_offsets_that_are_no_offsets(dev, cu, wide):
+    """Offsets that descend, overlap or leave the rows: results that nobody reads, and the next call is right."""
+    g = torch.Generator().manual_seed(6)
+    lens = [100, 6000 if wide else 90, 64, 300]
+    q, kc, vc, ks, vs, table, n, good = _batch(g, lens, [20, 4, 30, 10], 16, 8, 2, 64, "bf16")
+    args = [x.to(dev) for x in (q, kc, vc, table, n)]
+    print(f"offsets {cu} {wide}", flush=True)
+    PG.paged_prompt_attn(*args, torch.tensor(cu, dtype=I32, device=dev), 0.125)
+    torch.cuda.synchronize()
+    _check(PG.paged_prompt_attn(*args, good.to(dev), 0.125), q, kc, vc, 0.125, ks, vs, table, n, good)
 
 
 def test_strided_queries_and_shared_blocks(dev):
