@@ -24,7 +24,6 @@ struct PromptArgs {
   int cap, window, sinks;            // no window: 2^30
   int nsplit, tiles;                 // parts of a unit's keys; row tiles at most
   int flip;                          // the scale is negative: queries change sign
-  int once;                          // a cache row is read by about one workgroup
   int nwg, span;                     // few rows: workgroups among which keys are dealt, or 0; tokens that 32 rows reach over, at most
   float scale_log2, v_scale;
   FastDiv dHk, dG, dsplit, dnwg;

@@ -20,6 +20,20 @@
 // result's rounding; a second bf16 part would make three products of two); its sum stays in fp32.
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
+//
+// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2140
+// us, 1030 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
+// nothing loaded or stored, 2060; the clock falls to 1.9 GHz and the matrix units are busy for 46% of
+// it.  Left out one at a time (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
+// 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No
+// faster: products of one tile among the softmax of the other in one wave 2330, 64 rows per wave 3840
+// (registers), raised wave priority, dot products for the sums, one tile more on its way.  Over e4m3 with
+// scales 2290 (over e4m3 with one scale 2120): 64 multiplications more per lane and tile; folding the
+// keys' into the exponent's multiply-add takes 3% longer.
+//
+// A workgroup has 256 rows, eight waves, one to a CU, where that makes units for all CUs, and else
+// 128, two to a CU: 16K prompt 2210 and 2290, last 4096 of 16K 953 and 1028, a 4096 prompt 158 and 175;
+// 4 x 1024 after 476, which is two rounds of the larger tiles, 108 and 99.
 #include "paged_prompt.h"
 
 namespace bytes_amd {
@@ -139,13 +153,8 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && D == 128 && TYPE == kBf16Cache 
         const Elem *kp = kb + at(ka, base & ~15), *vp = vb + at(va, base & ~15);
         if constexpr (DMA) {
           char* to_k = smem[to] + base * (D * 2);
-          if (a.once) {
-            lds_dma16<true>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
-            lds_dma16<true>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
-          } else {
-            lds_dma16<false>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
-            lds_dma16<false>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
-          }
+          lds_dma16<false>(buf_rsrc(kp, 0xFFFFFFFFu), to_k, 2 * ko);
+          lds_dma16<false>(buf_rsrc(vp, 0xFFFFFFFFu), to_k + VT, 2 * vo);
         } else {
           kr[u] = ld16(kp + ko);
           vr[u] = ld16(vp + vo);
@@ -561,7 +570,6 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   a.cap = max_blocks * block_size;
   a.tiles = (int)plan.tiles;
   a.flip = scale < 0.f ? 1 : 0;
-  a.once = T * G <= (int64_t)B * plan.rows() ? 1 : 0;
   // (at least the smallest normal number: times -inf, a masked score, it is -inf)
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f), a.v_scale = v_scale;
   a.dHk = make_fastdiv((uint32_t)Hk), a.dG = make_fastdiv((uint32_t)G), a.dsplit = make_fastdiv((uint32_t)a.nsplit);

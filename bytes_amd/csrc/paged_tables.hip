@@ -46,7 +46,11 @@ constexpr int kPlanWaves = 8, kPlanThreads = kPlanWaves * 64;
 constexpr int kFillThreads = 256;
 constexpr int kBySelf = 4;           // places that a thread counts alone
 constexpr int kCuLds = 4096;         // sequences whose cu fits the fill's LDS
-constexpr int kSmallB = 128, kSmallT = 1024;   // a step that one workgroup takes in one launch
+// A step that one workgroup takes in one launch (us, eager, one launch and two: 32 sequences and
+// 32 rows of tokens 6.1 and 9.4, 1024 rows 6.5 and 9.4; 64 and 1024: 8.7 and 9.2; 128 and 128: 7.4 and
+// 9.2; 128 and 1024: 10.4 and 9.2).
+constexpr int kSmallB = 128;
+constexpr bool small_step(int B, int T) { return B <= kSmallB && T <= 1536 - 8 * B; }
 
 __device__ __forceinline__ bool names(int id, int N) { return id >= 0 && id < N; }
 __device__ __forceinline__ int places(const TablesArgs& a, int n) { return fast_div(n + a.bs - 1, a.dbs); }
@@ -347,7 +351,7 @@ int bytes_paged_resize(void* block_table, int64_t bt_sb, void* context_lens, voi
   a.window = window < (1 << 30) ? window : (1 << 30), a.sinks = sinks;
   a.dbs = make_fastdiv((uint32_t)block_size);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (B <= kSmallB && T <= kSmallT) {
+  if (small_step(B, T)) {
     hipLaunchKernelGGL(paged_tables_small_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
     return (int)hipGetLastError();
   }
