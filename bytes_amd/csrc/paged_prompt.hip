@@ -21,19 +21,19 @@
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
 //
-// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2140
-// us, 1030 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
+// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2080
+// us, 1060 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
 // nothing loaded or stored, 2060; the clock falls to 1.9 GHz and the matrix units are busy for 46% of
-// it.  Left out one at a time (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
+// it.  Left out one at a time, of 2240 then (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
 // 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No
 // faster: products of one tile among the softmax of the other in one wave 2330, 64 rows per wave 3840
 // (registers), raised wave priority, dot products for the sums, one tile more on its way.  Over e4m3 with
-// scales 2290 (over e4m3 with one scale 2120): 64 multiplications more per lane and tile; folding the
+// scales 2260 (over e4m3 with one scale 2090): 64 multiplications more per lane and tile; folding the
 // keys' into the exponent's multiply-add takes 3% longer.
 //
 // A workgroup has 256 rows, eight waves, one to a CU, where that makes units for all CUs, and else
-// 128, two to a CU: 16K prompt 2210 and 2290, last 4096 of 16K 953 and 1028, a 4096 prompt 158 and 175;
-// 4 x 1024 after 476, which is two rounds of the larger tiles, 108 and 99.
+// 128, two to a CU: 16K prompt 2050 and 2090, last 4096 of 16K 889 and 944, a 4096 prompt 147 and 161;
+// 4 x 1024 after 476 each, which is two rounds of the larger tiles, 98 and 93.
 #include "paged_prompt.h"
 
 namespace bytes_amd {
@@ -462,8 +462,9 @@ static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int D
     slots = cap < see ? cap : see;
   };
   cut(1);
-  // Up to 32 rows of a sequence read its cache once as one tile (eight sequences of 22K to 64K,
+  // Up to 32 rows of a sequence read its cache once as one tile (eight sequences of 27K to 64K,
   // 8 KV heads of 128, 24 rows: 248 us, 289 in tiles of 128; 33 rows, two tiles: 472 and 348).
+  // (Rows that are read once stream past the caches: with plain loads 276 and not 248.)
   // Where contexts are short, and as many tiles of 32 rows as the CUs hold at once, they take
   // fewer steps one after another (one prompt, 32 heads over 8 of 128, 500 tokens: 18.6 and 21.6 us,
   // 300 after 1200 32.8 and 38.4, 300 after 2700 57.9 and 44.6; 14 heads over 2 of 64,

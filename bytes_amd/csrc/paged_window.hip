@@ -14,9 +14,9 @@
 // keys' multiply the fp32 scores, the values' the fp32 weights before these are split
 // into bf16 parts, so codes enter the products exactly.
 //
-// Bound by memory: 29 sequences of 5.7K to 16K, 64 heads over 8 of 128, e4m3 with scales
+// Bound by memory: 29 sequences of 6.6K to 16K, 64 heads over 8 of 128, e4m3 with scales
 // (685 MB) take 121 us, 5.7 TB/s (one scale for the tensor 116; without any arithmetic, not an answer,
-// 115), where streaming reads reach 7.1; a window of 4096 and 4 sinks in 16 sequences of 11K to 32K, 8
+// 115), where streaming reads reach 7.1; a window of 4096 and 4 sinks in 16 sequences of 12K to 32K, 8
 // heads of 128 in bf16 (269 MB), 50 us, 5.4 TB/s with its join of 4.6.
 #include "paged_split.h"
 
