@@ -223,8 +223,8 @@ __device__ __forceinline__ void make_plan(const TablesArgs& a, PlanShared& sh, i
 }
 
 __device__ __forceinline__ int ring_at(const TablesArgs& a, int head, int64_t i) {
-  const int64_t x = head + i;                      // below 2 N in a pool that is one
-  return (int)(x < a.N ? x : x < 2 * (int64_t)a.N ? x - a.N : x % a.N);
+  const uint64_t x = (uint64_t)(head + i), N = (uint64_t)a.N;      // below 2 N in a pool that is one
+  return (int)(x < N ? x : x < 2 * N ? x - N : x % N);
 }
 
 // One wave: the blocks of sequence b that go back and come.

@@ -216,6 +216,34 @@ def test_infinite_and_nan_values_reach_the_rows_that_see_them(dev, kind, D, spli
     assert bool(out[7:11].isnan().all()) and not bool(out[:7].isnan().any()) and not bool(out[11:].isnan().any())
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("bs", [16, 20])
+def test_drafts_over_holes_and_garbage(dev, kind, bs):
+    """Few rows over long tables, which are dealt out: blocks that are gone, sequences without any or without new
+    tokens, lengths past the table and below zero, rows past the last sequence; the same twice and on a graph."""
+    g = torch.Generator().manual_seed(bs + 5)
+    Hq, Hk, D = 8, 2, 64
+    lens, new = [5000, 333, 90, 12, 2640, 7, 3000, 1], [6, 8, 5, 0, 7, 9, 2, 1]
+    q, kc, vc, ks, vs, table, n, cu = _batch(g, lens, new, bs, Hq, Hk, D, kind, extra=4)
+    table[0, 3:70], table[0, 100], table[1, 4] = -1, kc.shape[0], 2 ** 31 - 1
+    table[2] = -1
+    n[4] = table.shape[1] * bs + 3                   # its last 3 have no position
+    n[6] = -5
+    args = [_dev(x, dev) for x in (q, kc, vc, ks, vs, table, n, cu)]
+    for kw in ({}, dict(window=1500, sinks=40), dict(window=2, sinks=0)):
+        call = lambda: _run(dev, *args, 0.1, **kw)   # noqa: E731
+        out = call()
+        assert not bool(out[cu[-1]:].any()) and not bool(out[cu[2]:cu[3]].any()) and not bool(out[cu[6]:cu[7]].any())
+        assert not bool(out[cu[5] - 3:cu[5]].any()) and not bool(out[cu[5]:cu[5] + 2].any())
+        _check(out, q, kc, vc, 0.1, ks, vs, table, n, cu, kw.get("window"), kw.get("sinks", 0))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            again = call()
+        for _ in range(2):
+            graph.replay()
+            assert torch.equal(again, call()) and torch.equal(again, out)
+
+
 def test_large_scores(dev):
     """Scores far apart, running maxima that move in every tile and by little, scales that are negative, zero,
     large."""
