@@ -21,8 +21,8 @@
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
 //
-// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2080
-// us, 1060 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
+// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2080 to 2160
+// us by card, 1020 to 1060 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
 // nothing loaded or stored, 2060; the clock falls to 1.9 GHz and the matrix units are busy for 46% of
 // it.  Left out one at a time, of 2240 then (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
 // 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No
@@ -33,7 +33,8 @@
 //
 // A workgroup has 256 rows, eight waves, one to a CU, where that makes units for all CUs, and else
 // 128, two to a CU: 16K prompt 2050 and 2090, last 4096 of 16K 889 and 944, a 4096 prompt 147 and 161;
-// 4 x 1024 after 476 each, which is two rounds of the larger tiles, 98 and 93.
+// 4 x 1024 after 476 each, which is two rounds of the larger tiles, 98 and 93 (when a batch's
+// tiles started in the order of its sequences; see find_tile_by_keys).
 #include "paged_prompt.h"
 
 namespace bytes_amd {
@@ -61,7 +62,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && D == 128 && TYPE == kBf16Cache 
   const int tile = a.tiles - 1 - (int)blockIdx.x / per;              // the last rows, which see most, first
   const int rest = (int)blockIdx.x % per, split = fast_div(rest, a.dHk), hk = rest - split * a.Hk;
   RowTile x;
-  if (!find_tile<NW * 32>(a, tile, lane, x)) return;
+  if (a.by_keys) {
+    if (!find_tile_by_keys<NW * 32>(a, a.tiles - 1 - tile, lane, x)) return;
+  } else if (!find_tile<NW * 32>(a, tile, lane, x)) return;
   const int row = x.r0 + w * 32 + l32, rows = x.n * a.G;
   const bool exists = row < rows;
   const int i = fast_div(exists ? row : 0, a.dG), h = hk * a.G + (exists ? row : 0) - i * a.G;
@@ -566,6 +569,7 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   a.vs = static_cast<const float*>(v_scales), a.vs_sb = vs_sb, a.vs_sh = vs_sh;
   a.part_ml = static_cast<float*>(workspace);
   a.part_acc = a.part_ml + (plan.nwg ? (size_t)plan.nwg * 2 : (size_t)plan.units * plan.nsplit) * plan.rows() * 2;
+  a.by_keys = B > 1 && B < 64 && plan.nsplit == 1;
   a.nwg = plan.nwg, a.span = (int)row_span(32, G);
   a.T = T, a.B = B, a.Hk = Hk, a.G = (int)G, a.D = D;
   a.cap = max_blocks * block_size;
