@@ -36,7 +36,7 @@ int bytes_paged_decode_workspace_size(int B, int Hq, int Hk, int D, int kv_fp8, 
   if (rc) return rc;
   const int64_t cap = (int64_t)max_blocks * block_size;
   const DecodeShape s = decode_shape(B, Hq, Hk, cap);
-  *bytes = short_waves(s.units, cap, D, kv_fp8) ? 0 : decode_workspace(decode_grid(s.units, s.granules), D);
+  *bytes = short_waves(s.units, cap, D, PagedDecodeArgs::dim_cost(kv_fp8)) ? 0 : decode_workspace(decode_grid(s.units, s.granules), D);
   return 0;
 }
 
@@ -57,7 +57,7 @@ int bytes_paged_decode_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
   decode_args(a, q, q_sb, q_sh, k_paged, k_sb, k_sh, k_ss, v_paged, v_sb, v_sh, v_ss, block_table, bt_sb, context_lens,
               out, o_sb, o_sh, B, Hq, Hk, block_size, num_blocks, max_blocks, shape, workspace);
   a.scale_log2 = scale * kLog2e, a.v_scale = v_scale;
-  if (!short_waves(shape.units, cap, D, kv_fp8) && (!workspace || workspace_bytes < decode_workspace(a.nwg, D)))
+  if (!short_waves(shape.units, cap, D, PagedDecodeArgs::dim_cost(kv_fp8)) && (!workspace || workspace_bytes < decode_workspace(a.nwg, D)))
     return (int)hipErrorInvalidValue;
   hipStream_t st = static_cast<hipStream_t>(stream);
   return kv_fp8 ? launch_decode_of<PagedDecodeArgs, kFp8Cache>(a, D, shape, cap, st)

@@ -35,6 +35,8 @@ struct PagedDecodeArgs {
   __device__ __forceinline__ View view(int) const { return View{c.dbs}; }
   __device__ __forceinline__ int slots(int n) const { return n; }
   __device__ __forceinline__ PagedScales scales(int, float*) const { return PagedScales{}; }
+  // What a token's dim counts in the choice of short_waves: the bytes of a key and a value.
+  static constexpr int dim_cost(int type) { return type == kBf16Cache ? 4 : 2; }
 };
 
 // Granules of a sequence of n tokens: an empty one has one too, whose output is written like any other.
@@ -217,8 +219,8 @@ static int decode_grid(int64_t units, int64_t granules_max) {
 // 10.7 and 13.3, 1000 tokens 17.2 and 20.8).  Four waves where a tile each
 // covers the row, or where two workgroups to a CU have units enough (200 sequences
 // of 4 heads, 100 tokens: 15.8 with eight, 9.1 with four; split 18.0).
-static int short_waves(int64_t units, int64_t cap, int D, int fp8) {
-  const int64_t cus = device_cu_count(), bytes = cap * D * (fp8 ? 2 : 4);
+static int short_waves(int64_t units, int64_t cap, int D, int dim_cost) {
+  const int64_t cus = device_cu_count(), bytes = cap * D * dim_cost;
   if (bytes > (2 * units >= cus ? 512 << 10 : 256 << 10)) return 0;
   return cap <= 4 * kTile || units >= 2 * cus ? 4 : 8;
 }
@@ -237,7 +239,7 @@ static size_t decode_workspace(int nwg, int D) { return (size_t)nwg * 2 * 16 * (
 // The kernels of arguments a, whose tables hold `cap` slots at most; 0 or a hipError_t.
 template <class ARGS, int D, int TYPE, bool HALVES>
 int launch_decode(const ARGS& a, const DecodeShape& shape, int64_t cap, hipStream_t st) {
-  const int waves = short_waves(shape.units, cap, D, TYPE != kBf16Cache);
+  const int waves = short_waves(shape.units, cap, D, ARGS::dim_cost(TYPE));
   if (waves) {
     const dim3 grid((unsigned)shape.units);
     if (waves == 4) hipLaunchKernelGGL((paged_decode_short_kernel<ARGS, D, TYPE, HALVES, 4>), grid, dim3(256), 0, st, a);

@@ -46,6 +46,11 @@ struct PagedWindowArgs : PagedDecodeArgs {
   __device__ __forceinline__ PagedScales scales(int hk, float* lds) const {
     return PagedScales{ks + hk * ks_sh, vs + hk * vs_sh, ks_sb, vs_sb, lds};
   }
+  // A tile of bytes takes as long as one of bf16 and more, read alone (int8, us from a graph, a workgroup per unit
+  // and the even split: one sequence of 2 KV heads of 64, 500 tokens 6.7, 750 8.4 and 7.9, 1000 9.8 and 7.8,
+  // 2000 16.3 and 7.9; of 4 heads of 128, 300 tokens 7.3 and 8.9, 500 8.8 and 8.9, 1000 13.5 and 8.9; 64
+  // sequences of 2 heads of 64, 1500 tokens 14.4 and 15.3, 2000 17.6 and 17.9).
+  static constexpr int dim_cost(int type) { return type == kBf16Cache ? 4 : 5; }
 };
 
 // Slots that a table row of `cap` tokens can give.
@@ -69,7 +74,7 @@ int bytes_paged_window_workspace_size(int B, int Hq, int Hk, int D, int kv_type,
   if (rc) return rc;
   const int64_t cap = window_slots((int64_t)max_blocks * block_size, window, sinks);
   const DecodeShape s = decode_shape(B, Hq, Hk, cap);
-  *bytes = short_waves(s.units, cap, D, kv_type != kBf16Cache) ? 0 : decode_workspace(decode_grid(s.units, s.granules), D);
+  *bytes = short_waves(s.units, cap, D, PagedWindowArgs::dim_cost(kv_type)) ? 0 : decode_workspace(decode_grid(s.units, s.granules), D);
   return 0;
 }
 
@@ -96,7 +101,7 @@ int bytes_paged_window_attn(const void* q, int64_t q_sb, int64_t q_sh, const voi
   a.ks = static_cast<const float*>(k_scales), a.ks_sb = ks_sb, a.ks_sh = ks_sh;
   a.vs = static_cast<const float*>(v_scales), a.vs_sb = vs_sb, a.vs_sh = vs_sh;
   a.scale_log2 = scale * kLog2e, a.v_scale = v_scale;
-  if (!short_waves(shape.units, cap, D, kv_type != kBf16Cache) &&
+  if (!short_waves(shape.units, cap, D, PagedWindowArgs::dim_cost(kv_type)) &&
       (!workspace || workspace_bytes < decode_workspace(a.nwg, D)))
     return (int)hipErrorInvalidValue;
   hipStream_t st = static_cast<hipStream_t>(stream);
