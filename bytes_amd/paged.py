@@ -49,17 +49,18 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-def _by_block(k_scale: Scale, v_scale: Scale) -> bool:
-    """Whether the scales are tensors, one for each block and KV head (one of one element
-    without two dims is a number)."""
-    a, b = (isinstance(s, torch.Tensor) and (s.dim() == 2 or s.numel() > 1) for s in (k_scale, v_scale))
+def _by_block(k_scale: Scale, v_scale: Scale, k_paged: torch.Tensor) -> bool:
+    """Whether the scales are tensors, one for each block and KV head.  A tensor of one element is a
+    number, unless it is [1, 1] and the cache has one block and head."""
+    one = k_paged.dim() == 4 and k_paged.shape[0] * k_paged.shape[1] == 1
+    a, b = (isinstance(s, torch.Tensor) and (s.numel() != 1 or (one and s.dim() == 2)) for s in (k_scale, v_scale))
     if a != b:
         raise ValueError("k_scale and v_scale are both numbers or both tensors [num_blocks, H_k]")
     return a
 
 
-def _tensors(k_scale: Scale, v_scale: Scale) -> list:
-    return [k_scale, v_scale] if _by_block(k_scale, v_scale) else []
+def _tensors(k_scale: Scale, v_scale: Scale, k_paged: torch.Tensor) -> list:
+    return [k_scale, v_scale] if _by_block(k_scale, v_scale, k_paged) else []
 
 
 def _block_scales(k_scale: torch.Tensor, v_scale: torch.Tensor, N: int, Hk: int) -> None:
@@ -82,7 +83,7 @@ def _window(window: Optional[int], sinks: int) -> Tuple[int, int]:
 
 def _typed_cache(k_paged, v_paged, k_scale: Scale, v_scale: Scale):
     """-> (num_blocks, H_k, block_size, D, cache type of the C ABI), for caches of every kind."""
-    if not _by_block(k_scale, v_scale):
+    if not _by_block(k_scale, v_scale, k_paged):
         N, Hk, bs, D, fp8 = _cache(k_paged, v_paged, k_scale, v_scale)
         return N, Hk, bs, D, int(fp8)
     N, Hk, bs, D, _ = _cache(k_paged, v_paged, 1.0, 1.0, (_F8, torch.int8))
@@ -219,7 +220,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
     Blocks that receive tokens must belong to one sequence each, and be named once
     in its table row (blocks of a shared prefix are only read).  The caches and
     min / max must be memory of their own, without expanded dims."""
-    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale):
+    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale, k_paged):
         out = None if meta is not None else native().paged_append_blocks(
             k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, bool(interleaved), k_scale, v_scale)
         if out is not None:
@@ -239,7 +240,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_paged: torch.Tensor, v_p
 
 def _append(k, v, k_paged, v_paged, block_table, context_lens, cu_seqlens, q, cos, sin, interleaved, meta, k_scale, v_scale):
     """paged_kv_append where the native path does not take the call."""
-    C.cuda_tensors(k, v, k_paged, v_paged, block_table, context_lens, *_tensors(k_scale, v_scale),
+    C.cuda_tensors(k, v, k_paged, v_paged, block_table, context_lens, *_tensors(k_scale, v_scale, k_paged),
                    *(t for t in (cu_seqlens, q, cos, sin, *(meta or ())) if t is not None))
     N, Hk, bs, D, typ = _typed_cache(k_paged, v_paged, k_scale, v_scale)
     C.ndim(k, 3, "k"), C.ndim(v, 3, "v")
@@ -327,7 +328,7 @@ def paged_decode_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     that takes part gives that infinity, unless its weight underflows fp32 (below
     2^-100 of the row's largest it may give NaN).  Returns [B,H_q,1,D] bf16."""
     if window is not None or sinks or (
-            not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale)):
+            not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale, k_paged)):
         return _window_attn(q, k_paged, v_paged, block_table, context_lens, scale, window, sinks, k_scale, v_scale)
     out = native().paged_decode(q, k_paged, v_paged, block_table, context_lens, scale, k_scale, v_scale)
     if out is not None:
@@ -355,7 +356,7 @@ def _window_attn(q, k_paged, v_paged, block_table, context_lens, scale, window, 
     if out is not None:
         return out
     C.cuda_tensors(q, k_paged, v_paged, block_table, context_lens,
-                   *_tensors(k_scale, v_scale))
+                   *_tensors(k_scale, v_scale, k_paged))
     N, Hk, bs, D, typ = _typed_cache(k_paged, v_paged, k_scale, v_scale)
     window, sinks = _window(window, sinks)
     qs, B, Hq = _query(q, Hk, D)
@@ -396,7 +397,7 @@ def paged_prompt_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     if out is not None:
         return out
     C.cuda_tensors(q, k_paged, v_paged, block_table, context_lens, cu_seqlens,
-                   *_tensors(k_scale, v_scale))
+                   *_tensors(k_scale, v_scale, k_paged))
     N, Hk, bs, D, typ = _typed_cache(k_paged, v_paged, k_scale, v_scale)
     window, sinks = _window(window, sinks)
     C.ndim(q, 3, "q")
@@ -479,7 +480,7 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     [B,H_q,1,D] bf16 (and the selected blocks' places in the table, int32
     [B,H_q,min(ceil(kb / block_size), max_blocks)] ascending, if return_pages;
     places past a short sequence's blocks stand for nothing)."""
-    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale):
+    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale, k_paged):
         raise ValueError("page-sparse decode takes caches with one scale for the tensor")
     if not return_pages:
         out = native().paged_quest(q, k_paged, v_paged, *meta, block_table, context_lens, kb, scaling, local_w, k_scale,

@@ -95,6 +95,11 @@ def test_types_scales_and_windows(calls):
     calls.clear()                                    # one scale in a tensor of one element is a number
     _decode(x, k_scale=torch.tensor(0.5), v_scale=torch.tensor([0.25]))
     assert calls[-1][0] == "bytes_paged_decode_attn" and calls[-1][1][-5:-3] == (0.0625, 0.25)
+    _decode(x, k_scale=torch.full((1, 1), 0.5), v_scale=0.25)
+    assert calls[-1][0] == "bytes_paged_decode_attn" and calls[-1][1][-5:-3] == (0.0625, 0.25)
+    x = _inputs(dtype=F8, Hk=1, N=1, W=1)            # a cache of one block and head has such a scale
+    _decode(x)
+    assert calls[-1][0] == "bytes_paged_window_attn" and calls[-1][1][11] == 2
 
 
 def _bad(name, **change):
