@@ -484,8 +484,10 @@ static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int D
     if (lone && bytes > alone && granules <= 1 << 24) p.nwg = few_grid(granules);
     return p;
   }
+  // (Sequences of hardly 256 rows leave most of such a tile empty: 63 single tokens and a chunk of 512,
+  // 8K to 16K of context, 962 us and 845; 31 and a chunk of 2048, 4K to 8K, 391 and 370.)
   cut(8);
-  if (p.units < cus) cut(4);
+  if (p.units < cus || T * G < 512 * B) cut(4);
   if (p.units >= cus) return p;
   // parts: enough that two workgroups come to each CU, none of fewer than 8 key tiles
   const int64_t want = (2 * cus + p.units - 1) / (p.units < 1 ? 1 : p.units), most = slots / (8 * kKeys);

@@ -389,7 +389,9 @@ def paged_prompt_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     t > p - window or t < sinks.  Caches, scales and `scale` as in paged_decode_attn.
     fp32 scores, softmax and sums; weights rounded to bf16 for the value product.
     An infinite or NaN value reaches the rows that see its token only; one that takes
-    part gives that infinity, unless its weight underflows (NaN then).  Rows without a
+    part gives that infinity, unless its weight underflows (NaN then).  (Sequences with a single
+    new token may be among them; many of those beside a chunk are faster as a call of
+    paged_decode_attn of their own.)  Rows without a
     position, without a token to see, and past cu_seqlens[B] get zeros.  Returns
     [T,H_q,D] bf16."""
     out = native().paged_prompt(q, k_paged, v_paged, block_table, context_lens, cu_seqlens, scale, window, sinks, k_scale,
