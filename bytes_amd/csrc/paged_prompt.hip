@@ -480,8 +480,12 @@ static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int D
     // 22.5 and 24.0; 2000: 38.3 and 36.9), over 2 MB where there are enough for all (60 sequences
     // of 1200 to 2400 tokens: 81 and 91; 30 of 800 to 8000: 118 and 105).
     const int64_t granules = p.units * ((slots + 127) / 128), bytes = slots * D * 4;
-    const int64_t alone = p.units >= cus ? 2 << 20 : 2 * p.units >= cus ? 512 << 10 : 128 << 10;
-    if (lone && bytes > alone && granules <= 1 << 24) p.nwg = few_grid(granules);
+    // Several tiles to a sequence: only where the units are few and see over 256 KB (25 tokens after 802, 8
+    // heads of 128: 19.9 and 13.6; 100 after 1900, 14 heads over 2 of 64: 21.9 and 15.2; but 100 after 900
+    // of 8 heads of 64, 256 KB: 14.2 and 16.3; 307 after 975, 28 heads over 4 of 128: 28.8 and 41.7).
+    const bool idle = 2 * p.units < cus;
+    const int64_t alone = lone ? (p.units >= cus ? 2 << 20 : idle ? 128 << 10 : 512 << 10) : 256 << 10;
+    if ((lone || idle) && bytes > alone && granules <= 1 << 24) p.nwg = few_grid(granules);
     return p;
   }
   // (Sequences of hardly 256 rows leave most of such a tile empty: 63 single tokens and a chunk of 512,

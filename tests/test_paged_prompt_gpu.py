@@ -98,7 +98,8 @@ def test_prompts_within_a_window(dev, kind, Hq, Hk, D, bs, window, sinks):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("B,Hq,Hk,D,L,new,bs,window", [
     (2, 24, 8, 128, 9000, 8, 16, None), (1, 14, 2, 64, 20000, 3, 32, None), (3, 8, 1, 128, 7000, 40, 20, None),
-    (1, 8, 2, 64, 12000, 5, 16, 6000), (70, 8, 2, 64, 1500, 2, 16, None)])
+    (1, 8, 2, 64, 12000, 5, 16, 6000), (70, 8, 2, 64, 1500, 2, 16, None), (1, 24, 8, 128, 972, 12, 16, None),
+    (2, 14, 2, 64, 1468, 40, 20, None), (2, 14, 2, 64, 1800, 60, 32, 1500)])
 def test_few_rows_over_long_contexts(dev, kind, B, Hq, Hk, D, L, new, bs, window):
     """Draft tokens: the keys of a row are shared out and joined."""
     g = torch.Generator().manual_seed(L)
