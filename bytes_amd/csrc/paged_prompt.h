@@ -35,9 +35,11 @@ struct PromptArgs {
 struct RowTile {
   int b, t0, n, r0;
   int len;                           // of the sequence, as it is given
+  int index;                         // of the tile, in the order of the sequences
 };
 template <int ROWS>
 __device__ __forceinline__ bool find_tile(const PromptArgs& a, int r, int lane, RowTile& x) {
+  x.index = r;
   for (int b0 = 0; b0 <= a.B; b0 += 64) {
     const int b = b0 + lane, bc = min(b, a.B);
     const int c0 = min(max(a.cu[bc], 0), a.T), c1 = b < a.B ? min(max(a.cu[bc + 1], 0), a.T) : a.T;
@@ -90,7 +92,9 @@ __device__ __forceinline__ bool find_tile_by_keys(const PromptArgs& a, int r, in
   x.t0 = __builtin_amdgcn_readlane(c0, l);
   x.n = __builtin_amdgcn_readlane(n, l);
   x.len = __builtin_amdgcn_readlane(len, l);
-  x.r0 = (__builtin_amdgcn_readlane(tiles - over(lo) - (incl - mine), l) + left) * ROWS;
+  const int at = __builtin_amdgcn_readlane(tiles - over(lo) - (incl - mine), l) + left;
+  x.r0 = at * ROWS;
+  x.index = __builtin_amdgcn_readlane((int)wave_prefix_sum((uint32_t)tiles) - tiles, l) + at;
   return true;
 }
 

@@ -393,7 +393,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && D == 128 && TYPE == kBf16Cache 
   l_run = half_sum(l_run);
   if (!placed) l_run = 0.f;                        // a row without a position gets zeros
   if (a.nsplit > 1) {
-    const size_t slot = (((size_t)tile * a.Hk + hk) * a.nsplit + split) * (NW * 32) + w * 32 + l32;
+    const size_t slot = (((size_t)x.index * a.Hk + hk) * a.nsplit + split) * (NW * 32) + w * 32 + l32;
     if (!exists) return;
     float* pa = a.part_acc + slot * D;
 #pragma unroll
@@ -490,11 +490,18 @@ static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int D
   }
   // (Sequences of hardly 256 rows leave most of such a tile empty: 63 single tokens and a chunk of 512,
   // 8K to 16K of context, 962 us and 845; 31 and a chunk of 2048, 4K to 8K, 391 and 370.)
+  const int64_t room = D == 64 ? 2 * cus : cus;    // eight waves of D = 64 are half a CU's
   cut(8);
-  if (p.units < cus || T * G < 512 * B) cut(4);
-  if (p.units >= cus) return p;
-  // parts: enough that two workgroups come to each CU, none of fewer than 8 key tiles
-  const int64_t want = (2 * cus + p.units - 1) / (p.units < 1 ? 1 : p.units), most = slots / (8 * kKeys);
+  if (p.units < room || T * G < 512 * B) cut(4);
+  if (p.units >= room) return p;
+  // Tiles of D = 64 that hardly differ in their keys fill the CUs from 1.4 to each on (4 x 1000 after 2000, 14
+  // heads over 2: 68 us, 84 in two parts); whole prompts leave the CUs to the longest (4000 tokens 86 and
+  // 79; 1000 after 15000, 32 heads over 8: 318 and 184).
+  if (D == 64 && p.units * (2 * B * cap - (T < B * cap ? T : B * cap)) / (2 * B * cap) >= cus * 7 / 5) return p;
+  // parts: as many as the CUs hold at once, by the tiles that there are (half of a sequence's last one),
+  // none of fewer than 8 key tiles
+  const int64_t units = ((T * G + p.rows() - 1) / p.rows() + (B - 1) / 2) * Hk;
+  const int64_t want = 2 * room / units, most = slots / (8 * kKeys);
   const int64_t n = want < most ? want : most;
   p.nsplit = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
   return p;
@@ -575,7 +582,7 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   a.vs = static_cast<const float*>(v_scales), a.vs_sb = vs_sb, a.vs_sh = vs_sh;
   a.part_ml = static_cast<float*>(workspace);
   a.part_acc = a.part_ml + (plan.nwg ? (size_t)plan.nwg * 2 : (size_t)plan.units * plan.nsplit) * plan.rows() * 2;
-  a.by_keys = B > 1 && B < 64 && plan.nsplit == 1;
+  a.by_keys = B > 1 && B < 64;
   a.nwg = plan.nwg, a.span = (int)row_span(32, G);
   a.T = T, a.B = B, a.Hk = Hk, a.G = (int)G, a.D = D;
   a.cap = max_blocks * block_size;
