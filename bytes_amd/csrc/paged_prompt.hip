@@ -21,8 +21,8 @@
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
 //
-// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2080 to 2160
-// us by card, 1020 to 1060 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
+// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2080 to 2250
+// us by card, 980 to 1060 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
 // nothing loaded or stored, 2060; the clock falls to 1.9 GHz and the matrix units are busy for 46% of
 // it.  Left out one at a time, of 2240 then (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
 // 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No
