@@ -39,7 +39,7 @@
 
 namespace bytes_amd {
 
-constexpr int kKeys = 64;            // of a tile
+constexpr int kKeys = kPromptKeys;
 
 // NW waves of 32 rows.
 template <int D, int TYPE, bool HALVES, int NW>
@@ -421,90 +421,16 @@ __global__ __launch_bounds__(64) void paged_prompt_join_kernel(PromptArgs a) {
   constexpr int NSL = D / 64;
   const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
   const int slice = blockIdx.y % NSL, h = blockIdx.y / NSL, t = blockIdx.x;
-  // the sequence of row t and its first row tile
-  int tiles = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = b0 + lane, bc = min(b, a.B - 1);
-    const int c0 = min(max(a.cu[bc], 0), a.T), c1 = min(max(a.cu[bc + 1], 0), a.T);
-    const int n = b < a.B ? max(c1 - c0, 0) : 0;
-    const uint32_t mine = (uint32_t)((n * a.G + ROWS - 1) / ROWS);
-    const uint32_t incl = wave_prefix_sum(mine);
-    const unsigned long long in = __ballot(n > 0 && t >= c0 && t < c0 + n);
-    if (in) {
-      const int l = __ffsll(in) - 1;
-      const int i = t - __builtin_amdgcn_readlane(c0, l), hk = fast_div(h, a.dG);
-      const int row = i * a.G + h - hk * a.G, tile = tiles + __builtin_amdgcn_readlane((int)(incl - mine), l) + row / ROWS;
-      const size_t base = ((size_t)tile * a.Hk + hk) * a.nsplit * ROWS + row % ROWS;
-      auto slot = [&](int u) { return base + (size_t)u * ROWS; };
-      paged_join<4>(a.nsplit, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
-                    reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4,
-                    [&](const f32x4& A, float L) {
-                      if (grp == 0)
-                        paged_store(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
-                    });
-      return;
-    }
-    tiles += __builtin_amdgcn_readlane((int)incl, 63);
-  }
-}
-
-// cap: positions that a table row holds.
-static PromptPlan prompt_plan(int64_t T, int64_t B, int64_t Hk, int64_t G, int D, int64_t cap, int window, int sinks) {
-  const int64_t cus = device_cu_count();
-  PromptPlan p;
-  p.nwg = 0, p.nsplit = 1;
-  int64_t slots;                                   // that a row tile can see
-  // whole row tiles, and one that is not full per sequence (and of the rows past the
-  // last); none without rows
-  auto cut = [&](int waves) {
-    p.waves = waves;
-    const int64_t n = T * G / p.rows() + B + 1, most = T * ((G + p.rows() - 1) / p.rows());
-    p.tiles = n < most ? n : most;
-    p.units = p.tiles * Hk;
-    const int64_t see = (int64_t)window + sinks + row_span(p.rows(), G) + 2 * kKeys;
-    slots = cap < see ? cap : see;
-  };
-  cut(1);
-  // Up to 32 rows of a sequence read its cache once as one tile (eight sequences of 27K to 64K,
-  // 8 KV heads of 128, 24 rows: 248 us, 289 in tiles of 128; 33 rows, two tiles: 472 and 348).
-  // (Rows that are read once stream past the caches: with plain loads 276 and not 248.)
-  // Where contexts are short, and as many tiles of 32 rows as the CUs hold at once, they take
-  // fewer steps one after another (one prompt, 32 heads over 8 of 128, 500 tokens: 18.6 and 21.6 us,
-  // 300 after 1200 32.8 and 38.4, 300 after 2700 57.9 and 44.6; 14 heads over 2 of 64,
-  // 1500 tokens 19.9 and 36.5).
-  const bool lone = T * G <= 32 * B, fits = T * G * Hk / 32 <= cus * (D == 64 ? 4 : 2) && slots <= 2048;
-  if (lone || fits) {
-    // Dealt by the bytes of what a tile sees, which one workgroup reads alone: over 128 KB (one
-    // sequence, 8 heads of 128, 256 tokens: whole units 11.4 us, dealt 12.4; 512 tokens 14.7 and
-    // 12.3), over 512 KB where the units keep half the CUs busy anyway (16 sequences, 1000 tokens:
-    // 22.5 and 24.0; 2000: 38.3 and 36.9), over 2 MB where there are enough for all (60 sequences
-    // of 1200 to 2400 tokens: 81 and 91; 30 of 800 to 8000: 118 and 105).
-    const int64_t granules = p.units * ((slots + 127) / 128), bytes = slots * D * 4;
-    // Several tiles to a sequence: only where the units are few and see over 256 KB (25 tokens after 802, 8
-    // heads of 128: 19.9 and 13.6; 100 after 1900, 14 heads over 2 of 64: 21.9 and 15.2; but 100 after 900
-    // of 8 heads of 64, 256 KB: 14.2 and 16.3; 307 after 975, 28 heads over 4 of 128: 28.8 and 41.7).
-    const bool idle = 2 * p.units < cus;
-    const int64_t alone = lone ? (p.units >= cus ? 2 << 20 : idle ? 128 << 10 : 512 << 10) : 256 << 10;
-    if ((lone || idle) && bytes > alone && granules <= 1 << 24) p.nwg = few_grid(granules);
-    return p;
-  }
-  // (Sequences of hardly 256 rows leave most of such a tile empty: 63 single tokens and a chunk of 512,
-  // 8K to 16K of context, 962 us and 845; 31 and a chunk of 2048, 4K to 8K, 391 and 370.)
-  const int64_t room = D == 64 ? 2 * cus : cus;    // eight waves of D = 64 are half a CU's
-  cut(8);
-  if (p.units < room || T * G < 512 * B) cut(4);
-  if (p.units >= room) return p;
-  // Tiles of D = 64 that hardly differ in their keys fill the CUs from 1.4 to each on (4 x 1000 after 2000, 14
-  // heads over 2: 68 us, 84 in two parts); whole prompts leave the CUs to the longest (4000 tokens 86 and
-  // 79; 1000 after 15000, 32 heads over 8: 318 and 184).
-  if (D == 64 && p.units * (2 * B * cap - (T < B * cap ? T : B * cap)) / (2 * B * cap) >= cus * 7 / 5) return p;
-  // parts: as many as the CUs hold at once, by the tiles that there are (half of a sequence's last one),
-  // none of fewer than 8 key tiles
-  const int64_t units = ((T * G + p.rows() - 1) / p.rows() + (B - 1) / 2) * Hk;
-  const int64_t want = 2 * room / units, most = slots / (8 * kKeys);
-  const int64_t n = want < most ? want : most;
-  p.nsplit = (int)(n < 1 ? 1 : n > 128 ? 128 : n);
-  return p;
+  const int hk = fast_div(h, a.dG);
+  int tile, row;
+  if (!find_row<ROWS>(a, t, h - hk * a.G, lane, tile, row)) return;
+  const size_t base = ((size_t)tile * a.Hk + hk) * a.nsplit * ROWS + row;
+  auto slot = [&](int u) { return base + (size_t)u * ROWS; };
+  paged_join<4>(a.nsplit, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
+                reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4, [&](const f32x4& A, float L) {
+                  if (grp == 0)
+                    paged_store(a.out + (int64_t)t * a.o_st + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
+                });
 }
 
 template <int D, int TYPE, bool HALVES>
@@ -542,7 +468,7 @@ int bytes_paged_prompt_workspace_size(int T, int B, int Hq, int Hk, int D, int b
     *bytes = 0;
     return 0;
   }
-  *bytes = prompt_plan(T, B, Hk, Hq / Hk, D, (int64_t)max_blocks * block_size, window, sinks).workspace(D);
+  *bytes = prompt_plan(device_cu_count(), T, B, Hk, Hq / Hk, D, (int64_t)max_blocks * block_size, window, sinks).workspace(D);
   return 0;
 }
 
@@ -561,7 +487,7 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   if (rc0) return rc0;
   if (T == 0) return 0;
   const int64_t G = Hq / Hk;
-  const PromptPlan plan = prompt_plan(T, B, Hk, G, D, (int64_t)max_blocks * block_size, window, sinks);
+  const PromptPlan plan = prompt_plan(device_cu_count(), T, B, Hk, G, D, (int64_t)max_blocks * block_size, window, sinks);
   PromptArgs a = {};
   a.window = window < (1 << 30) ? window : (1 << 30), a.sinks = sinks < (1 << 30) ? sinks : (1 << 30);
   a.nsplit = plan.nsplit;

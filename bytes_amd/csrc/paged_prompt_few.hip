@@ -429,10 +429,6 @@ static int launch_of(const PromptArgs& a, dim3 grid, hipStream_t st) {
   else hipLaunchKernelGGL((paged_prompt_few_join_kernel<64>), jgrid, dim3(64), 0, st, a);
   return (int)hipGetLastError();
 }
-int few_grid(int64_t granules) {
-  const int64_t n = device_cu_count();
-  return (int)(granules < n ? granules : n);
-}
 int launch_prompt_few(const PromptArgs& a, int kv_type, const PromptPlan& plan, hipStream_t st) {
   const dim3 grid((unsigned)(plan.nwg ? plan.nwg : plan.units));
   switch (kv_type) {
