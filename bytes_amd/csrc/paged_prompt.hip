@@ -77,7 +77,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && D == 128 && TYPE == kBf16Cache 
   }
   // (what all lanes share goes to scalar registers)
   auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  const int p0 = same(x.len - x.n);                // the first new token's position
+  const int p0 = same(first_position(x.len, x.n));
   const int p = p0 + i;
   const bool placed = exists && p >= 0 && p < a.cap;
   const int first = fast_div(x.r0, a.dG), last = min(fast_div(x.r0 + NW * 32 - 1, a.dG), x.n - 1);

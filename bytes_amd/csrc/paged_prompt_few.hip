@@ -166,7 +166,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void paged_prompt_few_kernel(Pro
     int i, h;
     place_of(l32, i, h);
     const bool exists = r0 + l32 < rows;
-    const int p0 = same((int)max((int64_t)x.len - x.n, (int64_t)-x.n)), p = p0 + i;
+    const int p0 = same(first_position(x.len, x.n)), p = p0 + i;
     const bool placed = exists && p >= 0 && p < a.cap;
     const int first = fast_div(r0, a.dG), last = fast_div(min(r0 + 31, rows - 1), a.dG);
     const int p_lo = same(max(p0 + first, 0)), p_hi = same(min(p0 + last, a.cap - 1));

@@ -16,6 +16,9 @@ struct RowTile {
   int len;                           // of the sequence, as it is given
   int index;                         // of the tile, in the order of the sequences
 };
+// The position of the first of the n new tokens of a sequence of `len`; none of them has one where
+// `len` is below 0.
+__device__ __forceinline__ int first_position(int len, int n) { return max(len, 0) - n; }
 template <int ROWS, class ARGS>
 __device__ __forceinline__ bool find_tile(const ARGS& a, int r, int lane, RowTile& x) {
   x.index = r;
@@ -51,7 +54,7 @@ __device__ __forceinline__ bool find_tile_by_keys(const ARGS& a, int r, int lane
   const int b = min(lane, a.B);
   const int c0 = min(max(a.cu[b], 0), a.T), c1 = lane < a.B ? min(max(a.cu[min(b + 1, a.B)], 0), a.T) : a.T;
   const int len = a.c.lens[min(b, a.B - 1)], n = lane <= a.B ? max(c1 - c0, 0) : 0;
-  const int tiles = (n * a.G + ROWS - 1) / ROWS, p0 = lane < a.B ? max(min(len, a.cap) - n, 0) : 0;
+  const int tiles = (n * a.G + ROWS - 1) / ROWS, p0 = lane < a.B ? max(min(max(len, 0), a.cap) - n, 0) : 0;
   auto over = [&](int k) {                                 // this lane's tiles that see more than k keys
     const int y = k - p0;                                  // their last row's token is y or later
     return y <= 0 ? tiles : y >= n ? 0 : tiles - (int)((uint32_t)(y * a.G) / (uint32_t)ROWS);

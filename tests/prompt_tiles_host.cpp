@@ -1,7 +1,7 @@
 // paged_prompt_attn's plan and a wave's search for its row tile, as the kernels run them, on
 // the host.  stdin: calls of cus T B Hk G D cap window sinks, cu[B + 1], lens[B]; stdout for each:
-// waves tiles nsplit nwg, the number of row tiles that were found and those (b t0 n r0 index),
-// then the tile and row of some rows of q (every `step`-th) with head 0 of its group (-1 -1: none).
+// waves tiles nsplit nwg, the number of row tiles that were found and those (b t0 n r0 index, and the
+// first row's position), then the tile and row of some rows of q (every `step`-th) with head 0 of its group (-1 -1: none).
 #include "wave_host.h"
 #include "../bytes_amd/csrc/paged_prompt_tiles.h"
 
@@ -29,7 +29,7 @@ static void tiles_of(const Args& a) {
     if (ok[0]) found.push_back(x[0]);
   }
   printf("%zu\n", found.size());
-  for (const RowTile& x : found) printf("%d %d %d %d %d\n", x.b, x.t0, x.n, x.r0, x.index);
+  for (const RowTile& x : found) printf("%d %d %d %d %d %d\n", x.b, x.t0, x.n, x.r0, x.index, first_position(x.len, x.n));
   const int step = a.T / 24 + 1;
   for (int t = 0; t < a.T; t += step) {
     int tile = -1, row = -1;

@@ -65,3 +65,27 @@ def test_offsets_that_overlap(dev, B, T, Hq, Hk, D):
         print(f"offsets {cu[:B + 1]}", flush=True)
         c.run(lens, cu[:B + 1])
     c.check(lens, [b * T // B for b in range(B + 1)])
+
+
+@pytest.mark.parametrize("B,T,Hq,Hk,D", [(2, 700, 32, 8, 128), (5, 1500, 14, 2, 64), (70, 1000, 8, 1, 128), (3, 20, 8, 2, 64)])
+def test_lengths_below_their_new_tokens(dev, B, T, Hq, Hk, D):
+    """Down to -2^31: zeros, and the other sequences' rows as they are."""
+    c = Call(dev, B, T, Hq, Hk, D, 6000)
+    lens, cu = [5900 - 7 * b for b in range(B)], [b * T // B for b in range(B + 1)]
+    want = c.run(lens, cu).clone()
+    c.check(lens, cu)
+    for low in (-2 ** 31, -2 ** 31 + 1, -2 ** 31 + T // B, -1, 0):
+        some = [low if b % 2 else n for b, n in enumerate(lens)]
+        print(f"lengths {some[:4]}", flush=True)
+        out = c.run(some, cu)
+        for b in range(B):
+            rows = slice(cu[b], cu[b + 1])
+            if b % 2:
+                assert not bool(out[rows].any()), (low, b)
+            elif T > 32 * B // (Hq // Hk):
+                assert torch.equal(out[rows], want[rows]), (low, b)
+            else:
+                # few rows: keys are dealt by all lengths, so sums are cut elsewhere; each result is within 0.005 of the
+                # decode's in norm (test_long_prompt_rows), so they are within twice that of each other
+                diff = float((out[rows].float() - want[rows].float()).norm() / want[rows].float().norm())
+                assert diff < 0.01, (low, b, diff)

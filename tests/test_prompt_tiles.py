@@ -19,7 +19,7 @@ def _some(T):
 @pytest.fixture(scope="module")
 def host(tmp_path_factory):
     """Runs calls (cus, T, B, Hk, G, D, cap, window, sinks, cu, lens): for each (waves, tiles, nsplit, nwg), the row
-    tiles found (b, t0, n, r0, index), and some rows' (tile, row)."""
+    tiles found (b, t0, n, r0, index, first position), and some rows' (tile, row)."""
     cxx = os.environ.get("CXX") or shutil.which("g++") or "/opt/rocm/llvm/bin/clang++"
     exe = str(tmp_path_factory.mktemp("host") / "prompt_tiles")
     # -fwrapv: sums that leave 32 bits wrap, as they do on the GPU; no fortified jumps: the contexts' go from one
@@ -33,7 +33,7 @@ def host(tmp_path_factory):
         assert out.returncode == 0, out
         words = iter(out.stdout.split())
         take = lambda n: tuple(int(next(words)) for _ in range(n))           # noqa: E731
-        return [(take(4), [take(5) for _ in range(take(1)[0])], [take(2) for _ in _some(c[1])]) for c in calls]
+        return [(take(4), [take(6) for _ in range(take(1)[0])], [take(2) for _ in _some(c[1])]) for c in calls]
 
     return run
 
@@ -51,10 +51,12 @@ def _check(call, result, valid):
     T, B, G, cu, lens = call[1], call[2], call[4], call[9], call[10]
     (waves, tiles, nsplit, nwg), found, rows = result
     R = 32 * waves
-    for b, t0, n, r0, index in found:                # inside the rows, inside the workspace
+    for b, t0, n, r0, index, p0 in found:            # inside the rows, inside the workspace
         assert 0 <= b <= B and 0 <= t0 and 0 <= n and t0 + n <= T, (call, b, t0, n)
         assert 0 <= r0 < n * G and r0 % R == 0, (call, b, n, r0)
         assert 0 <= index < tiles, (call, tiles, index)
+        if b < B:                                    # before the sequence where it is none of its positions
+            assert p0 == max(lens[b] - n, -n), (call, b, p0)
     for tile, row in rows:
         assert (tile, row) == (-1, -1) or (0 <= tile < tiles and 0 <= row < R), (call, tiles, tile, row)
     if not valid:
@@ -66,7 +68,7 @@ def _check(call, result, valid):
         want += [(b, c0, c1 - c0, r, first + r // R) for r in range(0, (c1 - c0) * G, R)]
         if b < B:
             at[c0:c1] = [(first + i * G // R, i * G % R) for i in range(c1 - c0)]
-    assert sorted(found) == sorted(want), call
+    assert sorted(x[:5] for x in found) == sorted(want), call
     assert rows == [at[t] for t in _some(T)], call
 
 
@@ -111,3 +113,18 @@ def test_offsets_that_are_no_offsets_stay_inside(host):
         n = [max(0, min(max(y, 0), c[1]) - min(max(x, 0), c[1])) for x, y in zip(c[9], c[9][1:])]
         over += r[0][2] > 1 and sum(-(-x * c[4] // (32 * r[0][0])) for x in n) > r[0][1]
     assert over >= 10                                # more row tiles than the workspace has room for
+
+
+def test_lengths_that_are_no_lengths(host):
+    """Lengths down to -2^31 and up to 2^31 - 1: rows of such a sequence have no position, and the others are taken."""
+    rng = random.Random(3)
+    lowest = -2 ** 31
+    calls = [(256, 700, 2, 8, 4, 128, 6000, NO_WINDOW, 0, [0, 20, 700], [6000, lowest]),
+             (256, 700, 1, 8, 4, 128, 6000, NO_WINDOW, 0, [0, 700], [lowest])]
+    for _ in range(100):
+        s = _shape(rng)
+        cut = sorted(rng.randint(0, s["T"]) for _ in range(s["B"]))
+        lens = [rng.choice([lowest, lowest + 1, lowest + rng.randint(0, s["T"]), -1, 0, 7, 2 ** 31 - 1, s["cap"]]) for _ in range(s["B"])]
+        calls.append((*s.values(), [0] + cut, lens))
+    for c, r in zip(calls, host(calls)):
+        _check(c, r, True)
