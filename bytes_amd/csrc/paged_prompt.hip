@@ -17,7 +17,8 @@
 // product takes its keys in that order, so P goes from one to the other without leaving
 // the lane.  P is rounded to bf16 (nearest even, 2^-8 of a weight at most, as much as the
 // result's own rounding: error against 64 bits 0.0023 of the norm, 0.0017 of it the
-// result's rounding; a second bf16 part would make three products of two); its sum stays in fp32.
+// result's rounding; with a second bf16 part, which makes three products of two, 0.0017 and 16K 3100 us for 2150,
+// a window of 32K 808 for 581, 3K chunks over e4m3 265 for 205); its sum stays in fp32.
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
 //

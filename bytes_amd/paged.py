@@ -387,7 +387,9 @@ def paged_prompt_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     position context_lens[b] - 1.  The token at position p attends over the tokens
     t <= p of its sequence that take part; with a window, over those with
     t > p - window or t < sinks.  Caches, scales and `scale` as in paged_decode_attn.
-    fp32 scores, softmax and sums; weights rounded to bf16 for the value product.
+    fp32 scores, softmax and sums; weights enter the value product rounded to bf16, or, where rows
+    are few (T * H_q / H_k of up to 32 a sequence, as draft tokens give; short prompts), as two bf16
+    numbers (to 2^-16).
     An infinite or NaN value reaches the rows that see its token only; one that takes
     part gives that infinity, unless its weight underflows (NaN then).  (Sequences with a single
     new token may be among them; many of those beside a chunk are faster as a call of
