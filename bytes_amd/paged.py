@@ -6,7 +6,8 @@ the paged product-quantized operators (src/attention_kernels.py:588-622,
 :858-906), with dense rows.  Where k_scale and v_scale are tensors [num_blocks, H_k]
 fp32 (finite, not negative), the cache is float8_e4m3fn or int8 with a scale for each
 block and KV head: the append writes them, the attention operators read them (the
-page-sparse decode takes no such caches).  Any strides are taken as long as rows have unit
+page-sparse decode takes no such caches).  (A tensor of one element is a number, unless
+both are [1, 1] fp32 and the 8-bit cache has one block and head.)  Any strides are taken as long as rows have unit
 stride along D and start on 16-byte boundaries (a [.., block_size, H_k, D]
 storage as well); caches are never copied, other layouts are refused.  Token p of
 sequence b is row p % block_size of block block_table[b, p // block_size].
@@ -50,13 +51,14 @@ def _rows(t: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def _by_block(k_scale: Scale, v_scale: Scale, k_paged: torch.Tensor) -> bool:
-    """Whether the scales are tensors, one for each block and KV head.  A tensor of one element is a
-    number, unless it is [1, 1] and the cache has one block and head."""
-    one = k_paged.dim() == 4 and k_paged.shape[0] * k_paged.shape[1] == 1
-    a, b = (isinstance(s, torch.Tensor) and (s.numel() != 1 or (one and s.dim() == 2)) for s in (k_scale, v_scale))
+    """Whether the scales are tensors, one for each block and KV head.  Tensors of one element are numbers,
+    unless both are [1, 1] fp32 and the cache, of 8 bits, has one block and head."""
+    both = (k_scale, v_scale)
+    a, b = (isinstance(s, torch.Tensor) and s.numel() != 1 for s in both)
     if a != b:
         raise ValueError("k_scale and v_scale are both numbers or both tensors [num_blocks, H_k]")
-    return a
+    return a or (k_paged.dim() == 4 and k_paged.shape[0] * k_paged.shape[1] == 1 and k_paged.element_size() == 1 and
+                 all(isinstance(s, torch.Tensor) and s.dim() == 2 and s.dtype == torch.float32 for s in both))
 
 
 def _tensors(k_scale: Scale, v_scale: Scale, k_paged: torch.Tensor) -> list:
@@ -484,7 +486,7 @@ def paged_quest_decode(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Te
     [B,H_q,1,D] bf16 (and the selected blocks' places in the table, int32
     [B,H_q,min(ceil(kb / block_size), max_blocks)] ascending, if return_pages;
     places past a short sequence's blocks stand for nothing)."""
-    if not (type(k_scale) is float and type(v_scale) is float) and _by_block(k_scale, v_scale, k_paged):
+    if any(isinstance(s, torch.Tensor) and s.numel() != 1 for s in (k_scale, v_scale)):
         raise ValueError("page-sparse decode takes caches with one scale for the tensor")
     if not return_pages:
         out = native().paged_quest(q, k_paged, v_paged, *meta, block_table, context_lens, kb, scaling, local_w, k_scale,

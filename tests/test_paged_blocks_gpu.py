@@ -439,3 +439,22 @@ def test_native_path_and_wrapper_agree(dev, monkeypatch):
                 return (out, c[0].view(raw), c[1].view(raw), c[2], c[3])
             _both(monkeypatch, append, None)
             _both(monkeypatch, append, torch.tensor([0, 1, 2, 3], dtype=I32, device=dev))
+
+
+def test_one_element_scales_on_the_gpu(dev):
+    """A cache of one block and head: two [1, 1] fp32 tensors are its block scales, other tensors of one element numbers."""
+    g = torch.Generator().manual_seed(7)
+    q, cl, bt = (t.to(dev) for t in (_rand(g, 1, 8, 1, 64), torch.tensor([40], dtype=I32), torch.zeros(1, 1, dtype=I32)))
+    kc, vc = ((torch.randn(1, 1, 64, 64, generator=g) * 30).to(F8).to(dev) for _ in "kv")
+    one = torch.ones(1, 1, device=dev)
+    want = PG.paged_decode_attn(q, kc, vc, bt, cl, 0.125, k_scale=0.03, v_scale=0.25)
+    for k, v in ((one * 0.03, 0.25), (0.03, one * 0.25), (one.double() * 0.03, one.double() * 0.25), (one[0] * 0.03, one * 0.25)):
+        got = PG.paged_decode_attn(q, kc, vc, bt, cl, 0.125, k_scale=k, v_scale=v)
+        exact = PG.paged_decode_attn(q, kc, vc, bt, cl, 0.125, k_scale=float(k), v_scale=0.25)
+        assert torch.equal(got, exact)
+        assert torch.equal(PG.paged_prompt_attn(q[:, :, 0], kc, vc, bt, cl, cl.new_tensor([0, 1]), 0.125, k_scale=k, v_scale=v),
+                           PG.paged_prompt_attn(q[:, :, 0], kc, vc, bt, cl, cl.new_tensor([0, 1]), 0.125, k_scale=float(k), v_scale=0.25))
+    by_block = PG.paged_decode_attn(q, kc, vc, bt, cl, 0.125, k_scale=one * 0.03, v_scale=one * 0.25)
+    assert float((by_block.float() - want.float()).norm() / want.float().norm()) < 0.005
+    b = [t.to(BF16) for t in (kc, vc)]               # a bf16 cache's are 1.0
+    assert torch.equal(PG.paged_decode_attn(q, *b, bt, cl, 0.125, k_scale=one, v_scale=one), PG.paged_decode_attn(q, *b, bt, cl, 0.125))

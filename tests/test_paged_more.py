@@ -299,3 +299,33 @@ def test_c_entries_refuse():
     for bad in (dict(B=0), dict(W=0), dict(N=0), dict(T=-1), dict(bs=0), dict(win=-1), dict(sinks=-1), dict(sinks=2),
                 dict(table=None), dict(ws=None), dict(wb=10), dict(seqs=None), dict(W=2 ** 27), dict(T=2 ** 30 + 1)):
         assert resize(**bad), bad
+
+
+def test_one_element_scales_of_a_cache_of_one_block_and_head(calls):
+    """Tensors of one element are numbers, as they are for every other cache, unless both can be nothing but the
+    scales of an 8-bit cache's only block and head."""
+    one = torch.ones(1, 1)
+    x = _inputs(dtype=BF16, Hk=1, N=1, W=1)
+    meta = (torch.zeros(1, 1, 64, dtype=BF16), torch.zeros(1, 1, 64, dtype=BF16))
+    for op in OPS:
+        assert op(x, k_scale=one, v_scale=one).shape[1] == 8                 # (a bf16 cache's: 1.0)
+        with pytest.raises(ValueError, match="no scale"):
+            op(x, k_scale=one * 0.5, v_scale=one)
+    assert {n for n, _ in calls if not n.endswith("_size")} == {"bytes_paged_kv_append", "bytes_paged_decode_attn",
+                                                               "bytes_paged_prompt_attn"}
+    x = _inputs(dtype=F8, Hk=1, N=1, W=1)
+    for k, v in ((one * 0.5, 0.25), (0.5, one * 0.25), (one.double() * 0.5, one.double() * 0.25), (one * 0.5, torch.tensor(0.25)),
+                 (torch.tensor([0.5]), one * 0.25)):
+        calls.clear()
+        _decode(x, k_scale=k, v_scale=v), _append(x, k_scale=k, v_scale=v), _prompt(x, k_scale=k, v_scale=v)
+        made = {n: a for n, a in calls if not n.endswith("_size")}
+        assert made["bytes_paged_decode_attn"][-5:-3] == (0.0625, 0.25)
+        assert made["bytes_paged_kv_append"][-11:-9] == (0.5, 0.25)
+        assert made["bytes_paged_prompt_attn"][11] == 1 and made["bytes_paged_prompt_attn"][-5:-3] == (0.0625, 0.25)
+    calls.clear()                                    # the page-sparse decode knows numbers only
+    PG.paged_quest_decode(x["q"], x["kc"], x["vc"], meta, x["bt"], x["cl"], 16, 0.125, k_scale=one * 0.5, v_scale=one * 0.25)
+    assert calls[-1][0] == "bytes_paged_quest_attn" and calls[-1][1][-5:-3] == (0.0625, 0.25)
+    for dtype in (F8, I8):
+        x = _inputs(dtype=dtype, Hk=1, N=1, W=1)
+        _append(x), _prompt(x), _decode(x)
+        assert calls[-1][0] == "bytes_paged_window_attn" and calls[-1][1][11] == (2 if dtype == F8 else 3)
