@@ -89,3 +89,18 @@ def test_lengths_below_their_new_tokens(dev, B, T, Hq, Hk, D):
                 # decode's in norm (test_long_prompt_rows), so they are within twice that of each other
                 diff = float((out[rows].float() - want[rows].float()).norm() / want[rows].float().norm())
                 assert diff < 0.01, (low, b, diff)
+
+
+@pytest.mark.parametrize("T", [8, 200, 3000])
+def test_a_scale_that_is_no_number(dev, T):
+    """NaN in every row that sees a token, as paged_decode_attn gives; zeros in the others."""
+    g = torch.Generator().manual_seed(T)
+    k, v = (torch.randn(300, 2, 16, 64, generator=g).to(BF16).to(dev) for _ in "kv")
+    q = torch.randn(T + 3, 8, 64, generator=g).to(BF16).to(dev)
+    table = torch.randperm(300, generator=g).to(I32).to(dev).view(1, 300)
+    lens, cu = torch.tensor([T - 2], dtype=I32, device=dev), torch.tensor([0, T], dtype=I32, device=dev)
+    for kw in ({}, dict(window=50, sinks=3)):
+        out = PG.paged_prompt_attn(q, k, v, table, lens, cu, float("nan"), **kw)
+        assert bool(out[2:T].isnan().all()) and not bool(out[:2].any()) and not bool(out[T:].any())
+        one = PG.paged_decode_attn(q[None, T - 1, :, None], k, v, table, lens, float("nan"), **kw)
+        assert bool(one.isnan().all())
