@@ -28,7 +28,7 @@ struct PromptArgs {
   int flip;                          // the scale is negative: queries change sign
   int nwg, span;                     // few rows: workgroups among which keys are dealt, or 0; tokens that 32 rows reach over, at most
   float scale_log2, v_scale;
-  FastDiv dHk, dG, dsplit, dnwg;
+  FastDiv dHk, dG, dnwg;
 };
 
 // The first n of 64 bits.

@@ -518,7 +518,7 @@ int bytes_paged_prompt_attn(const void* q, int64_t q_st, int64_t q_sh, const voi
   // (at least the smallest normal number: times -inf, a masked score, it is -inf)
   a.scale_log2 = fmaxf(fabsf(scale) * kLog2e, 1.17549435e-38f);
   a.v_scale = scale == scale ? v_scale : scale;    // (no number: NaN in every row that sees a token)
-  a.dHk = make_fastdiv((uint32_t)Hk), a.dG = make_fastdiv((uint32_t)G), a.dsplit = make_fastdiv((uint32_t)a.nsplit);
+  a.dHk = make_fastdiv((uint32_t)Hk), a.dG = make_fastdiv((uint32_t)G);
   a.dnwg = make_fastdiv((uint32_t)(a.nwg ? a.nwg : 1));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (plan.waves == 1) return launch_prompt_few(a, kv_type, plan, st);

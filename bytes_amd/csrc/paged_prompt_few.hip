@@ -401,44 +401,44 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void paged_prompt_few_kernel(Pro
         } while (x.tiles == 0);
       }
     }
-    }
   }
+}
 
-  // Joins the parts of each unit that more than one workgroup had: one wave per (row of q, query
-  // head, 64 dims).
-  template <int D>
-  __global__ __launch_bounds__(64) void paged_prompt_few_join_kernel(PromptArgs a) {
-    constexpr int NSL = D / 64;
-    const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
-    const int slice = blockIdx.y % NSL, h = blockIdx.y / NSL, row_q = blockIdx.x;
-    const FewDeal all(a, lane);
-    // the sequence whose rows those are, and its granules' first
-    int b = -1;
-    for (int i = 0; i < all.per && b < 0; ++i) {
-      const int at = lane * all.per + i;
-      const FewSeq x = all.per == 1 ? all.own : few_seq(a, min(at, a.B - 1));
-      if (at < a.B && row_q >= x.t0 && row_q < x.t0 + x.n) b = at;
-    }
-    const unsigned long long in = __ballot(b >= 0);
-    if (!in) return;                                         // a row of no sequence
-    const int l = __ffsll(in) - 1;
-    b = __builtin_amdgcn_readlane(b, l);
-    uint32_t before = all.before_lane(l);
-    for (int i = l * all.per; i < b; ++i) before += all.seq(a, i).work();
-    const FewSeq x = all.seq(a, b);
-    const int hk = fast_div(h, a.dG), row = (row_q - x.t0) * a.G + h - hk * a.G, tile = row / 32;
-    const int64_t s = (int64_t)before * a.Hk + ((int64_t)tile * a.Hk + hk) * x.gran;
-    if (s + x.gran > all.total) return;                      // (offsets that overlap)
-    const int w0 = all.owner(a, (int)s), w1 = all.owner(a, (int)s + x.gran - 1);
-    if (w0 >= w1) return;                                    // finished in place
-    const int slot0 = all.start(a, w0) == (int)s ? 0 : 1;
-    auto slot = [&](int u) { return ((size_t)(w0 + u) * 2 + (u == 0 ? slot0 : 0)) * 32 + (row & 31); };
-    paged_join<4>(w1 - w0 + 1, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
-                  reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4, [&](const f32x4& A, float L) {
-                    if (grp == 0)
-                      paged_store(a.out + (int64_t)row_q * a.o_st + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
-                  });
+// Joins the parts of each unit that more than one workgroup had: one wave per (row of q, query
+// head, 64 dims).
+template <int D>
+__global__ __launch_bounds__(64) void paged_prompt_few_join_kernel(PromptArgs a) {
+  constexpr int NSL = D / 64;
+  const int lane = threadIdx.x, item = lane & 15, grp = lane >> 4;
+  const int slice = blockIdx.y % NSL, h = blockIdx.y / NSL, row_q = blockIdx.x;
+  const FewDeal all(a, lane);
+  // the sequence whose rows those are, and its granules' first
+  int b = -1;
+  for (int i = 0; i < all.per && b < 0; ++i) {
+    const int at = lane * all.per + i;
+    const FewSeq x = all.per == 1 ? all.own : few_seq(a, min(at, a.B - 1));
+    if (at < a.B && row_q >= x.t0 && row_q < x.t0 + x.n) b = at;
   }
+  const unsigned long long in = __ballot(b >= 0);
+  if (!in) return;                                         // a row of no sequence
+  const int l = __ffsll(in) - 1;
+  b = __builtin_amdgcn_readlane(b, l);
+  uint32_t before = all.before_lane(l);
+  for (int i = l * all.per; i < b; ++i) before += all.seq(a, i).work();
+  const FewSeq x = all.seq(a, b);
+  const int hk = fast_div(h, a.dG), row = (row_q - x.t0) * a.G + h - hk * a.G, tile = row / 32;
+  const int64_t s = (int64_t)before * a.Hk + ((int64_t)tile * a.Hk + hk) * x.gran;
+  if (s + x.gran > all.total) return;                      // (offsets that overlap)
+  const int w0 = all.owner(a, (int)s), w1 = all.owner(a, (int)s + x.gran - 1);
+  if (w0 >= w1) return;                                    // finished in place
+  const int slot0 = all.start(a, w0) == (int)s ? 0 : 1;
+  auto slot = [&](int u) { return ((size_t)(w0 + u) * 2 + (u == 0 ? slot0 : 0)) * 32 + (row & 31); };
+  paged_join<4>(w1 - w0 + 1, lane, slot, reinterpret_cast<const float2*>(a.part_ml),
+                reinterpret_cast<const f32x4*>(a.part_acc) + slice * 16 + item, D / 4, [&](const f32x4& A, float L) {
+                  if (grp == 0)
+                    paged_store(a.out + (int64_t)row_q * a.o_st + (int64_t)h * a.o_sh + slice * 64 + item * 4, A, L, a.v_scale);
+                });
+}
 
 template <int D, int TYPE>
 static void launch(const PromptArgs& a, dim3 grid, hipStream_t st) {
