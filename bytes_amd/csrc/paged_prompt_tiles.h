@@ -139,10 +139,12 @@ inline PromptPlan prompt_plan(int64_t cus, int64_t T, int64_t B, int64_t Hk, int
   // 8 KV heads of 128, 24 rows: 248 us, 289 in tiles of 128; 33 rows, two tiles: 472 and 348).
   // (Rows that are read once stream past the caches: with plain loads 276 and not 248.)
   // Where contexts are short, and as many tiles of 32 rows as the CUs hold at once, they take
-  // fewer steps one after another (one prompt, 32 heads over 8 of 128, 500 tokens: 18.6 and 21.6 us,
-  // 300 after 1200 32.8 and 38.4, 300 after 2700 57.9 and 44.6; 14 heads over 2 of 64,
-  // 1500 tokens 19.9 and 36.5).
-  const bool lone = T * G <= 32 * B, fits = T * G * Hk / 32 <= cus * (D == 64 ? 4 : 2) && slots <= 2048;
+  // fewer steps one after another (32 heads over 8 of 128: 500 tokens 19.2 and 19.7 us, 500 after 500 28.5 and 38.5,
+  // 300 after 930 33.9 and 35.8, 300 after 1200 38.1 and 33.8, 300 after 1700 46.5 and 37.1; 28 over 4, 307 after
+  // 975 32.0 and 33.4; 24 over 8, whose units are few, 25 after 1500 16.8 and 21.6, 100 after 1850 29.4 and 29.5;
+  // 14 over 2 of 64: 1500 tokens 22.4 and 31.6, 1000 after 1000 27.5 and 32.6).
+  const bool lone = T * G <= 32 * B, idle = 2 * p.units < cus;
+  const bool fits = T * G * Hk / 32 <= cus * (D == 64 ? 4 : 2) && slots <= (D == 64 || idle ? 2048 : 1280);
   if (lone || fits) {
     // Dealt by the bytes of what a tile sees, which one workgroup reads alone: over 128 KB (one
     // sequence, 8 heads of 128, 256 tokens: whole units 11.4 us, dealt 12.4; 512 tokens 14.7 and
@@ -153,7 +155,6 @@ inline PromptPlan prompt_plan(int64_t cus, int64_t T, int64_t B, int64_t Hk, int
     // Several tiles to a sequence: only where the units are few and see over 256 KB (25 tokens after 802, 8
     // heads of 128: 19.9 and 13.6; 100 after 1900, 14 heads over 2 of 64: 21.9 and 15.2; but 100 after 900
     // of 8 heads of 64, 256 KB: 14.2 and 16.3; 307 after 975, 28 heads over 4 of 128: 28.8 and 41.7).
-    const bool idle = 2 * p.units < cus;
     const int64_t alone = lone ? (p.units >= cus ? 2 << 20 : idle ? 128 << 10 : 512 << 10) : 256 << 10;
     if ((lone || idle) && bytes > alone && granules <= 1 << 24) p.nwg = (int)(granules < cus ? granules : cus);
     return p;
