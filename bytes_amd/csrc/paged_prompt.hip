@@ -22,12 +22,13 @@
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
 //
-// Bound by the matrix units' share of the card's power: a 16K prompt of 32 heads over 8 of 128 takes 2080 to 2250
+// Bound by products and softmax one after the other: a 16K prompt of 32 heads over 8 of 128 takes 2080 to 2250
 // us by card, 980 to 1060 TFLOP/s, where a 16384^3 bf16 product of the library reaches 1400 and products alone,
-// nothing loaded or stored, 2060; the clock falls to 1.9 GHz and the matrix units are busy for 46% of
-// it.  Left out one at a time, of 2240 then (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
-// 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No
-// faster: products of one tile among the softmax of the other in one wave 2330, 64 rows per wave 3840
+// nothing loaded or stored, 2060.  A wave's tile is 32 matrix instructions (1024 clocks) and 207 others (some 1200,
+// an exponential counted as four), and takes 2290 of its SIMD: the two waves there hardly work beside each
+// other.  The matrix units are busy for 45%, LDS is read in 34% and in conflict for 11%, the clock falls to 1.9 GHz.
+// Left out one at a time, of 2240 then (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
+// 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No faster: products of one tile among the softmax of the other in one wave 2330, 64 rows per wave 3840
 // (registers), raised wave priority, dot products for the sums, one tile more on its way.  Over e4m3 with
 // scales 2260 (over e4m3 with one scale 2090): 64 multiplications more per lane and tile; folding the
 // keys' into the exponent's multiply-add takes 3% longer.

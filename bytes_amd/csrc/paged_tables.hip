@@ -22,7 +22,9 @@
 // Bound by latency and launches: nothing here is read or written twice. A step of 32
 // sequences that moves 3 KB takes 5.3 us in one launch (lengths, entries, two rounds of
 // sums, the ring and the outputs follow one another), one of 256 with 34K new tokens 7.6
-// and 3.6 in two.  (Sixteen waves to the plan: 5.8, and 7.5 and 3.6.)
+// and 3.6 in two (states that no cache holds: 10.2 and 5.4).  Without rows that end that plan takes 4.7; rows with more
+// blocks to count than a thread takes alone go to the waves, one after another: 32 of them, as there, 5.5 more, 128 16.5,
+// 256 33.  (Sixteen waves to the plan: 5.8, and 7.5 and 3.6.)
 #include "common.h"
 
 namespace bytes_amd {

@@ -16,8 +16,9 @@
 //
 // Bound by memory: 29 sequences of 6.6K to 16K, 64 heads over 8 of 128, e4m3 with scales
 // (685 MB) take 121 us, 5.7 TB/s (one scale for the tensor 116; without any arithmetic, not an answer,
-// 115), where streaming reads reach 7.1; a window of 4096 and 4 sinks in 16 sequences of 12K to 32K, 8
-// heads of 128 in bf16 (269 MB), 50 us, 5.4 TB/s with its join of 4.6.
+// 115; int8, whose widening takes more instructions, 131), where streaming reads reach 7.1; a window of 4096 and 4 sinks in 16
+// sequences of 12K to 32K, 8 heads of 128 in bf16 (269 MB), 50 us, 5.4 TB/s with its join of 4.6, in 8 bits 36 (one scale),
+// 44 (e4m3) and 48 (int8).
 #include "paged_split.h"
 
 namespace bytes_amd {
@@ -49,7 +50,8 @@ struct PagedWindowArgs : PagedDecodeArgs {
   // A tile of bytes takes as long as one of bf16 and more, read alone (int8, us from a graph, a workgroup per unit
   // and the even split: one sequence of 2 KV heads of 64, 500 tokens 6.7, 750 8.4 and 7.9, 1000 9.8 and 7.8,
   // 2000 16.3 and 7.9; of 4 heads of 128, 300 tokens 7.3 and 8.9, 500 8.8 and 8.9, 1000 13.5 and 8.9; 64
-  // sequences of 2 heads of 64, 1500 tokens 14.4 and 15.3, 2000 17.6 and 17.9).
+  // sequences of 2 heads of 64, 1500 tokens 14.4 and 15.3, 2000 17.6 and 17.9; eagerly, where the host's second launch
+  // counts, 1000 tokens of 2 heads of 64 9.7 and 9.1 to 10.6).
   static constexpr int dim_cost(int type) { return type == kBf16Cache ? 4 : 5; }
 };
 
