@@ -17,8 +17,8 @@
 // product takes its keys in that order, so P goes from one to the other without leaving
 // the lane.  P is rounded to bf16 (nearest even, 2^-8 of a weight at most, as much as the
 // result's own rounding: error against 64 bits 0.0023 of the norm, 0.0017 of it the
-// result's rounding; with a second bf16 part, which makes three products of two, 0.0017 and 16K 3100 us for 2150,
-// a window of 32K 808 for 581, 3K chunks over e4m3 265 for 205); its sum stays in fp32.
+// result's rounding; with a second bf16 part, which makes three products of two, 0.0017, and a 16K prompt takes
+// 3100 us for 2150, a window of 32K 808 for 581, 3K chunks over e4m3 265 for 205); its sum stays in fp32.
 // The running maximum moves only where a score passes it by 2^8, so most tiles leave the
 // accumulators as they are; weights are then up to 2^8, which changes no relative error.
 //
@@ -28,7 +28,8 @@
 // an exponential counted as four), and takes 2290 of its SIMD: the two waves there hardly work beside each
 // other.  The matrix units are busy for 45%, LDS is read in 34% and in conflict for 11%, the clock falls to 1.9 GHz.
 // Left out one at a time, of 2240 then (not answers): loads to LDS 1870 us, exponentials 2080, reads of K
-// 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No faster: products of one tile among the softmax of the other in one wave 2330, 64 rows per wave 3840
+// 1870, of V 2060, the second product 1630, the first 1600; none of reads and loads 1370.  No faster:
+// products of one tile among the softmax of the other in one wave 2330, 64 rows per wave 3840
 // (registers), raised wave priority, dot products for the sums, one tile more on its way.  Over e4m3 with
 // scales 2260 (over e4m3 with one scale 2090): 64 multiplications more per lane and tile; folding the
 // keys' into the exponent's multiply-add takes 3% longer.
