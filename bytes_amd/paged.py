@@ -392,8 +392,9 @@ def paged_prompt_attn(q: torch.Tensor, k_paged: torch.Tensor, v_paged: torch.Ten
     fp32 scores, softmax and sums; weights enter the value product rounded to bf16, or, where rows
     are few (T * H_q / H_k of up to 32 a sequence, as draft tokens give; short prompts), as two bf16
     numbers (to 2^-16).
-    An infinite or NaN value reaches the rows that see its token only; one that takes
-    part gives that infinity, unless its weight underflows (NaN then).  (Sequences with a single
+    An infinite or NaN value reaches the rows that see its token only; an infinity that takes
+    part gives that infinity, unless its weight underflows (below 2^-100 of the row's
+    largest it may give NaN).  (Sequences with a single
     new token may be among them; many of those beside a chunk are faster as a call of
     paged_decode_attn of their own.)  Rows without a
     position, without a token to see, and past cu_seqlens[B] get zeros.  Returns
